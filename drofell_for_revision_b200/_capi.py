@@ -41,12 +41,33 @@ EXPORTED = (
     "w4a16_plan_shape", "w4a16_create_ex", "w4a16_gemm_t", "w4a16_workspace_size_t",
     "w4a16_rms_norm", "w4a16_silu_mul", "w4a16_mlp_forward", "w4a16_mlp_workspace_size", "w4a16_qkv_forward",
     "w4a16_qkv_workspace_size",
+    "w4a16_append_kv", "w4a16_paged_attention", "w4a16_paged_attention_workspace_size", "w4a16_copy_pages",
 )
 CREATE_NO_REPACK = 1
 IPC_HANDLE_BYTES = 72
 
 _lib = None
 _lock = threading.Lock()
+
+
+class Pages(ctypes.Structure):
+    """w4a16_pages: one layer's pages of the key-value cache."""
+    _fields_ = [("k_dev", ctypes.c_void_p), ("v_dev", ctypes.c_void_p), ("stride_page", ctypes.c_int64),
+                ("stride_head", ctypes.c_int64), ("stride_token", ctypes.c_int64), ("num_pages", ctypes.c_int),
+                ("heads_kv", ctypes.c_int), ("page_size", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("dtype", ctypes.c_int), ("device", ctypes.c_int)]
+
+
+class Seqs(ctypes.Structure):
+    """w4a16_seqs: the sequences of a call."""
+    _fields_ = [("tables_dev", ctypes.c_void_p), ("lens_dev", ctypes.c_void_p), ("cu_q_dev", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64), ("table_width", ctypes.c_int), ("batch", ctypes.c_int),
+                ("tokens", ctypes.c_int), ("max_q", ctypes.c_int)]
+
+
+class Rows(ctypes.Structure):
+    """w4a16_rows: rows of [tokens, heads, head_dim]."""
+    _fields_ = [("dev", ctypes.c_void_p), ("stride_token", ctypes.c_int64), ("stride_head", ctypes.c_int64)]
 
 
 class W4A16Error(RuntimeError):
@@ -118,6 +139,15 @@ def lib() -> ctypes.CDLL:
         L.w4a16_plan.restype = I
         L.w4a16_plan_shape.argtypes = [I, I, I, I, I, I, I, I, IP, ctypes.POINTER(S)]
         L.w4a16_plan_shape.restype = I
+        PG, SQ, RW = (ctypes.POINTER(t) for t in (Pages, Seqs, Rows))
+        L.w4a16_append_kv.argtypes = [PG, SQ, RW, RW, RW, RW, I, P, I, I, I, P]
+        L.w4a16_append_kv.restype = I
+        L.w4a16_paged_attention.argtypes = [PG, SQ, RW, RW, I, F, I, I, P, S, P]
+        L.w4a16_paged_attention.restype = I
+        L.w4a16_paged_attention_workspace_size.argtypes = [PG, SQ, I, I, I]
+        L.w4a16_paged_attention_workspace_size.restype = S
+        L.w4a16_copy_pages.argtypes = [P, P, ctypes.c_int64, ctypes.c_int64, I, I, ctypes.c_int64, IP, IP, I, I, P]
+        L.w4a16_copy_pages.restype = I
         L.w4a16_info.argtypes = [P, IP]
         L.w4a16_info.restype = I
         L.w4a16_device_error.argtypes = [P, P, IP]

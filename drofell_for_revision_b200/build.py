@@ -29,6 +29,9 @@ SOURCES = [
     "w4a16_gemv_mma.cu",
     "w4a16_gemm_sm100.cu",
     "w4a16_gemm_ns.cu",
+    "w4a16_paged.cu",
+    "w4a16_attn_split.cu",
+    "w4a16_paged_capi.cu",
 ]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]

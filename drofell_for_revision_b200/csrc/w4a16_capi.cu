@@ -13,7 +13,9 @@
 
 #include "../../include/drofell_w4a16.h"
 #include "w4a16_gather.cuh"
+#include "w4a16_host.h"
 #include "w4a16_internal.h"
+#include "w4a16_paged.h"
 
 using namespace w4a16;
 
@@ -53,32 +55,6 @@ int cuda_fail(cudaError_t e, const char* what) {
 }
 
 bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
-
-// Device whose primary context this thread has made current through cudaSetDevice.
-// A thread that never called it (a worker such as autograd's backward thread) reports
-// device 0 from cudaGetDevice but has no current context yet, and driver entry points
-// (cuTensorMapEncodeTiled) then fail with CUDA_ERROR_INVALID_CONTEXT.
-thread_local int t_bound_device = -1;
-
-// Switches to `dev` for the scope, with its context current, and restores the caller's
-// device afterwards (the reference calls cudaSetDevice and leaves it changed,
-// q4_matmul.cu:248,476).
-struct DeviceGuard {
-    int prev = -1;
-    bool ok = true;
-    explicit DeviceGuard(int dev) {
-        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-        if (prev != dev || t_bound_device != dev) {
-            ok = cudaSetDevice(dev) == cudaSuccess;
-            if (ok) t_bound_device = dev;
-        }
-    }
-    ~DeviceGuard() {
-        int cur = -1;
-        if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev && cudaSetDevice(prev) == cudaSuccess)
-            t_bound_device = prev;
-    }
-};
 
 PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
@@ -234,6 +210,28 @@ CUresult encode_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void*
     cuuint32_t estr[3] = {1, 1, 1};
     return fn(map, dtype, 3, const_cast<void*>(base), d, st, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+CUresult encode_tmap_4d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, const uint64_t dims[4],
+                        const uint64_t strides_bytes[3], const uint32_t box[4], CUtensorMapSwizzle swizzle) {
+    auto fn = get_encode_fn();
+    if (!fn) return CUDA_ERROR_NOT_FOUND;
+    cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
+    cuuint64_t st[3] = {strides_bytes[0], strides_bytes[1], strides_bytes[2]};
+    cuuint32_t b[4] = {box[0], box[1], box[2], box[3]};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    return fn(map, dtype, 4, const_cast<void*>(base), d, st, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+int report_error(int code, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    g_last_error = buf;
+    return code;
 }
 
 }  // namespace w4a16

@@ -143,5 +143,7 @@ CUresult encode_tmap_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void*
                         CUtensorMapSwizzle swizzle);
 CUresult encode_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, const uint64_t dims[3],
                         const uint64_t strides_bytes[2], const uint32_t box[3], CUtensorMapSwizzle swizzle);
+CUresult encode_tmap_4d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, const uint64_t dims[4],
+                        const uint64_t strides_bytes[3], const uint32_t box[4], CUtensorMapSwizzle swizzle);
 
 }  // namespace w4a16

@@ -1,0 +1,273 @@
+// C entry points of the paged key-value cache: argument checks (all before any CUDA call),
+// the choice of the attention kernel, launches.
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <climits>
+#include <cmath>
+#include <exception>
+#include <vector>
+
+#include "../../include/drofell_w4a16.h"
+#include "w4a16_host.h"
+#include "w4a16_paged.h"
+
+using namespace w4a16;
+
+namespace {
+
+int cuda_error(cudaError_t e, const char* what) {
+    return report_error(W4A16_ERR_CUDA, "%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int check_pages(const w4a16_pages* p) {
+    if (!p || !p->k_dev || !p->v_dev) return report_error(W4A16_ERR_INVALID, "null pages");
+    if (p->dtype != W4A16_DTYPE_FP16 && p->dtype != W4A16_DTYPE_BF16)
+        return report_error(W4A16_ERR_INVALID, "unknown dtype %d", p->dtype);
+    if (p->page_size < 8 || p->page_size > 256 || (p->page_size & (p->page_size - 1)))
+        return report_error(W4A16_ERR_UNSUPPORTED, "page size %d (a power of two from 8 to 256)", p->page_size);
+    if (p->head_dim < 8 || p->head_dim > 128 || p->head_dim % 8)
+        return report_error(W4A16_ERR_UNSUPPORTED, "head dim %d (a multiple of 8, at most 128)", p->head_dim);
+    if (p->num_pages <= 0 || p->heads_kv <= 0)
+        return report_error(W4A16_ERR_INVALID, "num_pages=%d heads_kv=%d", p->num_pages, p->heads_kv);
+    if (p->stride_page < 0 || p->stride_head < 0 || p->stride_token < 0 || p->stride_page % 8 || p->stride_head % 8 ||
+        p->stride_token % 8)
+        return report_error(W4A16_ERR_INVALID, "page strides must be non-negative multiples of 8 elements");
+    if (!aligned16(p->k_dev) || !aligned16(p->v_dev))
+        return report_error(W4A16_ERR_INVALID, "the pages must be 16-byte aligned");
+    return W4A16_OK;
+}
+
+int check_seqs(const w4a16_pages* p, const w4a16_seqs* s) {
+    if (!s) return report_error(W4A16_ERR_INVALID, "null seqs");
+    if (s->batch < 0 || s->tokens < 0 || s->max_q < 0 || s->table_width < 0 || s->table_stride < 0)
+        return report_error(W4A16_ERR_INVALID, "batch=%d tokens=%d max_q=%d table_width=%d: none may be negative",
+                            s->batch, s->tokens, s->max_q, s->table_width);
+    if (s->batch > 0 && (!s->lens_dev || (s->table_width > 0 && !s->tables_dev)))
+        return report_error(W4A16_ERR_INVALID, "null tables or lens");
+    if (!s->cu_q_dev && s->tokens != s->batch)
+        return report_error(W4A16_ERR_INVALID, "%d rows for %d sequences of one new token each", s->tokens, s->batch);
+    if (static_cast<int64_t>(s->table_width) * p->page_size > INT_MAX - 1024)
+        return report_error(W4A16_ERR_UNSUPPORTED, "tables of %d pages of %d tokens", s->table_width, p->page_size);
+    return W4A16_OK;
+}
+
+int check_rows(const w4a16_rows* r, const char* name) {
+    if (!r || !r->dev) return report_error(W4A16_ERR_INVALID, "null %s", name);
+    if (r->stride_token < 0 || r->stride_head < 0 || r->stride_token % 8 || r->stride_head % 8 || !aligned16(r->dev))
+        return report_error(W4A16_ERR_INVALID, "%s must be 16-byte aligned, its strides non-negative multiples of 8 elements",
+                            name);
+    return W4A16_OK;
+}
+
+PageView page_view(const w4a16_pages* p) {
+    PageView v;
+    v.k = static_cast<const uint16_t*>(p->k_dev);
+    v.v = static_cast<const uint16_t*>(p->v_dev);
+    v.stride_page = p->stride_page;
+    v.stride_head = p->stride_head;
+    v.stride_token = p->stride_token;
+    v.num_pages = p->num_pages;
+    v.heads_kv = p->heads_kv;
+    v.dim = p->head_dim;
+    v.page_shift = 0;
+    while ((1 << v.page_shift) < p->page_size) ++v.page_shift;
+    return v;
+}
+
+SeqView seq_view(const w4a16_seqs* s) {
+    SeqView v;
+    v.tables = s->tables_dev;
+    v.lens = s->lens_dev;
+    v.cu_q = s->cu_q_dev;
+    v.table_stride = s->table_stride;
+    v.width = s->table_width;
+    v.batch = s->batch;
+    v.tokens = s->tokens;
+    v.max_q = s->max_q;
+    return v;
+}
+
+int sm_count(int device) {
+    static std::atomic<int> known[64];
+    if (device >= 0 && device < 64) {
+        const int n = known[device].load(std::memory_order_relaxed);
+        if (n > 0) return n;
+    }
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) return 0;
+    if (device >= 0 && device < 64) known[device].store(n, std::memory_order_relaxed);
+    return n;
+}
+
+AttnArgs attn_args(const w4a16_pages* pages, const w4a16_seqs* seqs, int heads, int window, int sinks) {
+    AttnArgs a = {};
+    a.pages = page_view(pages);
+    a.seqs = seq_view(seqs);
+    a.seqs.max_q = seqs->cu_q_dev ? seqs->max_q : 1;
+    a.heads = heads;
+    a.group = heads / pages->heads_kv;
+    a.window = window;
+    a.sinks = sinks;
+    return a;
+}
+
+int check_attention(const w4a16_pages* pages, const w4a16_seqs* seqs, int heads, int window, int sinks) {
+    int rc = check_pages(pages);
+    if (rc == W4A16_OK) rc = check_seqs(pages, seqs);
+    if (rc != W4A16_OK) return rc;
+    if (heads <= 0 || heads % pages->heads_kv)
+        return report_error(W4A16_ERR_INVALID, "%d query heads on %d key-value heads", heads, pages->heads_kv);
+    if (window < 0 || sinks < 0) return report_error(W4A16_ERR_INVALID, "window=%d sinks=%d", window, sinks);
+    if (sinks > 0 && window == 0) return report_error(W4A16_ERR_INVALID, "sinks without a window");
+    if (static_cast<int64_t>(seqs->max_q) * (heads / pages->heads_kv) > INT_MAX / 2)
+        return report_error(W4A16_ERR_UNSUPPORTED, "max_q=%d", seqs->max_q);
+    return W4A16_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int w4a16_append_kv(const w4a16_pages* pages, const w4a16_seqs* seqs, const w4a16_rows* k, const w4a16_rows* v,
+                    const w4a16_rows* q, const w4a16_rows* q_out, int heads, const float* rope_dev, int rope_positions,
+                    int rope_dim, int interleaved, void* stream) {
+    int rc = check_pages(pages);
+    if (rc == W4A16_OK) rc = check_seqs(pages, seqs);
+    if (rc != W4A16_OK) return rc;
+    if (seqs->batch == 0 || seqs->tokens == 0) return W4A16_OK;
+    rc = check_rows(k, "k");
+    if (rc == W4A16_OK) rc = check_rows(v, "v");
+    const bool with_q = q && q->dev;
+    if (rc == W4A16_OK && with_q) {
+        rc = check_rows(q, "q");
+        if (rc == W4A16_OK) rc = check_rows(q_out, "q_out");
+        if (rc == W4A16_OK && heads <= 0) rc = report_error(W4A16_ERR_INVALID, "heads=%d", heads);
+    }
+    if (rc != W4A16_OK) return rc;
+    if (rope_dev) {
+        if (rope_dim <= 0 || rope_dim > pages->head_dim || rope_dim % (interleaved ? 8 : 16))
+            return report_error(W4A16_ERR_UNSUPPORTED, "rope dim %d of %d (a multiple of %d)", rope_dim,
+                                pages->head_dim, interleaved ? 8 : 16);
+        if (!aligned16(rope_dev)) return report_error(W4A16_ERR_INVALID, "the rope table must be 16-byte aligned");
+        if (rope_positions < static_cast<int64_t>(seqs->table_width) * pages->page_size)
+            return report_error(W4A16_ERR_INVALID, "a rope table of %d positions for tables of %lld tokens", rope_positions,
+                                static_cast<long long>(seqs->table_width) * pages->page_size);
+    }
+    AppendArgs a = {};
+    a.pages = page_view(pages);
+    a.seqs = seq_view(seqs);
+    a.k_out = static_cast<uint16_t*>(pages->k_dev);
+    a.v_out = static_cast<uint16_t*>(pages->v_dev);
+    a.k = static_cast<const uint16_t*>(k->dev);
+    a.v = static_cast<const uint16_t*>(v->dev);
+    a.k_token = k->stride_token, a.k_head = k->stride_head;
+    a.v_token = v->stride_token, a.v_head = v->stride_head;
+    if (with_q) {
+        a.q = static_cast<const uint16_t*>(q->dev);
+        a.q_out = static_cast<uint16_t*>(q_out->dev);
+        a.q_token = q->stride_token, a.q_head = q->stride_head;
+        a.qo_token = q_out->stride_token, a.qo_head = q_out->stride_head;
+        a.heads = heads;
+    }
+    a.rope = rope_dev;
+    a.rope_dim = rope_dim;
+    a.interleaved = interleaved ? 1 : 0;
+    // every new token is stored, whatever max_q says
+    a.seqs.max_q = INT_MAX;
+    DeviceGuard guard(pages->device);
+    if (!guard.ok) return report_error(W4A16_ERR_INVALID, "device %d", pages->device);
+    const cudaError_t e = launch_append(a, pages->dtype == W4A16_DTYPE_BF16, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? W4A16_OK : cuda_error(e, "append_kv launch");
+}
+
+size_t w4a16_paged_attention_workspace_size(const w4a16_pages* pages, const w4a16_seqs* seqs, int heads, int window,
+                                            int sinks) {
+    if (check_attention(pages, seqs, heads, window, sinks) != W4A16_OK) return 0;
+    if (seqs->batch == 0 || seqs->tokens == 0 || seqs->max_q == 0) return 0;
+    const int sms = sm_count(pages->device);
+    if (sms == 0) return 0;
+    return split_workspace_bytes(plan_split(attn_args(pages, seqs, heads, window, sinks), sms), pages->head_dim);
+}
+
+int w4a16_paged_attention(const w4a16_pages* pages, const w4a16_seqs* seqs, const w4a16_rows* q, const w4a16_rows* out,
+                          int heads, float scale, int window, int sinks, void* workspace_dev, size_t workspace_bytes,
+                          void* stream) {
+    int rc = check_attention(pages, seqs, heads, window, sinks);
+    if (rc != W4A16_OK) return rc;
+    if (!std::isfinite(scale)) return report_error(W4A16_ERR_INVALID, "scale is not finite");
+    if (seqs->batch == 0 || seqs->tokens == 0 || seqs->max_q == 0) return W4A16_OK;
+    rc = check_rows(q, "q");
+    if (rc == W4A16_OK) rc = check_rows(out, "out");
+    if (rc != W4A16_OK) return rc;
+    AttnArgs a = attn_args(pages, seqs, heads, window, sinks);
+    a.q = static_cast<const uint16_t*>(q->dev);
+    a.q_token = q->stride_token, a.q_head = q->stride_head;
+    a.out = static_cast<uint16_t*>(out->dev);
+    a.o_token = out->stride_token, a.o_head = out->stride_head;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    const int sms = sm_count(pages->device);
+    if (sms == 0) return report_error(W4A16_ERR_CUDA, "no device %d", pages->device);
+    DeviceGuard guard(pages->device);
+    if (!guard.ok) return report_error(W4A16_ERR_INVALID, "device %d", pages->device);
+    const bool bf16 = pages->dtype == W4A16_DTYPE_BF16;
+    const SplitPlan p = plan_split(a, sms);
+    const size_t need = split_workspace_bytes(p, pages->head_dim);
+    if (workspace_bytes < need || (need > 0 && !workspace_dev))
+        return report_error(W4A16_ERR_WORKSPACE, "workspace %zu bytes < %zu needed", workspace_bytes, need);
+    if (need > 0 && !aligned16(workspace_dev)) return report_error(W4A16_ERR_INVALID, "the workspace must be 16-byte aligned");
+    a.ws = need > 0 ? static_cast<float*>(workspace_dev) : nullptr;
+    const cudaError_t e = launch_split(a, p, bf16, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? W4A16_OK : cuda_error(e, "paged attention launch");
+}
+
+int w4a16_copy_pages(void* k_dev, void* v_dev, int64_t stride_layer_bytes, int64_t stride_page_bytes, int layers,
+                     int num_pages, int64_t page_bytes, const int32_t* src_host, const int32_t* dst_host, int pairs,
+                     int device, void* stream) try {
+    if (!k_dev || !v_dev) return report_error(W4A16_ERR_INVALID, "null pages");
+    if (pairs < 0 || num_pages <= 0 || layers < 0 || layers > 32767 || page_bytes <= 0)
+        return report_error(W4A16_ERR_INVALID, "pairs=%d num_pages=%d layers=%d page_bytes=%lld", pairs, num_pages, layers,
+                            static_cast<long long>(page_bytes));
+    if (page_bytes % 16 || stride_page_bytes % 16 || stride_layer_bytes % 16 || !aligned16(k_dev) || !aligned16(v_dev))
+        return report_error(W4A16_ERR_INVALID, "pages and their strides must be multiples of 16 bytes");
+    if (stride_page_bytes < page_bytes || stride_layer_bytes < 0)
+        return report_error(W4A16_ERR_INVALID, "pages that overlap");
+    if (pairs == 0 || layers == 0) return W4A16_OK;
+    if (!src_host || !dst_host) return report_error(W4A16_ERR_INVALID, "null page ids");
+    std::vector<uint8_t> seen(num_pages, 0);  // 1 written, 2 read
+    for (int i = 0; i < pairs; ++i) {
+        const int s = src_host[i], d = dst_host[i];
+        if (s < 0 || s >= num_pages || d < 0 || d >= num_pages)
+            return report_error(W4A16_ERR_INVALID, "copy %d of page %d to %d: %d pages", i, s, d, num_pages);
+        if (seen[d] || s == d || (seen[s] & 1))
+            return report_error(W4A16_ERR_INVALID, "copy %d of page %d to %d: a page written twice, or read and written", i,
+                                s, d);
+        seen[d] = 1;
+        seen[s] |= 2;
+    }
+    DeviceGuard guard(device);
+    if (!guard.ok) return report_error(W4A16_ERR_INVALID, "device %d", device);
+    CopyArgs a = {};
+    a.base[0] = static_cast<uint8_t*>(k_dev);
+    a.base[1] = static_cast<uint8_t*>(v_dev);
+    a.stride_layer = stride_layer_bytes;
+    a.stride_page = stride_page_bytes;
+    a.page_bytes = page_bytes;
+    a.layers = layers;
+    for (int i = 0; i < pairs; i += kCopyPairs) {
+        a.pairs = pairs - i < kCopyPairs ? pairs - i : kCopyPairs;
+        for (int j = 0; j < a.pairs; ++j) {
+            a.src[j] = src_host[i + j];
+            a.dst[j] = dst_host[i + j];
+        }
+        const cudaError_t e = launch_copy(a, static_cast<cudaStream_t>(stream));
+        if (e != cudaSuccess) return cuda_error(e, "copy_pages launch");
+    }
+    return W4A16_OK;
+} catch (const std::exception& e) {
+    return report_error(W4A16_ERR_INVALID, "copy_pages: %s", e.what());
+}
+
+}  // extern "C"

@@ -230,6 +230,80 @@ W4A16_API int w4a16_ipc_close(void* ptr);
 W4A16_API int w4a16_gemm_gather(w4a16_matrix* h, w4a16_comm* c, const void* x_dev, int M, void* const* y_all, int ld,
                       int col0, int dtype, void* workspace_dev, size_t workspace_bytes, void* stream);
 
+/* ---- Paged key-value cache (fp16 / bf16) --------------------------------------------
+ * What lies between w4a16_qkv_forward and the output projection: rotating q and k and
+ * storing k and v into pages, attention over the pages, copying pages. No counterpart on
+ * the reference's W4A16 path (it calls its vLLM fork there, cuda_extends/vllm_cache.py and
+ * vllm_attention.py). Serving only: no gradients.
+ *
+ * One layer's pages: element (page, head, slot, d) of K and of V lies at page *
+ * stride_page + head * stride_head + slot * stride_token + d (in elements; K and V have
+ * the same strides, multiples of 8; bases 16-byte aligned). page_size is a power of two
+ * from 8 to 256; head_dim is a multiple of 8, at most 128. */
+typedef struct w4a16_pages {
+    void* k_dev;
+    void* v_dev;
+    int64_t stride_page, stride_head, stride_token;
+    int num_pages, heads_kv, page_size, head_dim;
+    int dtype;  /* W4A16_DTYPE_* of the pages, q, k, v and the outputs */
+    int device;
+} w4a16_pages;
+
+/* The sequences of a call. Sequence b has lens_dev[b] tokens, the new ones counted; token
+ * t of it lies in page tables_dev[b * table_stride + t / page_size]. Its new tokens are
+ * rows cu_q_dev[b] .. cu_q_dev[b + 1] - 1 of q (cu_q_dev NULL: one new token each, row b),
+ * at positions lens[b] - n .. lens[b] - 1. `tokens` rows exist; rows of no sequence are
+ * left as they were. max_q bounds the new tokens of a sequence (rows beyond it get no
+ * attention). All on the device: nothing is read on the host, so calls can be captured in
+ * a graph and replayed with other lengths and tables. Device values are never trusted:
+ * a length past the table counts as the table's, a token whose page id is not a page is
+ * neither stored nor seen, row ranges are held to `tokens`. */
+typedef struct w4a16_seqs {
+    const int32_t* tables_dev;
+    const int32_t* lens_dev;
+    const int32_t* cu_q_dev;
+    int64_t table_stride;
+    int table_width, batch, tokens, max_q;
+} w4a16_seqs;
+
+/* Rows of [tokens, heads, head_dim]: strides in elements, multiples of 8. */
+typedef struct w4a16_rows {
+    void* dev;
+    int64_t stride_token, stride_head;
+} w4a16_rows;
+
+/* Store the new tokens' k and v into their pages, k rotated, and write q rotated to q_out
+ * (may be q; q with dev NULL: k and v only). rope_dev: fp32 [rope_positions, rope_dim], a
+ * row's cosines then its sines (NULL: no rotation); rope_positions must reach the table's
+ * width * page_size. Dimensions i and i + rope_dim / 2 rotate together, with interleaved
+ * 2 i and 2 i + 1; those past rope_dim pass through. rope_dim is a multiple of 16 (8 when
+ * interleaved). fp32 arithmetic, rounded once. Pages that two sequences share must not be
+ * written to. Tokens of a negative position (more new tokens than the length) are not
+ * stored, their q passes unrotated. */
+W4A16_API int w4a16_append_kv(const w4a16_pages* pages, const w4a16_seqs* seqs, const w4a16_rows* k,
+                              const w4a16_rows* v, const w4a16_rows* q, const w4a16_rows* q_out, int heads,
+                              const float* rope_dev, int rope_positions, int rope_dim, int interleaved, void* stream);
+
+/* out = softmax(scale q k^T) v of every new token over the visible tokens of its sequence:
+ * not after it, and with window > 0 the last `window` ones (itself counted) and the first
+ * `sinks` ones. heads is a multiple of heads_kv; query head i reads key-value head
+ * i / (heads / heads_kv). Rows that see nothing are 0. Softmax statistics and sums in
+ * fp32. No host synchronisation and no allocation: capturable. Calls that may overlap on
+ * the GPU need workspaces of their own. */
+W4A16_API int w4a16_paged_attention(const w4a16_pages* pages, const w4a16_seqs* seqs, const w4a16_rows* q,
+                                    const w4a16_rows* out, int heads, float scale, int window, int sinks,
+                                    void* workspace_dev, size_t workspace_bytes, void* stream);
+W4A16_API size_t w4a16_paged_attention_workspace_size(const w4a16_pages* pages, const w4a16_seqs* seqs, int heads,
+                                                      int window, int sinks);
+
+/* Copy whole pages, of every layer and of K and V: page dst_host[i] gets page src_host[i].
+ * A page is page_bytes contiguous bytes at layer * stride_layer_bytes + id *
+ * stride_page_bytes (all multiples of 16). The ids are read on the host during the call. No
+ * page may be written twice, or both read and written. */
+W4A16_API int w4a16_copy_pages(void* k_dev, void* v_dev, int64_t stride_layer_bytes, int64_t stride_page_bytes,
+                               int layers, int num_pages, int64_t page_bytes, const int32_t* src_host,
+                               const int32_t* dst_host, int pairs, int device, void* stream);
+
 /* Message of the last failure on this thread ("" if none). */
 W4A16_API const char* w4a16_last_error(void);
 
