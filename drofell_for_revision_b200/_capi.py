@@ -42,6 +42,7 @@ EXPORTED = (
     "w4a16_rms_norm", "w4a16_silu_mul", "w4a16_mlp_forward", "w4a16_mlp_workspace_size", "w4a16_qkv_forward",
     "w4a16_qkv_workspace_size",
     "w4a16_append_kv", "w4a16_paged_attention", "w4a16_paged_attention_workspace_size", "w4a16_copy_pages",
+    "w4a16_paged_error",
 )
 CREATE_NO_REPACK = 1
 IPC_HANDLE_BYTES = 72
@@ -146,6 +147,8 @@ def lib() -> ctypes.CDLL:
         L.w4a16_paged_attention.restype = I
         L.w4a16_paged_attention_workspace_size.argtypes = [PG, SQ, I, I, I]
         L.w4a16_paged_attention_workspace_size.restype = S
+        L.w4a16_paged_error.argtypes = [I, P, IP]
+        L.w4a16_paged_error.restype = I
         L.w4a16_copy_pages.argtypes = [P, P, ctypes.c_int64, ctypes.c_int64, I, I, ctypes.c_int64, IP, IP, I, I, P]
         L.w4a16_copy_pages.restype = I
         L.w4a16_info.argtypes = [P, IP]

@@ -31,6 +31,7 @@ SOURCES = [
     "w4a16_gemm_ns.cu",
     "w4a16_paged.cu",
     "w4a16_attn_split.cu",
+    "w4a16_attn_sm100.cu",
     "w4a16_paged_capi.cu",
 ]
 

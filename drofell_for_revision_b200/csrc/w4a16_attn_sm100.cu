@@ -1,0 +1,540 @@
+// Attention of prompts and chunks over a paged cache on the sm_100a tensor cores, causal,
+// with an optional sliding window and sinks.
+//
+// One CTA takes 256 query rows of one sequence and key-value head, as two tiles of 128: a
+// row is (token, query head of the group), token-major, so that all heads that share keys
+// share their loads. Over tiles of 128 keys, with the running maximum m and sum l of the
+// softmax (fp32, base 2):
+//   S = Q K^T (tcgen05, fp32 in TMEM), P = 2^(scale S - m) rounded to 16 bits, O += P V.
+// P replaces S in TMEM and is the A operand of the second product, read from there; V, whose
+// rows are keys, is an MN-major B operand. O stays in TMEM; it is rescaled only when a row's
+// maximum grew by more than 2^8 (P up to 256 keeps every bit; l and O share the factor), so
+// that the usual tile costs no round trip of O.
+//
+// Rounding P to the 16-bit type (at most half a step each) is what lets the second product
+// run on the tensor cores at their 16-bit rate; l sums the unrounded fp32 values.
+//
+// Warp roles (320 threads): warps 0-3 and 4-7 softmax and epilogue of the two row tiles,
+// one row a thread; warp 8 loads K and V page by page (TMA, lane = page; a page id that is
+// no page reads zeros behind the cache's end); warp 9 issues the MMAs: while one row tile
+// is in its softmax, the tensor cores work for the other.
+#include <algorithm>
+#include <atomic>
+#include <cuda.h>
+
+#include "w4a16_internal.h"
+#include "w4a16_paged.cuh"
+#include "w4a16_ptx.cuh"
+
+namespace w4a16 {
+namespace {
+
+constexpr int kTileKeys = 128;
+constexpr int kTileRows = 128;
+constexpr int kThreads = 10 * 32;
+constexpr int kLoadWarp = 8, kMmaWarp = 9;
+constexpr int kBlock = 128 * 128;  // bytes of a [128 rows x 64] operand block, 128-byte swizzle
+constexpr uint32_t kWaitLimit = 1u << 18;  // x ~10 us sleeps: a few seconds
+constexpr float kSlack = 8.f;              // log2 of the growth that O tolerates without rescaling
+
+enum : int { kErrLoad = 1, kErrMma = 2, kErrSoftmax = 3, kErrEnd = 4 };
+__device__ int g_attention_error;
+
+template <int DP>
+struct Cfg {
+    static constexpr int kBlocks = DP / 64;
+    static constexpr int kTileBytes = kBlocks * kBlock;  // 128 rows of Q, K or V
+    static constexpr int kSlots = DP == 128 ? 5 : 8;     // K and V tiles in turn
+    static constexpr int kKvOff = 2 * kTileBytes;
+    static constexpr int kBarOff = kKvOff + kSlots * kTileBytes;
+    static constexpr int kSmem = kBarOff + 256 + 1024;  // barriers; alignment
+    static_assert(kSmem <= 227 * 1024, "shared memory budget");
+    // TMEM columns: S of both row tiles (P in their first 64), O of both
+    static constexpr int kS = 0, kO = 256;
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
+                                            int c3) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+        "[%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(ptx::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "
+        "%24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, "
+        "%25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Bounded wait of a whole warp: the same answer in every lane.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
+    return __all_sync(0xffffffffu, ptx::mbar_wait_sleep_bounded(bar, parity, kWaitLimit, err, code));
+}
+
+// One row, key by key, each key by selection: for rows whose sums are not finite because a
+// product took in a value that the row does not see (0 x inf, 0 x NaN). A warp a row, lanes
+// over the head's dimensions.
+template <bool BF16>
+__device__ __noinline__ void careful_row(const AttnArgs& a, int b, int h, int64_t q_off, int64_t o_off, int p) {
+    const int lane = threadIdx.x & 31;
+    float q[4] = {}, o[4] = {}, m = -INFINITY, l = 0.f;
+    const int d = lane * 4;
+    const bool in = d < a.pages.dim;
+    auto load4 = [&](const uint16_t* src, float (&x)[4]) {
+        x[0] = x[1] = x[2] = x[3] = 0.f;
+        if (!in) return;
+        const uint2 r = *reinterpret_cast<const uint2*>(src + d);
+        const float2 u = unpack2<BF16>(r.x), v = unpack2<BF16>(r.y);
+        x[0] = u.x, x[1] = u.y, x[2] = v.x, x[3] = v.y;
+    };
+    load4(a.q + q_off, q);
+    const int32_t* table = a.seqs.tables + b * a.seqs.table_stride;
+    const int lo = a.window ? max(0, p + 1 - a.window) : 0;
+    for (int j = 0; j <= p; ++j) {
+        if (j >= a.sinks && j < lo) j = lo;
+        const int page = table[j >> a.pages.page_shift];
+        if (page < 0 || page >= a.pages.num_pages) continue;
+        const int64_t at = page * a.pages.stride_page + h * a.pages.stride_head +
+                           (j & ((1 << a.pages.page_shift) - 1)) * a.pages.stride_token;
+        float k[4], v[4];
+        load4(a.pages.k + at, k);
+        load4(a.pages.v + at, v);
+        float s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
+#pragma unroll
+        for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+        s *= a.scale_log2;
+        const float m2 = fmaxf(m, s), base = m2 == -INFINITY ? 0.f : m2;
+        const float f = m == m2 ? 1.f : exp2_approx(m - base), w = exp2_approx(s - base);
+        m = m2;
+        l = l * f + w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = (f == 0.f ? 0.f : o[e] * f) + w * v[e];
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (in)
+        *reinterpret_cast<uint2*>(a.out + o_off + d) =
+            make_uint2(pack2<BF16>(o[0] * inv, o[1] * inv), pack2<BF16>(o[2] * inv, o[3] * inv));
+}
+
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                  const __grid_constant__ AttnArgs a) {
+    using C = Cfg<DP>;
+    constexpr int CH = DP / 8;
+    constexpr int SL = C::kSlots;
+    extern __shared__ __align__(1024) uint8_t smem_dyn[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
+    uint64_t* empty = full + SL;
+    uint64_t* qfull = empty + SL;
+    uint64_t* sfull = qfull + 1;  // [2] S of a row tile is complete (and all products before it)
+    uint64_t* pfull = sfull + 2;  // [2] P is written, O rescaled
+    uint64_t* ofull = pfull + 2;  // all products are complete
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ofull + 1);
+
+    ptx::grid_dep_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int h = blockIdx.x, b = blockIdx.z;
+    const int pair = gridDim.y - 1 - blockIdx.y;  // the rows that see most keys first
+    const Seq sq = load_seq(a.seqs, a.pages.page_shift, b);
+    const int rows = sq.nq * a.group;
+    const int row0 = pair * 2 * kTileRows;
+    if (row0 >= rows) return;
+    const int row_end = min(rows, row0 + 2 * kTileRows);
+    // positions of each row tile's first and last row
+    int p_lo[2], p_hi[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int r0 = row0 + t * kTileRows, r1 = min(rows, r0 + kTileRows) - 1;
+        p_lo[t] = sq.p0 + r0 / a.group;
+        p_hi[t] = r0 < rows ? sq.p0 + r1 / a.group : -1;  // -1: no rows
+    }
+    const int last = sq.p0 + (row_end - 1) / a.group;
+    const KeyTiles<kTileKeys> kt(p_lo[0], last, a.window, a.sinks);
+    const int n = kt.count;
+    const int first_seen = a.window ? max(0, max(p_lo[0], 0) + 1 - a.window) : 0;  // of the window, any row
+    // whether any row of row tile t sees any key of the 128 from k0
+    auto active = [&](int t, int k0) {
+        return k0 <= p_hi[t] && (a.window == 0 || k0 + kTileKeys - 1 > max(p_lo[t], 0) - a.window || k0 < a.sinks);
+    };
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < SL; ++s) {
+            ptx::mbar_init(&full[s], 1);
+            ptx::mbar_init(&empty[s], 1);
+        }
+        ptx::mbar_init(qfull, 8);
+        for (int t = 0; t < 2; ++t) {
+            ptx::mbar_init(&sfull[t], 1);
+            ptx::mbar_init(&pfull[t], 4);
+        }
+        ptx::mbar_init(ofull, 1);
+        ptx::fence_mbar_init();
+        ptx::prefetch_tmap(&tm_k);
+        ptx::prefetch_tmap(&tm_v);
+    }
+    if (warp == kMmaWarp) {
+        ptx::tmem_alloc(tmem_slot, 512);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    int* err = &g_attention_error;
+
+    if (warp == kLoadWarp) {
+        // ------------------------------------------------ K and V, page by page
+        const int page_size = 1 << a.pages.page_shift;
+        const int box = min(page_size, kTileKeys);
+        const int boxes = kTileKeys / box;  // per tile, at most 16: one a lane
+        const int32_t* table = a.seqs.tables + b * a.seqs.table_stride;
+        auto page_of = [&](int j) {  // this lane's page of key tile j
+            int page = a.pages.num_pages;  // behind the cache's end: zeros
+            if (j < n && lane < boxes) {
+                const int key = kt.first(j) + lane * box;
+                if (key <= last) {
+                    const int x = table[key >> a.pages.page_shift];
+                    if (x >= 0 && x < a.pages.num_pages) page = x;
+                }
+            }
+            return page;
+        };
+        int issued = 0;
+        bool ok = true;
+        int page = page_of(0);
+        for (int j = 0; j < n && ok; ++j) {
+            const int key = kt.first(j) + lane * box;
+            const int next = page_of(j + 1);
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const int i = 2 * j + w, s = i % SL;
+                if (i >= SL) ok = warp_wait(&empty[s], ((i / SL) - 1) & 1, err, kErrLoad);
+                if (!ok) break;
+                if (lane == 0) ptx::mbar_arrive_expect_tx(&full[s], C::kTileBytes);
+                __syncwarp();
+                if (lane < boxes) {
+                    const uint32_t dst = ptx::smem_u32(smem + C::kKvOff + s * C::kTileBytes) + lane * box * 128;
+#pragma unroll
+                    for (int d = 0; d < C::kBlocks; ++d)
+                        tma_load_4d(dst + d * kBlock, w ? &tm_v : &tm_k, &full[s], d * 64, key & (page_size - 1), h, page);
+                }
+                ++issued;
+            }
+            page = next;
+        }
+        // no copy may be in flight when the CTA ends
+        for (int i = max(0, issued - SL); i < issued; ++i)
+            warp_wait(&full[i % SL], (i / SL) & 1, err, kErrLoad);
+    } else if (warp == kMmaWarp) {
+        // ------------------------------------------------ MMA issuer
+        constexpr uint32_t idesc_s = ptx::umma_idesc_f16(kTileRows, kTileKeys, BF16);
+        constexpr uint32_t idesc_o = ptx::umma_idesc_f16(kTileRows, DP, BF16) | (1u << 16);  // B = V is MN-major
+        bool ok = warp_wait(qfull, 0, err, kErrMma);
+        int done[2] = {0, 0};  // products P V issued
+        const uint32_t q_base = ptx::smem_u32(smem), kv_base = ptx::smem_u32(smem + C::kKvOff);
+        // step j: P V of tile j - 1, then the scores of tile j, of one row tile after the other
+        for (int j = 0; j <= n && ok; ++j) {
+            const int sk = (2 * j) % SL, sv = (2 * j + SL - 1) % SL;  // slots of K_j, V_{j-1}
+            if (j > 0) ok = warp_wait(&full[sv], ((2 * j - 1) / SL) & 1, err, kErrMma);
+            if (ok && j < n) ok = warp_wait(&full[sk], ((2 * j) / SL) & 1, err, kErrMma);
+            if (ok && j > 0) {
+                // values that no row sees (behind the length, before the window) are made 0: what
+                // such slots hold is anybody's, and 0 x NaN would reach every row
+                const int k0 = kt.first(j - 1);
+                const bool cut = k0 + kTileKeys - 1 > last || (k0 < first_seen && k0 + kTileKeys > a.sinks);
+                if (cut) {
+                    const uint32_t v = kv_base + sv * C::kTileBytes;
+                    for (int i = lane; i < kTileKeys * CH; i += 32) {
+                        const int r = i / CH, c = i % CH, key = k0 + r;
+                        if (key > last || (key < first_seen && key >= a.sinks))
+                            ptx::st_shared_v4(v + (c >> 3) * kBlock + r * 128 + (c & 7) * 16, make_uint4(0, 0, 0, 0));
+                    }
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const uint32_t ts = tmem + C::kS + t * 128, to = tmem + C::kO + t * 128;
+                if (ok && j > 0 && active(t, kt.first(j - 1))) {
+                    ok = warp_wait(&pfull[t], done[t] & 1, err, kErrMma);
+                    ptx::tc_fence_after();
+                    if (ok && lane == 0) {
+                        const uint32_t v = kv_base + sv * C::kTileBytes;
+#pragma unroll
+                        for (int kk = 0; kk < kTileKeys / 16; ++kk)
+                            ptx::umma_f16_ts(to, ts + kk * 8, ptx::umma_desc_sw128_mn(v + kk * 2048, kBlock, 1024), idesc_o,
+                                             done[t] > 0 || kk > 0 ? 1u : 0u);
+                    }
+                    ++done[t];
+                }
+                if (t == 1 && j > 0 && lane == 0) ptx::umma_commit(&empty[sv]);
+                if (ok && j < n && active(t, kt.first(j)) && lane == 0) {
+                    ptx::tc_fence_after();
+                    const uint32_t q = q_base + t * C::kTileBytes, k = kv_base + sk * C::kTileBytes;
+#pragma unroll
+                    for (int kk = 0; kk < DP / 16; ++kk) {
+                        const uint32_t off = (kk >> 2) * kBlock + (kk & 3) * 32;
+                        ptx::umma_f16(ts, ptx::umma_desc_sw128(q + off), ptx::umma_desc_sw128(k + off), idesc_s, kk > 0 ? 1u : 0u);
+                    }
+                    ptx::umma_commit(&sfull[t]);
+                }
+                if (t == 1 && j < n && lane == 0) ptx::umma_commit(&empty[sk]);
+                __syncwarp();
+            }
+        }
+        if (lane == 0) ptx::umma_commit(ofull);
+        __syncwarp();
+    } else {
+        // ------------------------------------------------ softmax of row tile t, a row a thread
+        const int t = warp >> 2, tid = threadIdx.x & 127;
+        {
+            // the tile's query rows, 16 bytes a thread, into the swizzled operand layout
+            const uint32_t dst = ptx::smem_u32(smem + t * C::kTileBytes);
+#pragma unroll 4
+            for (int i = tid; i < kTileRows * CH; i += 128) {
+                const int r = i / CH, c = i % CH, row = row0 + t * kTileRows + r;
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (row < rows && c * 8 < a.pages.dim)
+                    x = *reinterpret_cast<const uint4*>(a.q + (sq.t0 + row / a.group) * a.q_token +
+                                                        (h * a.group + row % a.group) * a.q_head + c * 8);
+                ptx::st_shared_v4(dst + (c >> 3) * kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4), x);
+            }
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(qfull);
+        }
+        const int row = row0 + t * kTileRows + tid;
+        const bool live_row = row < rows;
+        const int p = live_row ? max(-1, sq.p0 + row / a.group) : -1;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + C::kS + t * 128 + lanes, to = tmem + C::kO + t * 128 + lanes;
+        const int page_size = 1 << a.pages.page_shift;
+        const int step = min(page_size, kTileKeys), steps = kTileKeys / step;
+        const int32_t* table = a.seqs.tables + b * a.seqs.table_stride;
+        const float sc = a.scale_log2;
+        float m = -INFINITY, l = 0.f;  // m in units of the unscaled score
+        int seen = 0;
+        bool ok = true;
+        // which pages of a tile are pages, one a lane; looked up a tile ahead
+        auto page_ok = [&](int j) {
+            bool good = true;
+            if (j < n && lane < steps) {
+                const int key = kt.first(j) + lane * step;
+                if (key <= last) {
+                    const int x = table[key >> a.pages.page_shift];
+                    good = x >= 0 && x < a.pages.num_pages;
+                }
+            }
+            return good;
+        };
+        bool good = page_ok(0);
+        for (int j = 0; j < n; ++j) {
+            const bool good_now = good;
+            good = page_ok(j + 1);
+            const int k0 = kt.first(j);
+            if (!active(t, k0)) continue;
+            if (!warp_wait(&sfull[t], seen & 1, err, kErrSoftmax)) {
+                ok = false;
+                break;
+            }
+            ptx::tc_fence_after();
+            uint32_t s[kTileKeys];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, s + c * 32);
+            ptx::tmem_ld_wait();
+            const uint32_t pages = __ballot_sync(0xffffffffu, good_now);
+            const bool whole = pages == 0xffffffffu && k0 + kTileKeys - 1 <= p_lo[t] &&
+                               (a.window == 0 || p_hi[t] - k0 < a.window || k0 + kTileKeys <= a.sinks);
+            if (!whole) {
+                // keys k0 + [from, to) of the window, or before `sink`, on pages that are pages
+                const int hi = p - k0, lo = a.window ? hi - a.window : -1, sink = a.sinks - k0;
+#pragma unroll
+                for (int c = 0; c < kTileKeys; ++c) {
+                    const bool in = c <= hi && (c > lo || a.window == 0 || c < sink);
+                    if (!in) s[c] = 0xff800000u;
+                }
+                if (pages != 0xffffffffu) {
+#pragma unroll
+                    for (int c = 0; c < kTileKeys; ++c)
+                        if (!((pages >> (c / step)) & 1)) s[c] = 0xff800000u;
+                }
+            }
+            float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < kTileKeys; ++c) x[c & 3] = fmaxf(x[c & 3], __uint_as_float(s[c]));
+            const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+            if (seen == 0) {
+                m = top;
+            } else {
+                const bool grow = (top - m) * sc > kSlack || (m == -INFINITY && top > m);
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float f = grow ? exp2_approx((m - top) * sc) : 1.f;
+                    if (grow) m = top;
+                    l *= f;
+#pragma unroll 1
+                    for (int c = 0; c < DP; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(to + c, o);
+                        ptx::tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st32(to + c, o);
+                    }
+                }
+            }
+            const float base = m == -INFINITY ? 0.f : m * sc;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < kTileKeys; c += 2) {
+                const float u = exp2_approx(__uint_as_float(s[c]) * sc - base);
+                const float w = exp2_approx(__uint_as_float(s[c + 1]) * sc - base);
+                sum[c & 2] += u;
+                sum[(c & 2) + 1] += w;
+                s[c >> 1] = pack2<BF16>(u, w);
+            }
+            tmem_st32(ts, s);
+            tmem_st32(ts + 32, s + 32);
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            ptx::tmem_st_wait();
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&pfull[t]);
+            ++seen;
+        }
+        // ------------------------------------------------ epilogue
+        if (ok) ok = warp_wait(ofull, 0, err, kErrEnd);
+        ptx::tc_fence_after();
+        if (ok) {
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const int64_t o_off = (sq.t0 + row / a.group) * a.o_token + (h * a.group + row % a.group) * a.o_head;
+            bool odd = false;
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 32) {
+                uint32_t o[32];
+                if (seen > 0) {
+                    tmem_ld32(to + c, o);
+                    ptx::tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0u;  // no product was made
+                }
+                float nan = 0.f;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) nan += __uint_as_float(o[e]) * 0.f;
+                odd |= !(nan == 0.f);
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        w[i] = pack2<BF16>(__uint_as_float(o[e + 2 * i]) * inv, __uint_as_float(o[e + 2 * i + 1]) * inv);
+                    if (live_row && c + e < a.pages.dim)
+                        *reinterpret_cast<uint4*>(a.out + o_off + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            uint32_t again = __ballot_sync(0xffffffffu, odd && live_row);
+            while (again) {
+                const int r = row - lane + __ffs(again) - 1;
+                again &= again - 1;
+                __syncwarp();
+                careful_row<BF16>(a, b, h, (sq.t0 + r / a.group) * a.q_token + (h * a.group + r % a.group) * a.q_head,
+                                  (sq.t0 + r / a.group) * a.o_token + (h * a.group + r % a.group) * a.o_head,
+                                  sq.p0 + r / a.group);
+            }
+        }
+    }
+
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem, 512);
+    }
+}
+
+template <int DP, bool BF16>
+cudaError_t launch_prompt_t(const AttnArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t s) {
+    auto kern = prompt_kernel<DP, BF16>;
+    static std::atomic<uint64_t> ready{0};
+    cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), Cfg<DP>::kSmem, ready);
+    if (e != cudaSuccess) return e;
+    const int rows = a.seqs.max_q * a.group;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.pages.heads_kv, (rows + 2 * kTileRows - 1) / (2 * kTileRows), a.seqs.batch);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Cfg<DP>::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, tm_k, tm_v, a);
+}
+
+}  // namespace
+
+bool prompt_fits(const AttnArgs& a) {
+    const int64_t pairs = (static_cast<int64_t>(a.seqs.max_q) * a.group + 2 * kTileRows - 1) / (2 * kTileRows);
+    return pairs <= 65535 && a.seqs.batch <= 65535;
+}
+
+cudaError_t launch_prompt(const AttnArgs& a, bool bf16, cudaStream_t s) {
+    const PageView& p = a.pages;
+    const uint64_t size = uint64_t{1} << p.page_shift;
+    const uint64_t dims[4] = {static_cast<uint64_t>(p.dim), size, static_cast<uint64_t>(p.heads_kv),
+                              static_cast<uint64_t>(p.num_pages)};
+    // the stride of a dimension of one is never used, but must be a valid one
+    const uint64_t strides[3] = {static_cast<uint64_t>(p.stride_token) * 2,
+                                 p.heads_kv > 1 ? static_cast<uint64_t>(p.stride_head) * 2 : 16,
+                                 p.num_pages > 1 ? static_cast<uint64_t>(p.stride_page) * 2 : 16};
+    const uint32_t box[4] = {64, static_cast<uint32_t>(std::min<uint64_t>(size, kTileKeys)), 1, 1};
+    const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    CUtensorMap mk, mv;
+    if (encode_tmap_4d(&mk, dt, p.k, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B) != CUDA_SUCCESS ||
+        encode_tmap_4d(&mv, dt, p.v, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B) != CUDA_SUCCESS)
+        return cudaErrorInvalidValue;
+    if (p.dim <= 64) return bf16 ? launch_prompt_t<64, true>(a, mk, mv, s) : launch_prompt_t<64, false>(a, mk, mv, s);
+    return bf16 ? launch_prompt_t<128, true>(a, mk, mv, s) : launch_prompt_t<128, false>(a, mk, mv, s);
+}
+
+cudaError_t read_attention_error(int* out, cudaStream_t s) {
+    const int zero = 0;
+    cudaError_t e = cudaMemcpyFromSymbolAsync(out, g_attention_error, sizeof(int), 0, cudaMemcpyDeviceToHost, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    if (e == cudaSuccess && *out) e = cudaMemcpyToSymbolAsync(g_attention_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    return e;
+}
+
+}  // namespace w4a16

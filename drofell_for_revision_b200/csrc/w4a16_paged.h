@@ -64,6 +64,12 @@ SplitPlan plan_split(const AttnArgs& a, int num_sms);
 size_t split_workspace_bytes(const SplitPlan& p, int dim);
 cudaError_t launch_split(const AttnArgs& a, const SplitPlan& p, bool bf16, cudaStream_t s);
 
+// Attention of prompts on the tensor cores (w4a16_attn_sm100.cu).
+bool prompt_fits(const AttnArgs& a);
+cudaError_t launch_prompt(const AttnArgs& a, bool bf16, cudaStream_t s);
+// The current device's error word of its bounded waits, then cleared. Synchronises `s`.
+cudaError_t read_attention_error(int* out, cudaStream_t s);
+
 constexpr int kCopyPairs = 500;
 struct CopyArgs {
     uint8_t* base[2];  // K, V

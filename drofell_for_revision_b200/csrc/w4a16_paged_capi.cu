@@ -20,6 +20,12 @@ int cuda_error(cudaError_t e, const char* what) {
     return report_error(W4A16_ERR_CUDA, "%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
 }
 
+constexpr int kMostTokens = (1 << 30) - 1024;
+
+// Rows of a sequence and key-value head (new tokens x heads of the group) from which the
+// tensor-core kernel takes the call.
+constexpr int kPromptRows = 65;
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 int check_pages(const w4a16_pages* p) {
@@ -32,6 +38,8 @@ int check_pages(const w4a16_pages* p) {
         return report_error(W4A16_ERR_UNSUPPORTED, "head dim %d (a multiple of 8, at most 128)", p->head_dim);
     if (p->num_pages <= 0 || p->heads_kv <= 0)
         return report_error(W4A16_ERR_INVALID, "num_pages=%d heads_kv=%d", p->num_pages, p->heads_kv);
+    if ((p->num_pages > 1 && p->stride_page == 0) || (p->heads_kv > 1 && p->stride_head == 0) || p->stride_token == 0)
+        return report_error(W4A16_ERR_INVALID, "page strides of 0");
     if (p->stride_page < 0 || p->stride_head < 0 || p->stride_token < 0 || p->stride_page % 8 || p->stride_head % 8 ||
         p->stride_token % 8)
         return report_error(W4A16_ERR_INVALID, "page strides must be non-negative multiples of 8 elements");
@@ -49,8 +57,10 @@ int check_seqs(const w4a16_pages* p, const w4a16_seqs* s) {
         return report_error(W4A16_ERR_INVALID, "null tables or lens");
     if (!s->cu_q_dev && s->tokens != s->batch)
         return report_error(W4A16_ERR_INVALID, "%d rows for %d sequences of one new token each", s->tokens, s->batch);
-    if (static_cast<int64_t>(s->table_width) * p->page_size > INT_MAX - 1024)
-        return report_error(W4A16_ERR_UNSUPPORTED, "tables of %d pages of %d tokens", s->table_width, p->page_size);
+    // sums of a position, a key and a window stay within 32 bits
+    if (static_cast<int64_t>(s->table_width) * p->page_size > kMostTokens || s->tokens > kMostTokens)
+        return report_error(W4A16_ERR_UNSUPPORTED, "tables of %d pages of %d tokens, %d new tokens: at most %d tokens",
+                            s->table_width, p->page_size, s->tokens, kMostTokens);
     return W4A16_OK;
 }
 
@@ -109,9 +119,15 @@ AttnArgs attn_args(const w4a16_pages* pages, const w4a16_seqs* seqs, int heads, 
     a.seqs.max_q = seqs->cu_q_dev ? seqs->max_q : 1;
     a.heads = heads;
     a.group = heads / pages->heads_kv;
-    a.window = window;
-    a.sinks = sinks;
+    // a window of all the tables cover hides nothing
+    const int covered = seqs->table_width * pages->page_size;
+    a.window = window >= covered ? 0 : window;
+    a.sinks = a.window == 0 ? 0 : (sinks < covered ? sinks : covered);
     return a;
+}
+
+bool takes_prompt(const AttnArgs& a) {
+    return static_cast<int64_t>(a.seqs.max_q) * a.group >= kPromptRows && prompt_fits(a);
 }
 
 int check_attention(const w4a16_pages* pages, const w4a16_seqs* seqs, int heads, int window, int sinks) {
@@ -187,6 +203,7 @@ size_t w4a16_paged_attention_workspace_size(const w4a16_pages* pages, const w4a1
                                             int sinks) {
     if (check_attention(pages, seqs, heads, window, sinks) != W4A16_OK) return 0;
     if (seqs->batch == 0 || seqs->tokens == 0 || seqs->max_q == 0) return 0;
+    if (takes_prompt(attn_args(pages, seqs, heads, window, sinks))) return 0;
     const int sms = sm_count(pages->device);
     if (sms == 0) return 0;
     return split_workspace_bytes(plan_split(attn_args(pages, seqs, heads, window, sinks), sms), pages->head_dim);
@@ -197,7 +214,8 @@ int w4a16_paged_attention(const w4a16_pages* pages, const w4a16_seqs* seqs, cons
                           void* stream) {
     int rc = check_attention(pages, seqs, heads, window, sinks);
     if (rc != W4A16_OK) return rc;
-    if (!std::isfinite(scale)) return report_error(W4A16_ERR_INVALID, "scale is not finite");
+    if (!(scale > 0.f) || !std::isfinite(scale * 1.4426950408889634f))
+        return report_error(W4A16_ERR_INVALID, "scale must be positive and finite");
     if (seqs->batch == 0 || seqs->tokens == 0 || seqs->max_q == 0) return W4A16_OK;
     rc = check_rows(q, "q");
     if (rc == W4A16_OK) rc = check_rows(out, "out");
@@ -208,11 +226,17 @@ int w4a16_paged_attention(const w4a16_pages* pages, const w4a16_seqs* seqs, cons
     a.out = static_cast<uint16_t*>(out->dev);
     a.o_token = out->stride_token, a.o_head = out->stride_head;
     a.scale_log2 = scale * 1.4426950408889634f;
+    const bool bf16 = pages->dtype == W4A16_DTYPE_BF16;
+    if (takes_prompt(a)) {
+        DeviceGuard guard(pages->device);
+        if (!guard.ok) return report_error(W4A16_ERR_INVALID, "device %d", pages->device);
+        const cudaError_t e = launch_prompt(a, bf16, static_cast<cudaStream_t>(stream));
+        return e == cudaSuccess ? W4A16_OK : cuda_error(e, "paged attention launch");
+    }
     const int sms = sm_count(pages->device);
     if (sms == 0) return report_error(W4A16_ERR_CUDA, "no device %d", pages->device);
     DeviceGuard guard(pages->device);
     if (!guard.ok) return report_error(W4A16_ERR_INVALID, "device %d", pages->device);
-    const bool bf16 = pages->dtype == W4A16_DTYPE_BF16;
     const SplitPlan p = plan_split(a, sms);
     const size_t need = split_workspace_bytes(p, pages->head_dim);
     if (workspace_bytes < need || (need > 0 && !workspace_dev))
@@ -221,6 +245,14 @@ int w4a16_paged_attention(const w4a16_pages* pages, const w4a16_seqs* seqs, cons
     a.ws = need > 0 ? static_cast<float*>(workspace_dev) : nullptr;
     const cudaError_t e = launch_split(a, p, bf16, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? W4A16_OK : cuda_error(e, "paged attention launch");
+}
+
+int w4a16_paged_error(int device, void* stream, int* err_out) {
+    if (!err_out) return report_error(W4A16_ERR_INVALID, "null argument");
+    DeviceGuard guard(device);
+    if (!guard.ok) return report_error(W4A16_ERR_INVALID, "device %d", device);
+    const cudaError_t e = read_attention_error(err_out, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? W4A16_OK : cuda_error(e, "paged error read");
 }
 
 int w4a16_copy_pages(void* k_dev, void* v_dev, int64_t stride_layer_bytes, int64_t stride_page_bytes, int layers,

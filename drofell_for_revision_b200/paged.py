@@ -18,6 +18,7 @@ whatever they then hold. Calls run on the current stream. Nothing here has a gra
 """
 from __future__ import annotations
 
+import ctypes
 import heapq
 import math
 from typing import Dict, Iterable, List, Optional, Sequence, Tuple, Union
@@ -63,6 +64,16 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tab
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     return _ext().paged_attention(q, k_pages, v_pages, tables, lens, cu_q, max_q, scale, window, sinks, out)
+
+
+def device_error(device: Optional[torch.device] = None) -> int:
+    """Nonzero if a bounded wait inside an attention kernel on this device gave up since the
+    last call (outputs since then may be missing). Synchronises the current stream."""
+    index = torch.device(device or "cuda").index
+    index = torch.cuda.current_device() if index is None else index
+    v = ctypes.c_int(0)
+    _capi.check(_capi.lib().w4a16_paged_error(index, _capi.stream_ptr(index), ctypes.byref(v)))
+    return v.value
 
 
 def _ids(x: PageIds) -> torch.Tensor:

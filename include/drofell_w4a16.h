@@ -284,7 +284,7 @@ W4A16_API int w4a16_append_kv(const w4a16_pages* pages, const w4a16_seqs* seqs, 
                               const w4a16_rows* v, const w4a16_rows* q, const w4a16_rows* q_out, int heads,
                               const float* rope_dev, int rope_positions, int rope_dim, int interleaved, void* stream);
 
-/* out = softmax(scale q k^T) v of every new token over the visible tokens of its sequence:
+/* out = softmax(scale q k^T) v (scale > 0) of every new token over the visible tokens of its sequence:
  * not after it, and with window > 0 the last `window` ones (itself counted) and the first
  * `sinks` ones. heads is a multiple of heads_kv; query head i reads key-value head
  * i / (heads / heads_kv). Rows that see nothing are 0. Softmax statistics and sums in
@@ -295,6 +295,11 @@ W4A16_API int w4a16_paged_attention(const w4a16_pages* pages, const w4a16_seqs* 
                                     void* workspace_dev, size_t workspace_bytes, void* stream);
 W4A16_API size_t w4a16_paged_attention_workspace_size(const w4a16_pages* pages, const w4a16_seqs* seqs, int heads,
                                                       int window, int sinks);
+
+/* Read (and clear) the device's error word of w4a16_paged_attention: nonzero means that a
+ * bounded wait inside a kernel gave up, and outputs since the last read may be missing.
+ * Synchronises `stream`. Diagnostic only. */
+W4A16_API int w4a16_paged_error(int device, void* stream, int* err_out);
 
 /* Copy whole pages, of every layer and of K and V: page dst_host[i] gets page src_host[i].
  * A page is page_bytes contiguous bytes at layer * stride_layer_bytes + id *

@@ -22,6 +22,12 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 
 
+@pytest.fixture(autouse=True)
+def no_wait_gave_up():
+    yield
+    assert paged.device_error(DEV) == 0
+
+
 class Batch:
     """Sequences of given (length, new tokens) with pages in random order."""
 

@@ -48,7 +48,7 @@ def append(p=None, s=None, k=None, v=None, q=None, q_out=None, heads=4, rope=Non
     (dict(page_size=4), UNSUPPORTED), (dict(page_size=24), UNSUPPORTED), (dict(page_size=512), UNSUPPORTED),
     (dict(head_dim=132), UNSUPPORTED), (dict(head_dim=136), UNSUPPORTED), (dict(head_dim=0), UNSUPPORTED),
     (dict(stride_token=100), INVALID), (dict(stride_page=-8), INVALID), (dict(num_pages=0), INVALID),
-    (dict(heads_kv=0), INVALID)])
+    (dict(heads_kv=0), INVALID), (dict(stride_head=0), INVALID), (dict(stride_token=0), INVALID)])
 def test_pages_are_checked(kw, code):
     assert attention(p=pages(**kw)) == code
     assert append(p=pages(**kw)) == code
@@ -57,7 +57,8 @@ def test_pages_are_checked(kw, code):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(tables_dev=None), INVALID), (dict(lens_dev=None), INVALID), (dict(batch=-1), INVALID), (dict(tokens=3), INVALID),
-    (dict(table_width=-1), INVALID), (dict(max_q=-1), INVALID), (dict(table_width=1 << 28), UNSUPPORTED)])
+    (dict(table_width=-1), INVALID), (dict(max_q=-1), INVALID), (dict(table_width=1 << 28), UNSUPPORTED),
+    (dict(cu_q_dev=FAKE, tokens=1 << 30), UNSUPPORTED)])
 def test_sequences_are_checked(kw, code):
     assert attention(s=seqs(**kw)) == code
     assert append(s=seqs(**kw)) == code
@@ -70,12 +71,13 @@ def test_attention_arguments_are_checked():
     assert attention(window=4, sinks=-1) == INVALID
     assert attention(sinks=4) == INVALID
     assert b"sinks" in _capi.lib().w4a16_last_error()
-    for scale in (float("nan"), float("inf")):
+    for scale in (float("nan"), float("inf"), 0.0, -0.1):
         assert attention(scale=scale) == INVALID
     assert attention(q=rows(dev=None)) == INVALID
     assert attention(out=rows(stride_head=4)) == INVALID
     assert attention(out=rows(dev=FAKE + 2)) == INVALID
-    assert attention(s=seqs(cu_q_dev=FAKE, max_q=1 << 30, tokens=5)) == UNSUPPORTED
+    assert attention(s=seqs(cu_q_dev=FAKE, max_q=(1 << 31) - 1, tokens=5)) == UNSUPPORTED
+    assert _capi.lib().w4a16_paged_error(0, None, None) == INVALID
     # nothing to do: no CUDA call
     assert attention(s=seqs(batch=0, tokens=0)) == OK
     assert attention(s=seqs(cu_q_dev=FAKE, tokens=0)) == OK
