@@ -14,12 +14,17 @@
 // Rounding P to the 16-bit type (at most half a step each) is what lets the second product
 // run on the tensor cores at their 16-bit rate; l sums the unrounded fp32 values.
 //
-// Warp roles (320 threads): warps 0-3 and 4-7 softmax and epilogue of the two row tiles,
-// one row a thread; warp 8 loads K and V page by page (TMA, lane = page; a page id that is
-// no page reads zeros behind the cache's end); warp 9 issues the MMAs: while one row tile
-// is in its softmax, the tensor cores work for the other.
+// Warp roles (384 threads): warps 0-3 and 4-7 softmax and epilogue of the two row tiles, one
+// row a thread; warp 8 loads K and V page by page (TMA, lane = page; a page id that is no
+// page reads zeros behind the cache's end); warp 9 puts zeros into V where a tile holds keys
+// that no row sees; warps 10 and 11 issue the MMAs of one row tile each: while one is in its
+// softmax, the tensor cores work for the other. One warp for both left them idle a third of
+// the time: its waits, slowed to some 300 cycles each by the exponentials that share the
+// queue to the shared-memory and special-function units, added up.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
+
 #include <cuda.h>
 
 #include "w4a16_internal.h"
@@ -31,8 +36,13 @@ namespace {
 
 constexpr int kTileKeys = 128;
 constexpr int kTileRows = 128;
-constexpr int kThreads = 10 * 32;
-constexpr int kLoadWarp = 8, kMmaWarp = 9;
+constexpr int kThreads = 12 * 32;
+constexpr int kLoadWarp = 8, kCleanWarp = 9, kMmaWarp = 10;  // kMmaWarp + t: row tile t
+// Registers a thread: 168 at launch (65536 / 384); the last four warps give theirs to the
+// softmax warps, whose 128 scores a row stay in registers: 2 * 128 * 208 + 128 * 88 of the
+// 384 * 168 that the CTA was launched with.
+constexpr int kLaunchRegs = 168, kSoftmaxRegs = 208, kOtherRegs = 88;
+static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "more registers than launched with");
 constexpr int kBlock = 128 * 128;  // bytes of a [128 rows x 64] operand block, 128-byte swizzle
 constexpr uint32_t kWaitLimit = 1u << 18;  // x ~10 us sleeps: a few seconds
 constexpr float kSlack = 8.f;              // log2 of the growth that O tolerates without rescaling
@@ -93,9 +103,102 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-// Bounded wait of a whole warp: the same answer in every lane.
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 of_pair(uint64_t x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+
+// 2^x of two values on the FMA units, x <= 8: 2^round(x) by the exponent bits, 2^f for f in
+// [-1/2, 1/2] by the polynomial of degree 4 of least relative error with value 1 at 0
+// (2.8e-6, a hundredth of the 16-bit rounding that follows). Below -126 it runs out through
+// the denormals to exactly 0 at -127, where smaller x (and -inf) are held. NaN stays NaN.
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
+    const uint64_t v = pair_of(x.x, x.y);
+    const uint64_t r = add2(v, pair_of(12582912.f, 12582912.f));  // round(x) in the low bits
+    const uint64_t f = fma2(add2(r, pair_of(-12582912.f, -12582912.f)), pair_of(-1.f, -1.f), v);
+    uint64_t y = fma2(f, pair_of(0.009582700208f, 0.009582700208f), pair_of(0.05590687692f, 0.05590687692f));
+    y = fma2(y, f, pair_of(0.2402410358f, 0.2402410358f));
+    y = fma2(y, f, pair_of(0.6931241155f, 0.6931241155f));
+    y = fma2(y, f, pair_of(1.f, 1.f));
+    const float2 a = of_pair(y), b = of_pair(r);
+    return make_float2(__int_as_float(__float_as_int(a.x) + (__float_as_int(b.x) << 23)),
+                       __int_as_float(__float_as_int(a.y) + (__float_as_int(b.y) << 23)));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// A row's 128 weights 2^(sc s - base) into its columns of P at `ts`, in halves: the product
+// starts on one (an arrival on pfull[0]) while the other is still made. Returns their sum.
+// Every fourth pair is raised on the FMA units, beside the special-function units that bound
+// this phase.
+template <bool BF16>
+__device__ __forceinline__ float weights(uint32_t (&s)[kTileKeys], float sc, float base, uint32_t ts, uint64_t* pfull) {
+    const uint64_t sc2 = pair_of(sc, sc), base2 = pair_of(-base, -base);
+    uint64_t sum[2] = {0, 0};
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int c = half * 64; c < half * 64 + 64; c += 2) {
+            float2 x = of_pair(fma2(pair_of(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2, base2));
+            if ((c & 6) == 6) {
+                x = exp2_fma(x);
+            } else {
+                x.x = exp2_approx(x.x);
+                x.y = exp2_approx(x.y);
+            }
+            sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], pair_of(x.x, x.y));
+            s[c >> 1] = pack2<BF16>(x.x, x.y);
+        }
+        tmem_st32(ts + half * 32, s + half * 32);
+        ptx::tmem_st_wait();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&pfull[half]);
+    }
+    const float2 part = of_pair(add2(sum[0], sum[1]));
+    return part.x + part.y;
+}
+
+// Bounded wait that sleeps between polls. Not unrolled, as nothing in this kernel that need
+// not be: with everything unrolled it had 180 KB of instructions, and fetching them again for
+// every CTA and tile took longer than the work.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* err, int code) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < kWaitLimit; ++i)
+        if (ptx::mbar_try_wait_sleep(bar, parity, 10000u)) return true;
+    atomicCAS(err, 0, code);
+    return false;
+}
+// The same answer in every lane of the warp.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
-    return __all_sync(0xffffffffu, ptx::mbar_wait_sleep_bounded(bar, parity, kWaitLimit, err, code));
+    return __all_sync(0xffffffffu, wait(bar, parity, err, code));
+}
+
+// The lowest n bits, n held to 0 .. 32.
+__device__ __forceinline__ uint32_t first_bits(int n) {
+    return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
 }
 
 // One row, key by key, each key by selection: for rows whose sums are not finite because a
@@ -117,6 +220,7 @@ __device__ __noinline__ void careful_row(const AttnArgs& a, int b, int h, int64_
     load4(a.q + q_off, q);
     const int32_t* table = a.seqs.tables + b * a.seqs.table_stride;
     const int lo = a.window ? max(0, p + 1 - a.window) : 0;
+#pragma unroll 1
     for (int j = 0; j <= p; ++j) {
         if (j >= a.sinks && j < lo) j = lo;
         const int page = table[j >> a.pages.page_shift];
@@ -154,11 +258,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
     uint64_t* empty = full + SL;
-    uint64_t* qfull = empty + SL;
-    uint64_t* sfull = qfull + 1;  // [2] S of a row tile is complete (and all products before it)
-    uint64_t* pfull = sfull + 2;  // [2] P is written, O rescaled
-    uint64_t* ofull = pfull + 2;  // all products are complete
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ofull + 1);
+    uint64_t* qfull = empty + SL;  // [2] the query rows are in place
+    uint64_t* sfull = qfull + 2;   // [2] S of a row tile is complete (and all products before it)
+    uint64_t* pfull = sfull + 2;  // [2][2] half of P is written (the first: O rescaled)
+    uint64_t* ofull = pfull + 4;  // [2] all products are complete
+    uint64_t* dirty = ofull + 2;  // V of a tile that the mask cuts is loaded
+    uint64_t* clean = dirty + 1;  // and holds zeros where no row sees
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(clean + 1);
+    volatile uint32_t* bad = tmem_slot + 1;  // [8] boxes of tile j % 8 whose page id is no page
 
     ptx::grid_dep_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -181,6 +288,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const KeyTiles<kTileKeys> kt(p_lo[0], last, a.window, a.sinks);
     const int n = kt.count;
     const int first_seen = a.window ? max(0, max(p_lo[0], 0) + 1 - a.window) : 0;  // of the window, any row
+    // whether the 128 keys from k0 hold some that no row sees: behind the length or before the
+    // window. What lies there is anybody's, and 0 x NaN would reach every row.
+    auto cut = [&](int k0) { return k0 + kTileKeys - 1 > last || (k0 < first_seen && k0 + kTileKeys > a.sinks); };
     // whether any row of row tile t sees any key of the 128 from k0
     auto active = [&](int t, int k0) {
         return k0 <= p_hi[t] && (a.window == 0 || k0 + kTileKeys - 1 > max(p_lo[t], 0) - a.window || k0 < a.sinks);
@@ -189,14 +299,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0) {
         for (int s = 0; s < SL; ++s) {
             ptx::mbar_init(&full[s], 1);
-            ptx::mbar_init(&empty[s], 1);
+            ptx::mbar_init(&empty[s], 2);
         }
-        ptx::mbar_init(qfull, 8);
         for (int t = 0; t < 2; ++t) {
-            ptx::mbar_init(&sfull[t], 1);
-            ptx::mbar_init(&pfull[t], 4);
+            ptx::mbar_init(&qfull[t], 4);
+            ptx::mbar_init(&ofull[t], 1);
+            ptx::mbar_init(&sfull[t], 2);
+            ptx::mbar_init(&pfull[2 * t], 4);
+            ptx::mbar_init(&pfull[2 * t + 1], 4);
         }
-        ptx::mbar_init(ofull, 1);
+        ptx::mbar_init(dirty, 2);
+        ptx::mbar_init(clean, 1);
         ptx::fence_mbar_init();
         ptx::prefetch_tmap(&tm_k);
         ptx::prefetch_tmap(&tm_v);
@@ -211,156 +324,178 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = *tmem_slot;
     int* err = &g_attention_error;
 
-    if (warp == kLoadWarp) {
-        // ------------------------------------------------ K and V, page by page
-        const int page_size = 1 << a.pages.page_shift;
-        const int box = min(page_size, kTileKeys);
-        const int boxes = kTileKeys / box;  // per tile, at most 16: one a lane
-        const int32_t* table = a.seqs.tables + b * a.seqs.table_stride;
-        auto page_of = [&](int j) {  // this lane's page of key tile j
-            int page = a.pages.num_pages;  // behind the cache's end: zeros
-            if (j < n && lane < boxes) {
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == kLoadWarp) {
+            // ------------------------------------------------ K and V, page by page
+            const int page_size = 1 << a.pages.page_shift;
+            const int box = min(page_size, kTileKeys);
+            const int boxes = kTileKeys / box;  // per tile, at most 16: one a lane
+            const int32_t* table = a.seqs.tables + b * a.seqs.table_stride;
+            auto page_of = [&](int j) {  // this lane's page of key tile j
+                int page = a.pages.num_pages;  // behind the cache's end: zeros
+                if (j < n && lane < boxes) {
+                    const int key = kt.first(j) + lane * box;
+                    if (key <= last) page = table[key >> a.pages.page_shift];
+                }
+                return page;
+            };
+            int issued = 0;
+            bool ok = true;
+            int page = page_of(0);
+#pragma unroll 1
+            for (int j = 0; j < n && ok; ++j) {
                 const int key = kt.first(j) + lane * box;
-                if (key <= last) {
-                    const int x = table[key >> a.pages.page_shift];
-                    if (x >= 0 && x < a.pages.num_pages) page = x;
-                }
-            }
-            return page;
-        };
-        int issued = 0;
-        bool ok = true;
-        int page = page_of(0);
-        for (int j = 0; j < n && ok; ++j) {
-            const int key = kt.first(j) + lane * box;
-            const int next = page_of(j + 1);
+                const int next = page_of(j + 1);
+                const bool none = page < 0 || page >= a.pages.num_pages;
+                const uint32_t none_of = __ballot_sync(0xffffffffu, none && lane < boxes && key <= last);
+                if (none) page = a.pages.num_pages;
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                const int i = 2 * j + w, s = i % SL;
-                if (i >= SL) ok = warp_wait(&empty[s], ((i / SL) - 1) & 1, err, kErrLoad);
-                if (!ok) break;
-                if (lane == 0) ptx::mbar_arrive_expect_tx(&full[s], C::kTileBytes);
-                __syncwarp();
-                if (lane < boxes) {
-                    const uint32_t dst = ptx::smem_u32(smem + C::kKvOff + s * C::kTileBytes) + lane * box * 128;
-#pragma unroll
-                    for (int d = 0; d < C::kBlocks; ++d)
-                        tma_load_4d(dst + d * kBlock, w ? &tm_v : &tm_k, &full[s], d * 64, key & (page_size - 1), h, page);
-                }
-                ++issued;
-            }
-            page = next;
-        }
-        // no copy may be in flight when the CTA ends
-        for (int i = max(0, issued - SL); i < issued; ++i)
-            warp_wait(&full[i % SL], (i / SL) & 1, err, kErrLoad);
-    } else if (warp == kMmaWarp) {
-        // ------------------------------------------------ MMA issuer
-        constexpr uint32_t idesc_s = ptx::umma_idesc_f16(kTileRows, kTileKeys, BF16);
-        constexpr uint32_t idesc_o = ptx::umma_idesc_f16(kTileRows, DP, BF16) | (1u << 16);  // B = V is MN-major
-        bool ok = warp_wait(qfull, 0, err, kErrMma);
-        int done[2] = {0, 0};  // products P V issued
-        const uint32_t q_base = ptx::smem_u32(smem), kv_base = ptx::smem_u32(smem + C::kKvOff);
-        // step j: P V of tile j - 1, then the scores of tile j, of one row tile after the other
-        for (int j = 0; j <= n && ok; ++j) {
-            const int sk = (2 * j) % SL, sv = (2 * j + SL - 1) % SL;  // slots of K_j, V_{j-1}
-            if (j > 0) ok = warp_wait(&full[sv], ((2 * j - 1) / SL) & 1, err, kErrMma);
-            if (ok && j < n) ok = warp_wait(&full[sk], ((2 * j) / SL) & 1, err, kErrMma);
-            if (ok && j > 0) {
-                // values that no row sees (behind the length, before the window) are made 0: what
-                // such slots hold is anybody's, and 0 x NaN would reach every row
-                const int k0 = kt.first(j - 1);
-                const bool cut = k0 + kTileKeys - 1 > last || (k0 < first_seen && k0 + kTileKeys > a.sinks);
-                if (cut) {
-                    const uint32_t v = kv_base + sv * C::kTileBytes;
-                    for (int i = lane; i < kTileKeys * CH; i += 32) {
-                        const int r = i / CH, c = i % CH, key = k0 + r;
-                        if (key > last || (key < first_seen && key >= a.sinks))
-                            ptx::st_shared_v4(v + (c >> 3) * kBlock + r * 128 + (c & 7) * 16, make_uint4(0, 0, 0, 0));
+                for (int w = 0; w < 2; ++w) {
+                    const int i = 2 * j + w, s = i % SL;
+                    if (i >= SL) ok = warp_wait(&empty[s], ((i / SL) - 1) & 1, err, kErrLoad);
+                    if (!ok) break;
+                    if (lane == 0) {
+                        if (w == 0) bad[j & 7] = none_of;
+                        ptx::mbar_arrive_expect_tx(&full[s], C::kTileBytes);
                     }
-                    ptx::fence_proxy_async_smem();
                     __syncwarp();
+                    if (lane < boxes) {
+                        const uint32_t dst = ptx::smem_u32(smem + C::kKvOff + s * C::kTileBytes) + lane * box * 128;
+#pragma unroll
+                        for (int d = 0; d < C::kBlocks; ++d)
+                            tma_load_4d(dst + d * kBlock, w ? &tm_v : &tm_k, &full[s], d * 64, key & (page_size - 1), h, page);
+                    }
+                    ++issued;
                 }
+                page = next;
             }
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const uint32_t ts = tmem + C::kS + t * 128, to = tmem + C::kO + t * 128;
-                if (ok && j > 0 && active(t, kt.first(j - 1))) {
-                    ok = warp_wait(&pfull[t], done[t] & 1, err, kErrMma);
-                    ptx::tc_fence_after();
-                    if (ok && lane == 0) {
-                        const uint32_t v = kv_base + sv * C::kTileBytes;
-#pragma unroll
-                        for (int kk = 0; kk < kTileKeys / 16; ++kk)
-                            ptx::umma_f16_ts(to, ts + kk * 8, ptx::umma_desc_sw128_mn(v + kk * 2048, kBlock, 1024), idesc_o,
-                                             done[t] > 0 || kk > 0 ? 1u : 0u);
-                    }
-                    ++done[t];
+            // no copy may be in flight when the CTA ends
+#pragma unroll 1
+            for (int i = max(0, issued - SL); i < issued; ++i)
+                warp_wait(&full[i % SL], (i / SL) & 1, err, kErrLoad);
+        } else if (warp == kCleanWarp) {
+            // ------------------------------------------------ zeros into V where no row sees
+            // asked for by both MMA threads, one tile at a time (a barrier's parity tells only two
+            // phases apart: a warp that skips tiles cannot wait on `full`)
+            bool ok = true;
+            int asked = 0;
+#pragma unroll 1
+            for (int j = 0; j < n && ok; ++j) {
+                const int k0 = kt.first(j), s = (2 * j + 1) % SL;
+                if (!cut(k0)) continue;
+                ok = warp_wait(dirty, asked++ & 1, err, kErrMma);
+                const uint32_t v = ptx::smem_u32(smem + C::kKvOff + s * C::kTileBytes);
+#pragma unroll 1
+                for (int x = lane; ok && x < kTileKeys * CH; x += 32) {
+                    const int r = x / CH, c = x % CH, key = k0 + r;
+                    if (key > last || (key < first_seen && key >= a.sinks))
+                        ptx::st_shared_v4(v + (c >> 3) * kBlock + r * 128 + (c & 7) * 16, make_uint4(0, 0, 0, 0));
                 }
-                if (t == 1 && j > 0 && lane == 0) ptx::umma_commit(&empty[sv]);
-                if (ok && j < n && active(t, kt.first(j)) && lane == 0) {
-                    ptx::tc_fence_after();
-                    const uint32_t q = q_base + t * C::kTileBytes, k = kv_base + sk * C::kTileBytes;
-#pragma unroll
-                    for (int kk = 0; kk < DP / 16; ++kk) {
-                        const uint32_t off = (kk >> 2) * kBlock + (kk & 3) * 32;
-                        ptx::umma_f16(ts, ptx::umma_desc_sw128(q + off), ptx::umma_desc_sw128(k + off), idesc_s, kk > 0 ? 1u : 0u);
-                    }
-                    ptx::umma_commit(&sfull[t]);
-                }
-                if (t == 1 && j < n && lane == 0) ptx::umma_commit(&empty[sk]);
+                ptx::fence_proxy_async_smem();
                 __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(clean);
             }
+        } else if (ptx::elect_one_sync()) {
+            // ------------------------------------------------ MMA issuer of row tile t: one elected thread,
+            // so that the compiler knows it is one and keeps descriptors uniform (an MMA took 106
+            // cycles to issue in a `lane == 0` branch, 74 here: the tensor core's time)
+            const int t = warp - kMmaWarp;
+            constexpr uint32_t idesc_s = ptx::umma_idesc_f16(kTileRows, kTileKeys, BF16);
+            constexpr uint32_t idesc_o = ptx::umma_idesc_f16(kTileRows, DP, BF16) | (1u << 16);  // B = V is MN-major
+            const uint32_t ts = tmem + C::kS + t * 128, to = tmem + C::kO + t * 128;
+            const uint32_t q = ptx::smem_u32(smem) + t * C::kTileBytes, kv = ptx::smem_u32(smem + C::kKvOff);
+            bool ok = wait(&qfull[t], 0, err, kErrMma);
+            int done = 0, cleaned = 0;  // products P V issued; tiles taken from the cleaning warp
+            // step j: P V of tile j - 1, then the scores of tile j
+#pragma unroll 1
+            for (int j = 0; j <= n && ok; ++j) {
+                const int ik = 2 * j, iv = 2 * j - 1;
+                const int sk = ik % SL, sv = (iv + SL) % SL;  // slots of K_j, V_{j-1}
+                const int k0 = kt.first(j), v0 = kt.first(j - 1);
+                if (j > 0) {
+                    if (cut(v0)) ok = wait(clean, cleaned++ & 1, err, kErrMma);
+                    if (ok) ok = wait(&full[sv], (iv / SL) & 1, err, kErrMma);
+                }
+                if (ok && j < n) ok = wait(&full[sk], (ik / SL) & 1, err, kErrMma);
+                if (ok && j > 0 && active(t, v0)) {
+                    const uint32_t v = kv + sv * C::kTileBytes;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        if (ok) ok = wait(&pfull[2 * t + half], done & 1, err, kErrMma);
+                        ptx::tc_fence_after();
+#pragma unroll
+                        for (int kk = half * 4; kk < half * 4 + 4; ++kk)
+                            if (ok)
+                                ptx::umma_f16_ts(to, ts + kk * 8, ptx::umma_desc_sw128_mn(v + kk * 2048, kBlock, 1024), idesc_o,
+                                                 done > 0 || kk > 0 ? 1u : 0u);
+                    }
+                    ++done;
+                }
+                if (j > 0) ptx::umma_commit(&empty[sv]);
+                if (ok && j < n) {
+                    if (active(t, k0)) {
+                        ptx::mbar_arrive(&sfull[t]);  // passes on what the loading warp wrote before `full`
+                        const uint32_t k = kv + sk * C::kTileBytes;
+#pragma unroll
+                        for (int kk = 0; kk < DP / 16; ++kk) {
+                            const uint32_t off = (kk >> 2) * kBlock + (kk & 3) * 32;
+                            ptx::umma_f16(ts, ptx::umma_desc_sw128(q + off), ptx::umma_desc_sw128(k + off), idesc_s, kk > 0 ? 1u : 0u);
+                        }
+                        ptx::umma_commit(&sfull[t]);
+                    }
+                    ptx::umma_commit(&empty[sk]);
+                    if (cut(k0)) {
+                        ok = wait(&full[(ik + 1) % SL], ((ik + 1) / SL) & 1, err, kErrMma);
+                        ptx::mbar_arrive(dirty);
+                    }
+                }
+            }
+            ptx::umma_commit(&ofull[t]);
         }
-        if (lane == 0) ptx::umma_commit(ofull);
         __syncwarp();
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         // ------------------------------------------------ softmax of row tile t, a row a thread
         const int t = warp >> 2, tid = threadIdx.x & 127;
         {
-            // the tile's query rows, 16 bytes a thread, into the swizzled operand layout
+            // the tile's query rows, 16 bytes a thread and copy, into the swizzled operand layout
+            constexpr int kStep = 128 / CH;  // rows between a thread's chunks
             const uint32_t dst = ptx::smem_u32(smem + t * C::kTileBytes);
-#pragma unroll 4
-            for (int i = tid; i < kTileRows * CH; i += 128) {
-                const int r = i / CH, c = i % CH, row = row0 + t * kTileRows + r;
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (row < rows && c * 8 < a.pages.dim)
-                    x = *reinterpret_cast<const uint4*>(a.q + (sq.t0 + row / a.group) * a.q_token +
-                                                        (h * a.group + row % a.group) * a.q_head + c * 8);
-                ptx::st_shared_v4(dst + (c >> 3) * kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4), x);
+            const int r0 = tid / CH, c = tid % CH, left = rows - row0 - t * kTileRows;  // rows of this tile
+            const bool in = c * 8 < a.pages.dim;
+            int token = (row0 + t * kTileRows + r0) / a.group, g = row0 + t * kTileRows + r0 - token * a.group;
+            const int dt = kStep / a.group, dg = kStep - dt * a.group;
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const int r = r0 + i * kStep;
+                const bool ok = in && r < left;
+                const uint16_t* src = ok ? a.q + (sq.t0 + token) * a.q_token + (h * a.group + g) * a.q_head + c * 8 : a.q;
+                cp_async16(dst + (c >> 3) * kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4), src, ok ? 16u : 0u);
+                token += dt;
+                g += dg;
+                if (g >= a.group) {
+                    g -= a.group;
+                    ++token;
+                }
             }
+            cp_async_wait_all();
             ptx::fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(qfull);
+            if (lane == 0) ptx::mbar_arrive(&qfull[t]);
         }
         const int row = row0 + t * kTileRows + tid;
         const bool live_row = row < rows;
         const int p = live_row ? max(-1, sq.p0 + row / a.group) : -1;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + C::kS + t * 128 + lanes, to = tmem + C::kO + t * 128 + lanes;
-        const int page_size = 1 << a.pages.page_shift;
-        const int step = min(page_size, kTileKeys), steps = kTileKeys / step;
-        const int32_t* table = a.seqs.tables + b * a.seqs.table_stride;
+        const int step_shift = min(a.pages.page_shift, 7);
         const float sc = a.scale_log2;
         float m = -INFINITY, l = 0.f;  // m in units of the unscaled score
         int seen = 0;
         bool ok = true;
-        // which pages of a tile are pages, one a lane; looked up a tile ahead
-        auto page_ok = [&](int j) {
-            bool good = true;
-            if (j < n && lane < steps) {
-                const int key = kt.first(j) + lane * step;
-                if (key <= last) {
-                    const int x = table[key >> a.pages.page_shift];
-                    good = x >= 0 && x < a.pages.num_pages;
-                }
-            }
-            return good;
-        };
-        bool good = page_ok(0);
+#pragma unroll 1
         for (int j = 0; j < n; ++j) {
-            const bool good_now = good;
-            good = page_ok(j + 1);
             const int k0 = kt.first(j);
             if (!active(t, k0)) continue;
             if (!warp_wait(&sfull[t], seen & 1, err, kErrSoftmax)) {
@@ -368,31 +503,37 @@ __global__ void __launch_bounds__(kThreads, 1)
                 break;
             }
             ptx::tc_fence_after();
+            const uint32_t no_page = bad[j & 7];
             uint32_t s[kTileKeys];
 #pragma unroll
             for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, s + c * 32);
             ptx::tmem_ld_wait();
-            const uint32_t pages = __ballot_sync(0xffffffffu, good_now);
-            const bool whole = pages == 0xffffffffu && k0 + kTileKeys - 1 <= p_lo[t] &&
+            const bool whole = no_page == 0 && k0 + kTileKeys - 1 <= p_lo[t] &&
                                (a.window == 0 || p_hi[t] - k0 < a.window || k0 + kTileKeys <= a.sinks);
             if (!whole) {
-                // keys k0 + [from, to) of the window, or before `sink`, on pages that are pages
-                const int hi = p - k0, lo = a.window ? hi - a.window : -1, sink = a.sinks - k0;
+                // a bit a key, 32 at a time: up to the row's own, in its window or among the sinks,
+                // on pages that are pages
+                const int hi = p - k0, lo = a.window ? hi - a.window : -1, sink = a.window ? a.sinks - k0 : 0;
 #pragma unroll
-                for (int c = 0; c < kTileKeys; ++c) {
-                    const bool in = c <= hi && (c > lo || a.window == 0 || c < sink);
-                    if (!in) s[c] = 0xff800000u;
-                }
-                if (pages != 0xffffffffu) {
+                for (int c = 0; c < kTileKeys; c += 32) {
+                    uint32_t in = first_bits(hi + 1 - c) & (~first_bits(lo + 1 - c) | first_bits(sink - c));
+                    if (no_page != 0) {
+#pragma unroll 1
+                        for (int e = 0; e < 32; e += 8)
+                            if ((no_page >> ((c + e) >> step_shift)) & 1) in &= ~(0xffu << e);
+                    }
 #pragma unroll
-                    for (int c = 0; c < kTileKeys; ++c)
-                        if (!((pages >> (c / step)) & 1)) s[c] = 0xff800000u;
+                    for (int e = 0; e < 32; ++e)
+                        if (!((in >> e) & 1)) s[c + e] = 0xff800000u;
                 }
             }
-            float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            float x[4];
 #pragma unroll
-            for (int c = 0; c < kTileKeys; ++c) x[c & 3] = fmaxf(x[c & 3], __uint_as_float(s[c]));
-            const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+            for (int c = 0; c < 4; ++c) x[c] = fmaxf(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1]));
+#pragma unroll
+            for (int c = 8; c < kTileKeys; c += 2)
+                x[(c >> 1) & 3] = max3(x[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+            const float top = max3(x[0], x[1], fmaxf(x[2], x[3]));
             if (seen == 0) {
                 m = top;
             } else {
@@ -413,26 +554,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             const float base = m == -INFINITY ? 0.f : m * sc;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < kTileKeys; c += 2) {
-                const float u = exp2_approx(__uint_as_float(s[c]) * sc - base);
-                const float w = exp2_approx(__uint_as_float(s[c + 1]) * sc - base);
-                sum[c & 2] += u;
-                sum[(c & 2) + 1] += w;
-                s[c >> 1] = pack2<BF16>(u, w);
-            }
-            tmem_st32(ts, s);
-            tmem_st32(ts + 32, s + 32);
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            ptx::tmem_st_wait();
-            ptx::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&pfull[t]);
+            l += weights<BF16>(s, sc, base, ts, &pfull[2 * t]);
             ++seen;
         }
         // ------------------------------------------------ epilogue
-        if (ok) ok = warp_wait(ofull, 0, err, kErrEnd);
+        if (ok) ok = warp_wait(&ofull[t], 0, err, kErrEnd);
         ptx::tc_fence_after();
         if (ok) {
             const float inv = l == 0.f ? 0.f : 1.f / l;
