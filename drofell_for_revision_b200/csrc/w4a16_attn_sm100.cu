@@ -57,7 +57,8 @@ struct Cfg {
     static constexpr int kSlots = DP == 128 ? 5 : 8;     // K and V tiles in turn
     static constexpr int kKvOff = 2 * kTileBytes;
     static constexpr int kBarOff = kKvOff + kSlots * kTileBytes;
-    static constexpr int kSmem = kBarOff + 256 + 1024;  // barriers; alignment
+    static constexpr int kListOff = kBarOff + 384;           // barriers and posted items before it
+    static constexpr int kSmem = kListOff + (kThreads + 1) * 4 + 1020;  // and alignment
     static_assert(kSmem <= 227 * 1024, "shared memory budget");
     // TMEM columns: S of both row tiles (P in their first 64), O of both
     static constexpr int kS = 0, kO = 256;
@@ -69,6 +70,14 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
         "[%2];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(ptx::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+            dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(ptx::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
         : "memory");
 }
 
@@ -247,10 +256,61 @@ __device__ __noinline__ void careful_row(const AttnArgs& a, int b, int h, int64_
             make_uint2(pack2<BF16>(o[0] * inv, o[1] * inv), pack2<BF16>(o[2] * inv, o[3] * inv));
 }
 
+// The most items there can be: batch x row pairs x heads, capped well above what is taken.
+int64_t most_items(const AttnArgs& a) {
+    const int64_t rows = static_cast<int64_t>(std::min(a.seqs.max_q, a.seqs.tokens)) * a.group;
+    const int64_t pairs = (rows + 2 * kTileRows - 1) / (2 * kTileRows) * a.pages.heads_kv;
+    return pairs > (int64_t{1} << 31) ? pairs : pairs * a.seqs.batch;
+}
+
+// One unit of work: 256 query rows of one sequence and key-value head.
+struct Item {
+    int b, h, row0;   // sequence, head, first row
+    int rows;         // of the sequence
+    int t0, p0;       // as Seq
+};
+
+// What the warps derive from an item: positions, key tiles, which tiles matter to whom.
+struct View {
+    int p_lo[2], p_hi[2];  // of each row tile's first and last row; p_hi -1: no rows
+    int last;              // position of the last row
+    int first_seen;        // first key of the earliest window
+    int window, sinks;
+    KeyTiles<kTileKeys> kt;
+    __device__ __forceinline__ View(const Item& it, const AttnArgs& a)
+        : last(it.p0 + (min(it.rows, it.row0 + 2 * kTileRows) - 1) / a.group),
+          first_seen(a.window ? max(0, max(it.p0 + it.row0 / a.group, 0) + 1 - a.window) : 0),
+          window(a.window),
+          sinks(a.sinks),
+          kt(it.p0 + it.row0 / a.group, last, a.window, a.sinks) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int r0 = it.row0 + t * kTileRows, r1 = min(it.rows, r0 + kTileRows) - 1;
+            p_lo[t] = it.p0 + r0 / a.group;
+            p_hi[t] = r0 < it.rows ? it.p0 + r1 / a.group : -1;
+        }
+    }
+    // Whether the 128 keys from k0 hold some that no row sees: behind the length or before the
+    // window. What lies there is anybody's, and 0 x NaN would reach every row.
+    __device__ __forceinline__ bool cut(int k0) const {
+        return k0 + kTileKeys - 1 > last || (k0 < first_seen && k0 + kTileKeys > sinks);
+    }
+    // Whether any row of row tile t sees any key of the 128 from k0.
+    __device__ __forceinline__ bool active(int t, int k0) const {
+        return k0 <= p_hi[t] && (window == 0 || k0 + kTileKeys - 1 > max(p_lo[t], 0) - window || k0 < sinks);
+    }
+};
+
+// Items of sequence b: its row pairs, those that see most keys first, over the heads.
+__device__ __forceinline__ int64_t items_of(const AttnArgs& a, int b) {
+    const Seq s = load_seq(a.seqs, a.pages.page_shift, b);
+    return static_cast<int64_t>((s.nq * a.group + 2 * kTileRows - 1) / (2 * kTileRows)) * a.pages.heads_kv;
+}
+
 template <int DP, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                  const __grid_constant__ AttnArgs a) {
+                  const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ AttnArgs a, const int q_by_tma) {
     using C = Cfg<DP>;
     constexpr int CH = DP / 8;
     constexpr int SL = C::kSlots;
@@ -258,61 +318,62 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
     uint64_t* empty = full + SL;
-    uint64_t* qfull = empty + SL;  // [2] the query rows are in place
-    uint64_t* sfull = qfull + 2;   // [2] S of a row tile is complete (and all products before it)
-    uint64_t* pfull = sfull + 2;  // [2][2] half of P is written (the first: O rescaled)
-    uint64_t* ofull = pfull + 4;  // [2] all products are complete
-    uint64_t* dirty = ofull + 2;  // V of a tile that the mask cuts is loaded
-    uint64_t* clean = dirty + 1;  // and holds zeros where no row sees
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(clean + 1);
-    volatile uint32_t* bad = tmem_slot + 1;  // [8] boxes of tile j % 8 whose page id is no page
+    uint64_t* qfull = empty + SL;   // the query rows are in place
+    uint64_t* qempty = qfull + 1;   // and all scores of them are made
+    uint64_t* sfull = qempty + 1;   // [2] S of a row tile is complete (and all products before it)
+    uint64_t* pfull = sfull + 2;    // [2][2] half of P is written (the first: O rescaled)
+    uint64_t* ofull = pfull + 4;    // [2] all products of a row tile are complete
+    uint64_t* dirty = ofull + 2;    // V of a tile that the mask cuts is loaded
+    uint64_t* clean = dirty + 1;    // and holds zeros where no row sees
+    uint64_t* ifull = clean + 1;    // [2] an item is posted
+    uint64_t* iempty = ifull + 2;   // [2] and was read by all
+    uint64_t* turn = iempty + 2;    // [2] a row tile's turn at the tensor cores
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + 2);
+    volatile uint32_t* bad = tmem_slot + 1;                         // [8] boxes of tile j % 8 whose page id is no page
+    volatile int* posted = reinterpret_cast<volatile int*>(bad + 8);  // [2][8] items; b = -1: no more
+    int* before = reinterpret_cast<int*>(smem + C::kListOff);       // [kThreads + 1] items before a thread's sequences
 
     ptx::grid_dep_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int h = blockIdx.x, b = blockIdx.z;
-    const int pair = gridDim.y - 1 - blockIdx.y;  // the rows that see most keys first
-    const Seq sq = load_seq(a.seqs, a.pages.page_shift, b);
-    const int rows = sq.nq * a.group;
-    const int row0 = pair * 2 * kTileRows;
-    if (row0 >= rows) return;
-    const int row_end = min(rows, row0 + 2 * kTileRows);
-    // positions of each row tile's first and last row
-    int p_lo[2], p_hi[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const int r0 = row0 + t * kTileRows, r1 = min(rows, r0 + kTileRows) - 1;
-        p_lo[t] = sq.p0 + r0 / a.group;
-        p_hi[t] = r0 < rows ? sq.p0 + r1 / a.group : -1;  // -1: no rows
-    }
-    const int last = sq.p0 + (row_end - 1) / a.group;
-    const KeyTiles<kTileKeys> kt(p_lo[0], last, a.window, a.sinks);
-    const int n = kt.count;
-    const int first_seen = a.window ? max(0, max(p_lo[0], 0) + 1 - a.window) : 0;  // of the window, any row
-    // whether the 128 keys from k0 hold some that no row sees: behind the length or before the
-    // window. What lies there is anybody's, and 0 x NaN would reach every row.
-    auto cut = [&](int k0) { return k0 + kTileKeys - 1 > last || (k0 < first_seen && k0 + kTileKeys > a.sinks); };
-    // whether any row of row tile t sees any key of the 128 from k0
-    auto active = [&](int t, int k0) {
-        return k0 <= p_hi[t] && (a.window == 0 || k0 + kTileKeys - 1 > max(p_lo[t], 0) - a.window || k0 < a.sinks);
-    };
 
+    // ---- how many items come before each thread's share of the sequences
+    const int per = (a.seqs.batch + kThreads - 1) / kThreads;
+    {
+        const int b0 = min(a.seqs.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.seqs.batch, b0 + per);
+        int64_t mine = 0;
+        for (int b = b0; b < b1; ++b) mine += items_of(a, b);
+        // the host has made sure that the items of all sequences fit 31 bits
+        int sum = static_cast<int>(mine);
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += o;
+        }
+        before[threadIdx.x + 1] = sum;
+        if (threadIdx.x == 0) before[0] = 0;
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < SL; ++s) {
             ptx::mbar_init(&full[s], 1);
             ptx::mbar_init(&empty[s], 2);
         }
+        ptx::mbar_init(qfull, 1);
+        ptx::mbar_init(qempty, 2);
         for (int t = 0; t < 2; ++t) {
-            ptx::mbar_init(&qfull[t], 4);
             ptx::mbar_init(&ofull[t], 1);
             ptx::mbar_init(&sfull[t], 2);
             ptx::mbar_init(&pfull[2 * t], 4);
             ptx::mbar_init(&pfull[2 * t + 1], 4);
+            ptx::mbar_init(&ifull[t], 1);
+            ptx::mbar_init(&iempty[t], 11);
+            ptx::mbar_init(&turn[t], 1);
         }
         ptx::mbar_init(dirty, 2);
         ptx::mbar_init(clean, 1);
         ptx::fence_mbar_init();
         ptx::prefetch_tmap(&tm_k);
         ptx::prefetch_tmap(&tm_v);
+        if (q_by_tma) ptx::prefetch_tmap(&tm_q);
     }
     if (warp == kMmaWarp) {
         ptx::tmem_alloc(tmem_slot, 512);
@@ -320,81 +381,211 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     ptx::tc_fence_before();
     __syncthreads();
+    if (warp == kLoadWarp) {  // the warps' sums into one running sum
+        int base = 0;
+#pragma unroll 1
+        for (int w = 0; w < kThreads / 32; ++w) {
+            const int x = before[w * 32 + lane + 1] + base;
+            __syncwarp();
+            before[w * 32 + lane + 1] = x;
+            base = __shfl_sync(0xffffffffu, x, 31);
+        }
+    }
     ptx::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     int* err = &g_attention_error;
 
+    // Item k of this CTA as the loading warp posted it; false: there is none (or a wait gave up).
+    auto next_item = [&](int k, Item& it, bool whole_warp) {
+        const int s = k & 1, parity = (k >> 1) & 1;
+        bool ok = wait(&ifull[s], parity, err, kErrLoad);
+        if (whole_warp) ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return false;
+        it.b = posted[s * 8];
+        it.h = posted[s * 8 + 1];
+        it.row0 = posted[s * 8 + 2];
+        it.rows = posted[s * 8 + 3];
+        it.t0 = posted[s * 8 + 4];
+        it.p0 = posted[s * 8 + 5];
+        if (whole_warp) __syncwarp();
+        if (!whole_warp || lane == 0) ptx::mbar_arrive(&iempty[s]);
+        return it.b >= 0;
+    };
+
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         if (warp == kLoadWarp) {
-            // ------------------------------------------------ K and V, page by page
+            // ------------------------------------------------ items; Q; K and V, page by page
             const int page_size = 1 << a.pages.page_shift;
             const int box = min(page_size, kTileKeys);
             const int boxes = kTileKeys / box;  // per tile, at most 16: one a lane
-            const int32_t* table = a.seqs.tables + b * a.seqs.table_stride;
-            auto page_of = [&](int j) {  // this lane's page of key tile j
-                int page = a.pages.num_pages;  // behind the cache's end: zeros
-                if (j < n && lane < boxes) {
-                    const int key = kt.first(j) + lane * box;
-                    if (key <= last) page = table[key >> a.pages.page_shift];
-                }
-                return page;
-            };
-            int issued = 0;
+            __syncwarp();
+            const int total = before[kThreads];
+            const int ctas = gridDim.x;
+            int i = 0, q_loads = 0;  // tiles of K and V, row pairs of Q so far
             bool ok = true;
-            int page = page_of(0);
 #pragma unroll 1
-            for (int j = 0; j < n && ok; ++j) {
-                const int key = kt.first(j) + lane * box;
-                const int next = page_of(j + 1);
-                const bool none = page < 0 || page >= a.pages.num_pages;
-                const uint32_t none_of = __ballot_sync(0xffffffffu, none && lane < boxes && key <= last);
-                if (none) page = a.pages.num_pages;
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    const int i = 2 * j + w, s = i % SL;
-                    if (i >= SL) ok = warp_wait(&empty[s], ((i / SL) - 1) & 1, err, kErrLoad);
-                    if (!ok) break;
-                    if (lane == 0) {
-                        if (w == 0) bad[j & 7] = none_of;
-                        ptx::mbar_arrive_expect_tx(&full[s], C::kTileBytes);
+            for (int k = 0; ok; ++k) {
+                // rounds of the CTAs run forth and back over the items, whose work falls along a
+                // sequence: a CTA's shares even out
+                const int64_t at = static_cast<int64_t>(k) * ctas + ((k & 1) ? ctas - 1 - static_cast<int>(blockIdx.x) : blockIdx.x);
+                Item it;
+                it.b = -1;
+                it.h = it.row0 = it.rows = it.t0 = it.p0 = 0;
+                if (at < total) {
+                    int lo = 0, hi = kThreads;  // before[lo] <= at < before[hi]
+                    while (hi - lo > 1) {
+                        const int mid = (lo + hi) >> 1;
+                        if (before[mid] <= at) {
+                            lo = mid;
+                        } else {
+                            hi = mid;
+                        }
                     }
-                    __syncwarp();
-                    if (lane < boxes) {
-                        const uint32_t dst = ptx::smem_u32(smem + C::kKvOff + s * C::kTileBytes) + lane * box * 128;
-#pragma unroll
-                        for (int d = 0; d < C::kBlocks; ++d)
-                            tma_load_4d(dst + d * kBlock, w ? &tm_v : &tm_k, &full[s], d * 64, key & (page_size - 1), h, page);
+                    int rest = static_cast<int>(at) - before[lo], b = lo * per;
+                    for (;; ++b) {
+                        const int n = static_cast<int>(items_of(a, b));
+                        if (rest < n) break;
+                        rest -= n;
                     }
-                    ++issued;
+                    const Seq sq = load_seq(a.seqs, a.pages.page_shift, b);
+                    const int pairs = (sq.nq * a.group + 2 * kTileRows - 1) / (2 * kTileRows);
+                    it.b = b;
+                    it.row0 = (pairs - 1 - rest / a.pages.heads_kv) * 2 * kTileRows;
+                    it.h = rest % a.pages.heads_kv;
+                    it.rows = sq.nq * a.group;
+                    it.t0 = sq.t0;
+                    it.p0 = sq.p0;
                 }
-                page = next;
+                const int s = k & 1;
+                if (k >= 2) ok = warp_wait(&iempty[s], ((k >> 1) - 1) & 1, err, kErrLoad);
+                if (lane == 0) {
+                    posted[s * 8] = ok ? it.b : -1;
+                    posted[s * 8 + 1] = it.h;
+                    posted[s * 8 + 2] = it.row0;
+                    posted[s * 8 + 3] = it.rows;
+                    posted[s * 8 + 4] = it.t0;
+                    posted[s * 8 + 5] = it.p0;
+                    ptx::mbar_arrive(&ifull[s]);
+                }
+                if (it.b < 0 || !ok) break;
+                const View vw(it, a);
+                const int n = vw.kt.count;
+                const int32_t* table = a.seqs.tables + it.b * a.seqs.table_stride;
+                auto page_of = [&](int j) {  // this lane's page of key tile j
+                    int page = a.pages.num_pages;  // behind the cache's end: zeros
+                    if (j < n && lane < boxes) {
+                        const int key = vw.kt.first(j) + lane * box;
+                        if (key <= vw.last) page = table[key >> a.pages.page_shift];
+                    }
+                    return page;
+                };
+                int page = page_of(0);
+#pragma unroll 1
+                for (int j = 0; j < n && ok; ++j) {
+                    const int key = vw.kt.first(j) + lane * box;
+                    const int next = page_of(j + 1);
+                    const bool none = page < 0 || page >= a.pages.num_pages;
+                    const uint32_t none_of = __ballot_sync(0xffffffffu, none && lane < boxes && key <= vw.last);
+                    if (none) page = a.pages.num_pages;
+#pragma unroll 1
+                    for (int w = 0; w < 2; ++w, ++i) {
+                        const int sl = i % SL;
+                        if (i >= SL) ok = warp_wait(&empty[sl], ((i / SL) - 1) & 1, err, kErrLoad);
+                        if (!ok) break;
+                        if (lane == 0) {
+                            if (w == 0) bad[(i >> 1) & 7] = none_of;
+                            ptx::mbar_arrive_expect_tx(&full[sl], C::kTileBytes);
+                        }
+                        __syncwarp();
+                        if (lane < boxes) {
+                            const uint32_t dst = ptx::smem_u32(smem + C::kKvOff + sl * C::kTileBytes) + lane * box * 128;
+#pragma unroll
+                            for (int d = 0; d < C::kBlocks; ++d)
+                                tma_load_4d(dst + d * kBlock, w ? &tm_v : &tm_k, &full[sl], d * 64, key & (page_size - 1), it.h,
+                                            page);
+                        }
+                    }
+                    page = next;
+                    if (j == 0 && ok && q_by_tma) {
+                        // after the first keys: the rows of the last item may still be in use
+                        if (k > 0) ok = warp_wait(qempty, (k - 1) & 1, err, kErrLoad);
+                        if (ok && lane == 0) {
+                            ptx::mbar_arrive_expect_tx(qfull, 2 * C::kTileBytes);
+                            const int tokens = kTileRows / a.group, token = it.t0 + it.row0 / a.group;
+                            for (int x = 0; x < 2 * C::kBlocks; ++x)
+                                tma_load_3d(ptx::smem_u32(smem) + x * kBlock, &tm_q, qfull, (x % C::kBlocks) * 64, it.h * a.group,
+                                            token + (x / C::kBlocks) * tokens);
+                        }
+                        if (ok) ++q_loads;
+                    }
+                }
+                // an item without keys takes no Q: its phases pass all the same
+                if (n == 0 && ok && q_by_tma) {
+                    if (k > 0) ok = warp_wait(qempty, (k - 1) & 1, err, kErrLoad);
+                    if (ok && lane == 0) ptx::mbar_arrive(qfull);
+                    if (ok) ++q_loads;
+                }
             }
             // no copy may be in flight when the CTA ends
 #pragma unroll 1
-            for (int i = max(0, issued - SL); i < issued; ++i)
-                warp_wait(&full[i % SL], (i / SL) & 1, err, kErrLoad);
+            for (int x = max(0, i - SL); x < i; ++x) warp_wait(&full[x % SL], (x / SL) & 1, err, kErrLoad);
+            if (q_loads > 0) warp_wait(qfull, (q_loads - 1) & 1, err, kErrLoad);
         } else if (warp == kCleanWarp) {
-            // ------------------------------------------------ zeros into V where no row sees
-            // asked for by both MMA threads, one tile at a time (a barrier's parity tells only two
-            // phases apart: a warp that skips tiles cannot wait on `full`)
+            // ------------------------------------------------ zeros into V where no row sees; Q, where a
+            // group of heads does not divide a row tile
+            int i = 0, asked = 0;
             bool ok = true;
-            int asked = 0;
+            Item it;
 #pragma unroll 1
-            for (int j = 0; j < n && ok; ++j) {
-                const int k0 = kt.first(j), s = (2 * j + 1) % SL;
-                if (!cut(k0)) continue;
-                ok = warp_wait(dirty, asked++ & 1, err, kErrMma);
-                const uint32_t v = ptx::smem_u32(smem + C::kKvOff + s * C::kTileBytes);
-#pragma unroll 1
-                for (int x = lane; ok && x < kTileKeys * CH; x += 32) {
-                    const int r = x / CH, c = x % CH, key = k0 + r;
-                    if (key > last || (key < first_seen && key >= a.sinks))
-                        ptx::st_shared_v4(v + (c >> 3) * kBlock + r * 128 + (c & 7) * 16, make_uint4(0, 0, 0, 0));
+            for (int k = 0; ok && next_item(k, it, true); ++k) {
+                const View vw(it, a);
+                const int n = vw.kt.count;
+                if (!q_by_tma) {
+                    if (k > 0) ok = warp_wait(qempty, (k - 1) & 1, err, kErrMma);
+                    if (!ok) break;
+                    // 16 bytes a lane and copy, into the swizzled operand layout
+                    constexpr int kStep = 32 / CH;  // rows between a lane's chunks
+                    const uint32_t dst = ptx::smem_u32(smem);
+                    const int c = lane % CH, left = it.rows - it.row0;  // rows of this item
+                    int r = lane / CH, token = (it.row0 + r) / a.group, g = it.row0 + r - token * a.group;
+#pragma unroll 2
+                    for (; r < 2 * kTileRows; r += kStep) {
+                        const bool in = c * 8 < a.pages.dim && r < left && n > 0;
+                        const uint16_t* src =
+                            in ? a.q + (it.t0 + token) * a.q_token + (it.h * a.group + g) * a.q_head + c * 8 : a.q;
+                        cp_async16(dst + (r >> 7) * C::kTileBytes + (c >> 3) * kBlock + (r & 127) * 128 +
+                                       (((c & 7) ^ (r & 7)) << 4),
+                                   src, in ? 16u : 0u);
+                        g += kStep;
+                        while (g >= a.group) {
+                            g -= a.group;
+                            ++token;
+                        }
+                    }
+                    cp_async_wait_all();
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(qfull);
                 }
-                ptx::fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(clean);
+                // asked for by both MMA threads, one tile at a time (a barrier's parity tells only two
+                // phases apart: a warp that skips tiles cannot wait on `full`)
+#pragma unroll 1
+                for (int j = 0; j < n && ok; ++j, i += 2) {
+                    const int k0 = vw.kt.first(j);
+                    if (!vw.cut(k0)) continue;
+                    ok = warp_wait(dirty, asked++ & 1, err, kErrMma);
+                    const uint32_t v = ptx::smem_u32(smem + C::kKvOff + ((i + 1) % SL) * C::kTileBytes);
+#pragma unroll 1
+                    for (int x = lane; ok && x < kTileKeys * CH; x += 32) {
+                        const int r = x / CH, c = x % CH, key = k0 + r;
+                        if (key > vw.last || (key < vw.first_seen && key >= a.sinks))
+                            ptx::st_shared_v4(v + (c >> 3) * kBlock + r * 128 + (c & 7) * 16, make_uint4(0, 0, 0, 0));
+                    }
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(clean);
+                }
             }
         } else if (ptx::elect_one_sync()) {
             // ------------------------------------------------ MMA issuer of row tile t: one elected thread,
@@ -405,169 +596,179 @@ __global__ void __launch_bounds__(kThreads, 1)
             constexpr uint32_t idesc_o = ptx::umma_idesc_f16(kTileRows, DP, BF16) | (1u << 16);  // B = V is MN-major
             const uint32_t ts = tmem + C::kS + t * 128, to = tmem + C::kO + t * 128;
             const uint32_t q = ptx::smem_u32(smem) + t * C::kTileBytes, kv = ptx::smem_u32(smem + C::kKvOff);
-            bool ok = wait(&qfull[t], 0, err, kErrMma);
-            int done = 0, cleaned = 0;  // products P V issued; tiles taken from the cleaning warp
-            // step j: P V of tile j - 1, then the scores of tile j
+            int i = 0, done = 0, cleaned = 0;  // tiles of K and V, products P V, tiles taken from the cleaning warp
+            int turns = 0;
+            bool ok = true;
+            auto my_turn = [&]() {  // row tile 0 has the first
+                const int x = turns++ - (t == 0 ? 1 : 0);
+                return x < 0 || wait(&turn[t], x & 1, err, kErrMma);
+            };
+            Item it;
 #pragma unroll 1
-            for (int j = 0; j <= n && ok; ++j) {
-                const int ik = 2 * j, iv = 2 * j - 1;
-                const int sk = ik % SL, sv = (iv + SL) % SL;  // slots of K_j, V_{j-1}
-                const int k0 = kt.first(j), v0 = kt.first(j - 1);
-                if (j > 0) {
-                    if (cut(v0)) ok = wait(clean, cleaned++ & 1, err, kErrMma);
-                    if (ok) ok = wait(&full[sv], (iv / SL) & 1, err, kErrMma);
-                }
-                if (ok && j < n) ok = wait(&full[sk], (ik / SL) & 1, err, kErrMma);
-                if (ok && j > 0 && active(t, v0)) {
+            for (int k = 0; ok && next_item(k, it, false); ++k) {
+                const View vw(it, a);
+                const int n = vw.kt.count;
+                ok = wait(qfull, k & 1, err, kErrMma);
+                bool first = true;
+                // step j: P V of tile j - 1, then the scores of tile j
+#pragma unroll 1
+                for (int j = 0; j <= n && ok; ++j, i += 2) {
+                    const int iv = i - 1;                            // of V_{j-1}; K_j is i
+                    const int sk = i % SL, sv = (iv + SL) % SL;
+                    const int k0 = vw.kt.first(j), v0 = vw.kt.first(j - 1);
+                    if (j > 0) {
+                        if (vw.cut(v0)) ok = wait(clean, cleaned++ & 1, err, kErrMma);
+                        if (ok) ok = wait(&full[sv], (iv / SL) & 1, err, kErrMma);
+                    }
+                    if (ok && j < n) ok = wait(&full[sk], (i / SL) & 1, err, kErrMma);
+                    // the first half of P V whenever P is there; the second half and the next scores in
+                    // turn with the other row tile: left to interleave, both end together, and then both
+                    // softmaxes run at once while the tensor cores idle (4700 cycles a tile, 3200 in turn)
+                    const bool product = j > 0 && vw.active(t, v0);
                     const uint32_t v = kv + sv * C::kTileBytes;
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
+                    auto half_product = [&](int half) {
                         if (ok) ok = wait(&pfull[2 * t + half], done & 1, err, kErrMma);
                         ptx::tc_fence_after();
+                        if (half == 1 && ok) ok = my_turn();
 #pragma unroll
                         for (int kk = half * 4; kk < half * 4 + 4; ++kk)
                             if (ok)
                                 ptx::umma_f16_ts(to, ts + kk * 8, ptx::umma_desc_sw128_mn(v + kk * 2048, kBlock, 1024), idesc_o,
-                                                 done > 0 || kk > 0 ? 1u : 0u);
+                                                 !first || kk > 0 ? 1u : 0u);
+                    };
+                    if (ok && product) {
+                        half_product(0);
+                        half_product(1);
+                        ++done;
+                        first = false;
+                    } else if (ok) {
+                        ok = my_turn();
                     }
-                    ++done;
-                }
-                if (j > 0) ptx::umma_commit(&empty[sv]);
-                if (ok && j < n) {
-                    if (active(t, k0)) {
-                        ptx::mbar_arrive(&sfull[t]);  // passes on what the loading warp wrote before `full`
-                        const uint32_t k = kv + sk * C::kTileBytes;
+                    if (j > 0) ptx::umma_commit(&empty[sv]);
+                    if (ok && j < n) {
+                        if (vw.active(t, k0)) {
+                            ptx::mbar_arrive(&sfull[t]);  // passes on what the loading warp wrote before `full`
+                            const uint32_t kd = kv + sk * C::kTileBytes;
 #pragma unroll
-                        for (int kk = 0; kk < DP / 16; ++kk) {
-                            const uint32_t off = (kk >> 2) * kBlock + (kk & 3) * 32;
-                            ptx::umma_f16(ts, ptx::umma_desc_sw128(q + off), ptx::umma_desc_sw128(k + off), idesc_s, kk > 0 ? 1u : 0u);
+                            for (int kk = 0; kk < DP / 16; ++kk) {
+                                const uint32_t off = (kk >> 2) * kBlock + (kk & 3) * 32;
+                                ptx::umma_f16(ts, ptx::umma_desc_sw128(q + off), ptx::umma_desc_sw128(kd + off), idesc_s,
+                                              kk > 0 ? 1u : 0u);
+                            }
+                            ptx::umma_commit(&sfull[t]);
                         }
-                        ptx::umma_commit(&sfull[t]);
-                    }
-                    ptx::umma_commit(&empty[sk]);
-                    if (cut(k0)) {
-                        ok = wait(&full[(ik + 1) % SL], ((ik + 1) / SL) & 1, err, kErrMma);
-                        ptx::mbar_arrive(dirty);
+                        ptx::umma_commit(&empty[sk]);
+                        ptx::mbar_arrive(&turn[t ^ 1]);
+                        if (j == n - 1) ptx::umma_commit(qempty);
+                        if (vw.cut(k0)) {
+                            ok = wait(&full[(i + 1) % SL], ((i + 1) / SL) & 1, err, kErrMma);
+                            ptx::mbar_arrive(dirty);
+                        }
+                    } else if (ok) {
+                        ptx::mbar_arrive(&turn[t ^ 1]);
                     }
                 }
+                i -= 2;  // step n has no K
+                if (n == 0) ptx::umma_commit(qempty);
+                ptx::umma_commit(&ofull[t]);
             }
-            ptx::umma_commit(&ofull[t]);
         }
         __syncwarp();
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         // ------------------------------------------------ softmax of row tile t, a row a thread
         const int t = warp >> 2, tid = threadIdx.x & 127;
-        {
-            // the tile's query rows, 16 bytes a thread and copy, into the swizzled operand layout
-            constexpr int kStep = 128 / CH;  // rows between a thread's chunks
-            const uint32_t dst = ptx::smem_u32(smem + t * C::kTileBytes);
-            const int r0 = tid / CH, c = tid % CH, left = rows - row0 - t * kTileRows;  // rows of this tile
-            const bool in = c * 8 < a.pages.dim;
-            int token = (row0 + t * kTileRows + r0) / a.group, g = row0 + t * kTileRows + r0 - token * a.group;
-            const int dt = kStep / a.group, dg = kStep - dt * a.group;
-#pragma unroll
-            for (int i = 0; i < CH; ++i) {
-                const int r = r0 + i * kStep;
-                const bool ok = in && r < left;
-                const uint16_t* src = ok ? a.q + (sq.t0 + token) * a.q_token + (h * a.group + g) * a.q_head + c * 8 : a.q;
-                cp_async16(dst + (c >> 3) * kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4), src, ok ? 16u : 0u);
-                token += dt;
-                g += dg;
-                if (g >= a.group) {
-                    g -= a.group;
-                    ++token;
-                }
-            }
-            cp_async_wait_all();
-            ptx::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&qfull[t]);
-        }
-        const int row = row0 + t * kTileRows + tid;
-        const bool live_row = row < rows;
-        const int p = live_row ? max(-1, sq.p0 + row / a.group) : -1;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + C::kS + t * 128 + lanes, to = tmem + C::kO + t * 128 + lanes;
         const int step_shift = min(a.pages.page_shift, 7);
         const float sc = a.scale_log2;
-        float m = -INFINITY, l = 0.f;  // m in units of the unscaled score
-        int seen = 0;
+        int i = 0, seen = 0;  // tiles of keys; scores taken
         bool ok = true;
+        Item it;
 #pragma unroll 1
-        for (int j = 0; j < n; ++j) {
-            const int k0 = kt.first(j);
-            if (!active(t, k0)) continue;
-            if (!warp_wait(&sfull[t], seen & 1, err, kErrSoftmax)) {
-                ok = false;
-                break;
+        for (int k = 0; ok && next_item(k, it, true); ++k) {
+            const View vw(it, a);
+            const int n = vw.kt.count;
+            const int row = it.row0 + t * kTileRows + tid;
+            const bool live_row = row < it.rows;
+            const int p = live_row ? max(-1, it.p0 + row / a.group) : -1;
+            float m = -INFINITY, l = 0.f;  // m in units of the unscaled score
+            bool first = true;
+#pragma unroll 1
+            for (int j = 0; j < n; ++j, ++i) {
+                const int k0 = vw.kt.first(j);
+                if (!vw.active(t, k0)) continue;
+                if (!warp_wait(&sfull[t], seen & 1, err, kErrSoftmax)) {
+                    ok = false;
+                    break;
+                }
+                ptx::tc_fence_after();
+                const uint32_t no_page = bad[i & 7];
+                uint32_t s[kTileKeys];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, s + c * 32);
+                ptx::tmem_ld_wait();
+                const bool whole = no_page == 0 && k0 + kTileKeys - 1 <= vw.p_lo[t] &&
+                                   (a.window == 0 || vw.p_hi[t] - k0 < a.window || k0 + kTileKeys <= a.sinks);
+                if (!whole) {
+                    // a bit a key, 32 at a time: up to the row's own, in its window or among the sinks,
+                    // on pages that are pages
+                    const int hi = p - k0, lo = a.window ? hi - a.window : -1, sink = a.window ? a.sinks - k0 : 0;
+#pragma unroll
+                    for (int c = 0; c < kTileKeys; c += 32) {
+                        uint32_t in = first_bits(hi + 1 - c) & (~first_bits(lo + 1 - c) | first_bits(sink - c));
+                        if (no_page != 0) {
+#pragma unroll 1
+                            for (int e = 0; e < 32; e += 8)
+                                if ((no_page >> ((c + e) >> step_shift)) & 1) in &= ~(0xffu << e);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!((in >> e) & 1)) s[c + e] = 0xff800000u;
+                    }
+                }
+                float x[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) x[c] = fmaxf(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1]));
+#pragma unroll
+                for (int c = 8; c < kTileKeys; c += 2)
+                    x[(c >> 1) & 3] = max3(x[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+                const float top = max3(x[0], x[1], fmaxf(x[2], x[3]));
+                if (first) {
+                    m = top;
+                } else {
+                    const bool grow = (top - m) * sc > kSlack || (m == -INFINITY && top > m);
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float f = grow ? exp2_approx((m - top) * sc) : 1.f;
+                        if (grow) m = top;
+                        l *= f;
+#pragma unroll 1
+                        for (int c = 0; c < DP; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(to + c, o);
+                            ptx::tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st32(to + c, o);
+                        }
+                    }
+                }
+                const float base = m == -INFINITY ? 0.f : m * sc;
+                l += weights<BF16>(s, sc, base, ts, &pfull[2 * t]);
+                ++seen;
+                first = false;
             }
+            // ------------------------------------------------ epilogue
+            if (ok) ok = warp_wait(&ofull[t], k & 1, err, kErrEnd);
+            if (!ok) break;
             ptx::tc_fence_after();
-            const uint32_t no_page = bad[j & 7];
-            uint32_t s[kTileKeys];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, s + c * 32);
-            ptx::tmem_ld_wait();
-            const bool whole = no_page == 0 && k0 + kTileKeys - 1 <= p_lo[t] &&
-                               (a.window == 0 || p_hi[t] - k0 < a.window || k0 + kTileKeys <= a.sinks);
-            if (!whole) {
-                // a bit a key, 32 at a time: up to the row's own, in its window or among the sinks,
-                // on pages that are pages
-                const int hi = p - k0, lo = a.window ? hi - a.window : -1, sink = a.window ? a.sinks - k0 : 0;
-#pragma unroll
-                for (int c = 0; c < kTileKeys; c += 32) {
-                    uint32_t in = first_bits(hi + 1 - c) & (~first_bits(lo + 1 - c) | first_bits(sink - c));
-                    if (no_page != 0) {
-#pragma unroll 1
-                        for (int e = 0; e < 32; e += 8)
-                            if ((no_page >> ((c + e) >> step_shift)) & 1) in &= ~(0xffu << e);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (!((in >> e) & 1)) s[c + e] = 0xff800000u;
-                }
-            }
-            float x[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) x[c] = fmaxf(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1]));
-#pragma unroll
-            for (int c = 8; c < kTileKeys; c += 2)
-                x[(c >> 1) & 3] = max3(x[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-            const float top = max3(x[0], x[1], fmaxf(x[2], x[3]));
-            if (seen == 0) {
-                m = top;
-            } else {
-                const bool grow = (top - m) * sc > kSlack || (m == -INFINITY && top > m);
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float f = grow ? exp2_approx((m - top) * sc) : 1.f;
-                    if (grow) m = top;
-                    l *= f;
-#pragma unroll 1
-                    for (int c = 0; c < DP; c += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(to + c, o);
-                        ptx::tmem_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        tmem_st32(to + c, o);
-                    }
-                }
-            }
-            const float base = m == -INFINITY ? 0.f : m * sc;
-            l += weights<BF16>(s, sc, base, ts, &pfull[2 * t]);
-            ++seen;
-        }
-        // ------------------------------------------------ epilogue
-        if (ok) ok = warp_wait(&ofull[t], 0, err, kErrEnd);
-        ptx::tc_fence_after();
-        if (ok) {
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            const int64_t o_off = (sq.t0 + row / a.group) * a.o_token + (h * a.group + row % a.group) * a.o_head;
+            const int64_t o_off = (it.t0 + row / a.group) * a.o_token + (it.h * a.group + row % a.group) * a.o_head;
             bool odd = false;
 #pragma unroll 1
             for (int c = 0; c < DP; c += 32) {
                 uint32_t o[32];
-                if (seen > 0) {
+                if (!first) {
                     tmem_ld32(to + c, o);
                     ptx::tmem_ld_wait();
                 } else {
@@ -582,8 +783,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int e = 0; e < 32; e += 8) {
                     uint32_t w[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        w[i] = pack2<BF16>(__uint_as_float(o[e + 2 * i]) * inv, __uint_as_float(o[e + 2 * i + 1]) * inv);
+                    for (int y = 0; y < 4; ++y)
+                        w[y] = pack2<BF16>(__uint_as_float(o[e + 2 * y]) * inv, __uint_as_float(o[e + 2 * y + 1]) * inv);
                     if (live_row && c + e < a.pages.dim)
                         *reinterpret_cast<uint4*>(a.out + o_off + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
@@ -593,9 +794,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int r = row - lane + __ffs(again) - 1;
                 again &= again - 1;
                 __syncwarp();
-                careful_row<BF16>(a, b, h, (sq.t0 + r / a.group) * a.q_token + (h * a.group + r % a.group) * a.q_head,
-                                  (sq.t0 + r / a.group) * a.o_token + (h * a.group + r % a.group) * a.o_head,
-                                  sq.p0 + r / a.group);
+                careful_row<BF16>(a, it.b, it.h, (it.t0 + r / a.group) * a.q_token + (it.h * a.group + r % a.group) * a.q_head,
+                                  (it.t0 + r / a.group) * a.o_token + (it.h * a.group + r % a.group) * a.o_head,
+                                  it.p0 + r / a.group);
             }
         }
     }
@@ -609,14 +810,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <int DP, bool BF16>
-cudaError_t launch_prompt_t(const AttnArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t s) {
+cudaError_t launch_prompt_t(const AttnArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const CUtensorMap& tm_q,
+                            bool q_by_tma, int num_sms, cudaStream_t s) {
     auto kern = prompt_kernel<DP, BF16>;
     static std::atomic<uint64_t> ready{0};
     cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), Cfg<DP>::kSmem, ready);
     if (e != cudaSuccess) return e;
-    const int rows = a.seqs.max_q * a.group;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.pages.heads_kv, (rows + 2 * kTileRows - 1) / (2 * kTileRows), a.seqs.batch);
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(num_sms, most_items(a))));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = Cfg<DP>::kSmem;
     cfg.stream = s;
@@ -625,17 +826,14 @@ cudaError_t launch_prompt_t(const AttnArgs& a, const CUtensorMap& tm_k, const CU
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, tm_k, tm_v, a);
+    return cudaLaunchKernelEx(&cfg, kern, tm_k, tm_v, tm_q, a, q_by_tma ? 1 : 0);
 }
 
 }  // namespace
 
-bool prompt_fits(const AttnArgs& a) {
-    const int64_t pairs = (static_cast<int64_t>(a.seqs.max_q) * a.group + 2 * kTileRows - 1) / (2 * kTileRows);
-    return pairs <= 65535 && a.seqs.batch <= 65535;
-}
+bool prompt_fits(const AttnArgs& a) { return most_items(a) <= (1 << 30); }
 
-cudaError_t launch_prompt(const AttnArgs& a, bool bf16, cudaStream_t s) {
+cudaError_t launch_prompt(const AttnArgs& a, bool bf16, int num_sms, cudaStream_t s) {
     const PageView& p = a.pages;
     const uint64_t size = uint64_t{1} << p.page_shift;
     const uint64_t dims[4] = {static_cast<uint64_t>(p.dim), size, static_cast<uint64_t>(p.heads_kv),
@@ -650,8 +848,24 @@ cudaError_t launch_prompt(const AttnArgs& a, bool bf16, cudaStream_t s) {
     if (encode_tmap_4d(&mk, dt, p.k, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B) != CUDA_SUCCESS ||
         encode_tmap_4d(&mv, dt, p.v, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B) != CUDA_SUCCESS)
         return cudaErrorInvalidValue;
-    if (p.dim <= 64) return bf16 ? launch_prompt_t<64, true>(a, mk, mv, s) : launch_prompt_t<64, false>(a, mk, mv, s);
-    return bf16 ? launch_prompt_t<128, true>(a, mk, mv, s) : launch_prompt_t<128, false>(a, mk, mv, s);
+    // Q rows token-major by heads of a group: a box of the group's heads and 128 / group tokens is
+    // a row tile, where the group divides it
+    const bool q_by_tma = kTileRows % a.group == 0 && (a.heads == 1 || a.q_head > 0) && (a.seqs.tokens == 1 || a.q_token > 0);
+    CUtensorMap mq = mk;
+    if (q_by_tma) {
+        const uint64_t qdims[3] = {static_cast<uint64_t>(p.dim), static_cast<uint64_t>(a.heads),
+                                   static_cast<uint64_t>(a.seqs.tokens)};
+        const uint64_t qstrides[2] = {a.heads > 1 ? static_cast<uint64_t>(a.q_head) * 2 : 16,
+                                      a.seqs.tokens > 1 ? static_cast<uint64_t>(a.q_token) * 2 : 16};
+        const uint32_t qbox[3] = {64, static_cast<uint32_t>(a.group), static_cast<uint32_t>(kTileRows / a.group)};
+        if (encode_tmap_3d(&mq, dt, a.q, qdims, qstrides, qbox, CU_TENSOR_MAP_SWIZZLE_128B) != CUDA_SUCCESS)
+            return cudaErrorInvalidValue;
+    }
+    if (p.dim <= 64)
+        return bf16 ? launch_prompt_t<64, true>(a, mk, mv, mq, q_by_tma, num_sms, s)
+                    : launch_prompt_t<64, false>(a, mk, mv, mq, q_by_tma, num_sms, s);
+    return bf16 ? launch_prompt_t<128, true>(a, mk, mv, mq, q_by_tma, num_sms, s)
+                : launch_prompt_t<128, false>(a, mk, mv, mq, q_by_tma, num_sms, s);
 }
 
 cudaError_t read_attention_error(int* out, cudaStream_t s) {

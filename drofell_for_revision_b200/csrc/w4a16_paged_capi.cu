@@ -227,16 +227,14 @@ int w4a16_paged_attention(const w4a16_pages* pages, const w4a16_seqs* seqs, cons
     a.o_token = out->stride_token, a.o_head = out->stride_head;
     a.scale_log2 = scale * 1.4426950408889634f;
     const bool bf16 = pages->dtype == W4A16_DTYPE_BF16;
-    if (takes_prompt(a)) {
-        DeviceGuard guard(pages->device);
-        if (!guard.ok) return report_error(W4A16_ERR_INVALID, "device %d", pages->device);
-        const cudaError_t e = launch_prompt(a, bf16, static_cast<cudaStream_t>(stream));
-        return e == cudaSuccess ? W4A16_OK : cuda_error(e, "paged attention launch");
-    }
     const int sms = sm_count(pages->device);
     if (sms == 0) return report_error(W4A16_ERR_CUDA, "no device %d", pages->device);
     DeviceGuard guard(pages->device);
     if (!guard.ok) return report_error(W4A16_ERR_INVALID, "device %d", pages->device);
+    if (takes_prompt(a)) {
+        const cudaError_t e = launch_prompt(a, bf16, sms, static_cast<cudaStream_t>(stream));
+        return e == cudaSuccess ? W4A16_OK : cuda_error(e, "paged attention launch");
+    }
     const SplitPlan p = plan_split(a, sms);
     const size_t need = split_workspace_bytes(p, pages->head_dim);
     if (workspace_bytes < need || (need > 0 && !workspace_dev))
