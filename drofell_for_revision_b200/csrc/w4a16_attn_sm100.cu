@@ -134,23 +134,10 @@ __device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
     return r;
 }
 
-// 2^x of two values on the FMA units, x <= 8: 2^round(x) by the exponent bits, 2^f for f in
-// [-1/2, 1/2] by the polynomial of degree 4 of least relative error with value 1 at 0
-// (2.8e-6, a hundredth of the 16-bit rounding that follows). Below -126 it runs out through
-// the denormals to exactly 0 at -127, where smaller x (and -inf) are held. NaN stays NaN.
-__device__ __forceinline__ float2 exp2_fma(float2 x) {
-    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));
-    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
-    const uint64_t v = pair_of(x.x, x.y);
-    const uint64_t r = add2(v, pair_of(12582912.f, 12582912.f));  // round(x) in the low bits
-    const uint64_t f = fma2(add2(r, pair_of(-12582912.f, -12582912.f)), pair_of(-1.f, -1.f), v);
-    uint64_t y = fma2(f, pair_of(0.009582700208f, 0.009582700208f), pair_of(0.05590687692f, 0.05590687692f));
-    y = fma2(y, f, pair_of(0.2402410358f, 0.2402410358f));
-    y = fma2(y, f, pair_of(0.6931241155f, 0.6931241155f));
-    y = fma2(y, f, pair_of(1.f, 1.f));
-    const float2 a = of_pair(y), b = of_pair(r);
-    return make_float2(__int_as_float(__float_as_int(a.x) + (__float_as_int(b.x) << 23)),
-                       __int_as_float(__float_as_int(a.y) + (__float_as_int(b.y) << 23)));
+__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
@@ -158,36 +145,41 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// A row's 128 weights 2^(sc s - base) into its columns of P at `ts`, in halves: the product
-// starts on one (an arrival on pfull[0]) while the other is still made. Returns their sum.
-// Every fourth pair is raised on the FMA units, beside the special-function units that bound
-// this phase.
+// 64 of a row's weights, 2^(sc s - base), packed into the first 32 of s; returns their sum.
+// All exponentials on the special-function units: a share of them as polynomials on the FMA
+// units (an eighth to a half were tried) changed nothing, the tensor cores are waited for.
 template <bool BF16>
-__device__ __forceinline__ float weights(uint32_t (&s)[kTileKeys], float sc, float base, uint32_t ts, uint64_t* pfull) {
+__device__ __forceinline__ float weights(uint32_t* s, float sc, float base) {
     const uint64_t sc2 = pair_of(sc, sc), base2 = pair_of(-base, -base);
     uint64_t sum[2] = {0, 0};
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-#pragma unroll
-        for (int c = half * 64; c < half * 64 + 64; c += 2) {
-            float2 x = of_pair(fma2(pair_of(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2, base2));
-            if ((c & 6) == 6) {
-                x = exp2_fma(x);
-            } else {
-                x.x = exp2_approx(x.x);
-                x.y = exp2_approx(x.y);
-            }
-            sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], pair_of(x.x, x.y));
-            s[c >> 1] = pack2<BF16>(x.x, x.y);
-        }
-        tmem_st32(ts + half * 32, s + half * 32);
-        ptx::tmem_st_wait();
-        ptx::tc_fence_before();
-        __syncwarp();
-        if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&pfull[half]);
+    for (int c = 0; c < 64; c += 2) {
+        float2 x = of_pair(fma2(pair_of(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2, base2));
+        x.x = exp2_approx(x.x);
+        x.y = exp2_approx(x.y);
+        sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], pair_of(x.x, x.y));
+        s[c >> 1] = pack2<BF16>(x.x, x.y);
     }
     const float2 part = of_pair(add2(sum[0], sum[1]));
     return part.x + part.y;
+}
+// The largest of 64 scores.
+__device__ __forceinline__ float largest(const uint32_t* s) {
+    float x[2] = {fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1])), fmaxf(__uint_as_float(s[2]), __uint_as_float(s[3]))};
+#pragma unroll
+    for (int c = 4; c < 64; c += 4) {
+        x[0] = max3(x[0], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+        x[1] = max3(x[1], __uint_as_float(s[c + 2]), __uint_as_float(s[c + 3]));
+    }
+    return fmaxf(x[0], x[1]);
+}
+// Half of P into its columns at `ts`, and the arrival that lets its product start.
+__device__ __forceinline__ void put_half(uint32_t ts, const uint32_t* s, uint64_t* pfull) {
+    tmem_st32(ts, s);
+    ptx::tmem_st_wait();
+    ptx::tc_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(pfull);
 }
 
 // Bounded wait that sleeps between polls. Not unrolled, as nothing in this kernel that need
@@ -627,9 +619,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const bool product = j > 0 && vw.active(t, v0);
                     const uint32_t v = kv + sv * C::kTileBytes;
                     auto half_product = [&](int half) {
+                        if (half == 1 && ok) ok = my_turn();
                         if (ok) ok = wait(&pfull[2 * t + half], done & 1, err, kErrMma);
                         ptx::tc_fence_after();
-                        if (half == 1 && ok) ok = my_turn();
 #pragma unroll
                         for (int kk = half * 4; kk < half * 4 + 4; ++kk)
                             if (ok)
@@ -682,6 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t ts = tmem + C::kS + t * 128 + lanes, to = tmem + C::kO + t * 128 + lanes;
         const int step_shift = min(a.pages.page_shift, 7);
         const float sc = a.scale_log2;
+        const bool wide = ((reinterpret_cast<uintptr_t>(a.out) & 31) | ((a.o_token | a.o_head | a.pages.dim) & 15)) == 0;
         int i = 0, seen = 0;  // tiles of keys; scores taken
         bool ok = true;
         Item it;
@@ -704,57 +697,64 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 ptx::tc_fence_after();
                 const uint32_t no_page = bad[i & 7];
-                uint32_t s[kTileKeys];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, s + c * 32);
-                ptx::tmem_ld_wait();
                 const bool whole = no_page == 0 && k0 + kTileKeys - 1 <= vw.p_lo[t] &&
                                    (a.window == 0 || vw.p_hi[t] - k0 < a.window || k0 + kTileKeys <= a.sinks);
-                if (!whole) {
-                    // a bit a key, 32 at a time: up to the row's own, in its window or among the sinks,
-                    // on pages that are pages
-                    const int hi = p - k0, lo = a.window ? hi - a.window : -1, sink = a.window ? a.sinks - k0 : 0;
+                // The first half's weights are taken against the maximum so far, while this tile's own
+                // is still being found; only a row that outgrew it by 2^8 has them taken once more.
+                uint32_t s[kTileKeys];
+                float part;
+                for (;;) {
+                    tmem_ld32(ts, s);
+                    tmem_ld32(ts + 32, s + 32);
+                    ptx::tmem_ld_wait();
+                    tmem_ld32(ts + 64, s + 64);
+                    tmem_ld32(ts + 96, s + 96);
+                    if (!whole) {
+                        ptx::tmem_ld_wait();
+                        // a bit a key, 32 at a time: up to the row's own, in its window or among the sinks,
+                        // on pages that are pages
+                        const int hi = p - k0, lo = a.window ? hi - a.window : -1, sink = a.window ? a.sinks - k0 : 0;
 #pragma unroll
-                    for (int c = 0; c < kTileKeys; c += 32) {
-                        uint32_t in = first_bits(hi + 1 - c) & (~first_bits(lo + 1 - c) | first_bits(sink - c));
-                        if (no_page != 0) {
+                        for (int c = 0; c < kTileKeys; c += 32) {
+                            uint32_t in = first_bits(hi + 1 - c) & (~first_bits(lo + 1 - c) | first_bits(sink - c));
+                            if (no_page != 0) {
 #pragma unroll 1
-                            for (int e = 0; e < 32; e += 8)
-                                if ((no_page >> ((c + e) >> step_shift)) & 1) in &= ~(0xffu << e);
+                                for (int e = 0; e < 32; e += 8)
+                                    if ((no_page >> ((c + e) >> step_shift)) & 1) in &= ~(0xffu << e);
+                            }
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (!((in >> e) & 1)) s[c + e] = 0xff800000u;
                         }
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (!((in >> e) & 1)) s[c + e] = 0xff800000u;
                     }
-                }
-                float x[4];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) x[c] = fmaxf(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1]));
-#pragma unroll
-                for (int c = 8; c < kTileKeys; c += 2)
-                    x[(c >> 1) & 3] = max3(x[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-                const float top = max3(x[0], x[1], fmaxf(x[2], x[3]));
-                if (first) {
-                    m = top;
-                } else {
+                    float top = largest(s);
+                    if (first) {
+                        ptx::tmem_ld_wait();
+                        m = fmaxf(top, largest(s + 64));
+                    }
+                    part = weights<BF16>(s, sc, m == -INFINITY ? 0.f : m * sc);
+                    if (first) break;
+                    ptx::tmem_ld_wait();
+                    top = fmaxf(top, largest(s + 64));
                     const bool grow = (top - m) * sc > kSlack || (m == -INFINITY && top > m);
-                    if (__any_sync(0xffffffffu, grow)) {
-                        const float f = grow ? exp2_approx((m - top) * sc) : 1.f;
-                        if (grow) m = top;
-                        l *= f;
+                    if (!__any_sync(0xffffffffu, grow)) break;
+                    const float f = grow ? exp2_approx((m - top) * sc) : 1.f;
+                    if (grow) m = top;
+                    l *= f;
 #pragma unroll 1
-                        for (int c = 0; c < DP; c += 32) {
-                            uint32_t o[32];
-                            tmem_ld32(to + c, o);
-                            ptx::tmem_ld_wait();
+                    for (int c = 0; c < DP; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(to + c, o);
+                        ptx::tmem_ld_wait();
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                            tmem_st32(to + c, o);
-                        }
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st32(to + c, o);
                     }
                 }
-                const float base = m == -INFINITY ? 0.f : m * sc;
-                l += weights<BF16>(s, sc, base, ts, &pfull[2 * t]);
+                put_half(ts, s, &pfull[2 * t]);
+                part += weights<BF16>(s + 64, sc, m == -INFINITY ? 0.f : m * sc);
+                put_half(ts + 32, s + 64, &pfull[2 * t + 1]);
+                l += part;
                 ++seen;
                 first = false;
             }
@@ -775,18 +775,33 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int e = 0; e < 32; ++e) o[e] = 0u;  // no product was made
                 }
-                float nan = 0.f;
+                uint64_t nan = 0;  // stays 0 if all are finite
+                uint32_t w[16];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) nan += __uint_as_float(o[e]) * 0.f;
-                odd |= !(nan == 0.f);
+                for (int e = 0; e < 32; e += 2) {
+                    const uint64_t y = pair_of(__uint_as_float(o[e]), __uint_as_float(o[e + 1]));
+                    nan = fma2(y, 0, nan);
+                    const float2 z = of_pair(mul2(y, pair_of(inv, inv)));
+                    w[e >> 1] = pack2<BF16>(z.x, z.y);
+                }
+                const float2 z = of_pair(nan);
+                odd |= !(z.x + z.y == 0.f);
+                if (live_row) {
+                    if (wide) {  // whole 32-byte sectors a thread: half the requests
 #pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    uint32_t w[4];
+                        for (int e = 0; e < 16; e += 8)
+                            if (c + 2 * e < a.pages.dim)
+                                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(a.out + o_off + c + 2 * e),
+                                             "r"(w[e]), "r"(w[e + 1]), "r"(w[e + 2]), "r"(w[e + 3]), "r"(w[e + 4]), "r"(w[e + 5]),
+                                             "r"(w[e + 6]), "r"(w[e + 7])
+                                             : "memory");
+                    } else {
 #pragma unroll
-                    for (int y = 0; y < 4; ++y)
-                        w[y] = pack2<BF16>(__uint_as_float(o[e + 2 * y]) * inv, __uint_as_float(o[e + 2 * y + 1]) * inv);
-                    if (live_row && c + e < a.pages.dim)
-                        *reinterpret_cast<uint4*>(a.out + o_off + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                        for (int e = 0; e < 16; e += 4)
+                            if (c + 2 * e < a.pages.dim)
+                                *reinterpret_cast<uint4*>(a.out + o_off + c + 2 * e) =
+                                    make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
+                    }
                 }
             }
             uint32_t again = __ballot_sync(0xffffffffu, odd && live_row);
