@@ -106,12 +106,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
         : "memory");
 }
 
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ uint64_t pair_of(float x, float y) {
     uint64_t r;
@@ -200,52 +194,6 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* e
 // The lowest n bits, n held to 0 .. 32.
 __device__ __forceinline__ uint32_t first_bits(int n) {
     return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
-}
-
-// One row, key by key, each key by selection: for rows whose sums are not finite because a
-// product took in a value that the row does not see (0 x inf, 0 x NaN). A warp a row, lanes
-// over the head's dimensions.
-template <bool BF16>
-__device__ __noinline__ void careful_row(const AttnArgs& a, int b, int h, int64_t q_off, int64_t o_off, int p) {
-    const int lane = threadIdx.x & 31;
-    float q[4] = {}, o[4] = {}, m = -INFINITY, l = 0.f;
-    const int d = lane * 4;
-    const bool in = d < a.pages.dim;
-    auto load4 = [&](const uint16_t* src, float (&x)[4]) {
-        x[0] = x[1] = x[2] = x[3] = 0.f;
-        if (!in) return;
-        const uint2 r = *reinterpret_cast<const uint2*>(src + d);
-        const float2 u = unpack2<BF16>(r.x), v = unpack2<BF16>(r.y);
-        x[0] = u.x, x[1] = u.y, x[2] = v.x, x[3] = v.y;
-    };
-    load4(a.q + q_off, q);
-    const int32_t* table = a.seqs.tables + b * a.seqs.table_stride;
-    const int lo = a.window ? max(0, p + 1 - a.window) : 0;
-#pragma unroll 1
-    for (int j = 0; j <= p; ++j) {
-        if (j >= a.sinks && j < lo) j = lo;
-        const int page = table[j >> a.pages.page_shift];
-        if (page < 0 || page >= a.pages.num_pages) continue;
-        const int64_t at = page * a.pages.stride_page + h * a.pages.stride_head +
-                           (j & ((1 << a.pages.page_shift) - 1)) * a.pages.stride_token;
-        float k[4], v[4];
-        load4(a.pages.k + at, k);
-        load4(a.pages.v + at, v);
-        float s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
-#pragma unroll
-        for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        s *= a.scale_log2;
-        const float m2 = fmaxf(m, s), base = m2 == -INFINITY ? 0.f : m2;
-        const float f = m == m2 ? 1.f : exp2_approx(m - base), w = exp2_approx(s - base);
-        m = m2;
-        l = l * f + w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = (f == 0.f ? 0.f : o[e] * f) + w * v[e];
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (in)
-        *reinterpret_cast<uint2*>(a.out + o_off + d) =
-            make_uint2(pack2<BF16>(o[0] * inv, o[1] * inv), pack2<BF16>(o[2] * inv, o[3] * inv));
 }
 
 // The most items there can be: batch x row pairs x heads, capped well above what is taken.
@@ -809,9 +757,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int r = row - lane + __ffs(again) - 1;
                 again &= again - 1;
                 __syncwarp();
-                careful_row<BF16>(a, it.b, it.h, (it.t0 + r / a.group) * a.q_token + (it.h * a.group + r % a.group) * a.q_head,
-                                  (it.t0 + r / a.group) * a.o_token + (it.h * a.group + r % a.group) * a.o_head,
-                                  it.p0 + r / a.group);
+                const int token = r / a.group, head = it.h * a.group + r - token * a.group;
+                careful_row<kTileKeys, BF16>(a, it.b, it.h, (it.t0 + token) * a.q_token + head * a.q_head, it.p0 + token, vw.kt,
+                                             0, n)
+                    .template store<BF16>(a, (it.t0 + token) * a.o_token + head * a.o_head);
             }
         }
     }

@@ -84,4 +84,70 @@ __device__ __forceinline__ float2 unpack2(uint32_t x) {
     }
 }
 
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A row's maximum, sum of weights and weighted sum of values (four dimensions a lane).
+struct RowSum {
+    float m, l, o[4];
+    template <bool BF16>
+    __device__ __forceinline__ void store(const AttnArgs& a, int64_t o_off) const {
+        const int d = (threadIdx.x & 31) * 4;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (d < a.pages.dim)
+            *reinterpret_cast<uint2*>(a.out + o_off + d) =
+                make_uint2(pack2<BF16>(o[0] * inv, o[1] * inv), pack2<BF16>(o[2] * inv, o[3] * inv));
+    }
+};
+
+// One row over key tiles [i0, i1), key by key and each key by selection: for rows whose sums
+// are not finite because a product took in a value that the row does not see. A warp a row,
+// lanes over the head's dimensions. Slow, and as rare as infinities and NaN are.
+template <int TILE, bool BF16>
+__device__ __noinline__ RowSum careful_row(const AttnArgs& a, int b, int h, int64_t q_off, int p, const KeyTiles<TILE> kt,
+                                           int i0, int i1) {
+    const int d = (threadIdx.x & 31) * 4;
+    const bool in = d < a.pages.dim;
+    auto load4 = [&](const uint16_t* src, float (&x)[4]) {
+        x[0] = x[1] = x[2] = x[3] = 0.f;
+        if (!in) return;
+        const uint2 r = *reinterpret_cast<const uint2*>(src + d);
+        const float2 u = unpack2<BF16>(r.x), v = unpack2<BF16>(r.y);
+        x[0] = u.x, x[1] = u.y, x[2] = v.x, x[3] = v.y;
+    };
+    RowSum r = {-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
+    float q[4];
+    load4(a.q + q_off, q);
+    const int32_t* table = a.seqs.tables + b * a.seqs.table_stride;
+#pragma unroll 1
+    for (int i = i0; i < i1; ++i) {
+#pragma unroll 1
+        for (int c = 0; c < TILE; ++c) {
+            const int j = kt.first(i) + c;
+            if (!visible(j, p, a.window, a.sinks)) continue;
+            const int page = table[j >> a.pages.page_shift];
+            if (page < 0 || page >= a.pages.num_pages) continue;
+            const int64_t at = page * a.pages.stride_page + h * a.pages.stride_head +
+                               (j & ((1 << a.pages.page_shift) - 1)) * a.pages.stride_token;
+            float k[4], v[4];
+            load4(a.pages.k + at, k);
+            load4(a.pages.v + at, v);
+            float s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
+#pragma unroll
+            for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+            s *= a.scale_log2;
+            const float m = fmaxf(r.m, s), base = m == -INFINITY ? 0.f : m;
+            const float f = r.m == m ? 1.f : exp2_approx(r.m - base), w = exp2_approx(s - base);
+            r.m = m;
+            r.l = r.l * f + w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r.o[e] = (f == 0.f ? 0.f : r.o[e] * f) + w * v[e];
+        }
+    }
+    return r;
+}
+
 }  // namespace w4a16

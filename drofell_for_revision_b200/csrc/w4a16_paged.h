@@ -56,9 +56,8 @@ cudaError_t launch_append(const AppendArgs& a, bool bf16, cudaStream_t s);
 
 // Attention split over the cache's length and joined.
 struct SplitPlan {
-    int ctas;       // CTAs that share the work
-    int min_tiles;  // least 64-key tiles per CTA
-    bool join;      // false: no sequence can be long enough to be split
+    int ctas;       // CTAs that share the work, four workers each
+    int min_units;  // least 16-key tiles per worker
 };
 SplitPlan plan_split(const AttnArgs& a, int num_sms);
 size_t split_workspace_bytes(const SplitPlan& p, int dim);
