@@ -11,7 +11,8 @@
 //
 // Work: every warp is a worker of its own. A unit is a tile of 16 keys of one item (sequence,
 // key-value head, 16 rows); all units in item order are cut into equal ranges, one per
-// worker, so that uneven lengths balance, loads run on from one item into the next, no warp
+// worker (an item counts kItemUnits more than its tiles: its query rows and its end), so that
+// uneven lengths balance, loads run on from one item into the next, no warp
 // waits for another, and the workspace has a fixed size: at most the first and the last piece
 // of a range are parts of an item. Those go to the workspace in fp32 and split_join_kernel
 // adds them in range order (the same result for the same lengths, whatever runs when).
@@ -28,20 +29,27 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 16;  // keys
 constexpr int kRows = 16;
+// What an item costs besides its tiles, in tiles: 48 sequences of 1 to 8191 tokens took 104 us
+// at 0 (the workers with many short ones came last), 71 at 1, 59 at 2, 57 at 4, 59 at 6.
+constexpr int kItemUnits = 4;
 
-template <int DP>
+// A ring of K and V tiles per warp: as deep as two CTAs an SM allow, or one where there are no
+// more CTAs than SMs (DEEP: there latency is what counts, and a worker's few tiles are all in
+// flight at once; one sequence of 777 tokens took 14.4 us with the shallow ring).
+template <int DP, bool DEEP>
 struct SplitCfg {
     static constexpr int kStageBytes = 2 * kTile * DP * 2;  // K and V rows
-    static constexpr int kStages = DP == 128 ? 3 : 6;
-    static constexpr int kSmem = kWarps * kStages * kStageBytes;  // a ring per warp; two CTAs an SM
+    static constexpr int kStages = (DP == 128 ? 3 : 6) * (DEEP ? 2 : 1);
+    static constexpr int kSmem = kWarps * kStages * kStageBytes;
 };
 
 // Workspace: of each worker two pieces m[16], l[16], o[16][DP] (the one it begins with, the
 // one it ends with), then what the item is that it continues: {there is one, sequence, head,
-// row tile, its first worker, its last}.
+// row tile, its first worker, its last, its rows in q: first and number}.
 constexpr int piece_floats(int dp) { return 2 * kRows + kRows * dp; }
 constexpr int kDescInts = 8;
 
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
@@ -83,20 +91,20 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
     return static_cast<uint32_t>(r * DP * 2 + ((c ^ (r & 7)) << 4));
 }
 
-// Units of a sequence: key tiles x row tiles x heads.
+// Units of a sequence: key tiles (and kItemUnits) x row tiles x heads. The launcher sees to it
+// that all of a launch fit 31 bits.
 struct Units {
-    int tiles, row_tiles;
-    int64_t units;
+    int tiles, row_tiles, units;
 };
 __device__ __forceinline__ Units units_of(const AttnArgs& a, const Seq& s) {
     Units u;
     u.tiles = s.nq > 0 ? KeyTiles<kTile>(s.p0, s.p0 + s.nq - 1, a.window, a.sinks).count : 0;
     u.row_tiles = (s.nq * a.group + kRows - 1) / kRows;
-    u.units = static_cast<int64_t>(u.tiles) * u.row_tiles * a.pages.heads_kv;
+    u.units = u.tiles > 0 ? (u.tiles + kItemUnits) * u.row_tiles * a.pages.heads_kv : 0;
     return u;
 }
 
-// A place among the units: a key tile of an item of a sequence.
+// A place among the units: a key tile of an item of a sequence (or before its first).
 struct Cursor {
     int b, h, rt, tile;
     Seq sq;
@@ -104,6 +112,7 @@ struct Cursor {
     KeyTiles<kTile> kt;
 
     __device__ __forceinline__ void load(const AttnArgs& a) {  // of sequence b, or the next with units
+#pragma unroll 1
         for (;; ++b) {
             sq = load_seq(a.seqs, a.pages.page_shift, b);
             un = units_of(a, sq);
@@ -112,16 +121,16 @@ struct Cursor {
         kt = KeyTiles<kTile>(sq.p0, sq.p0 + sq.nq - 1, a.window, a.sinks);
     }
     // `off` units into sequence b
-    __device__ __forceinline__ Cursor(const AttnArgs& a, int seq, int64_t off) : b(seq), kt(0, -1, 0, 0) {
+    __device__ __forceinline__ Cursor(const AttnArgs& a, int seq, int off) : b(seq), kt(0, -1, 0, 0) {
         load(a);
-        const int64_t item = off / un.tiles;
-        tile = static_cast<int>(off - item * un.tiles);
-        h = static_cast<int>(item / un.row_tiles);
-        rt = static_cast<int>(item - static_cast<int64_t>(h) * un.row_tiles);
+        const int item = off / (un.tiles + kItemUnits);
+        tile = off - item * (un.tiles + kItemUnits) - kItemUnits;  // below 0: not begun
+        h = item / un.row_tiles;
+        rt = item - h * un.row_tiles;
     }
-    // to the first tile of the next item
+    // to the start of the next item
     __device__ __forceinline__ void next_item(const AttnArgs& a) {
-        tile = 0;
+        tile = -kItemUnits;
         if (++rt < un.row_tiles) return;
         rt = 0;
         if (++h < a.pages.heads_kv) return;
@@ -131,14 +140,14 @@ struct Cursor {
     }
 };
 
-template <int DP, bool BF16>
-__global__ void __launch_bounds__(kThreads, 2) split_kernel(const __grid_constant__ AttnArgs a, const int min_units) {
-    using C = SplitCfg<DP>;
+template <int DP, bool BF16, bool DEEP>
+__global__ void __launch_bounds__(kThreads, DEEP ? 1 : 2) split_kernel(const __grid_constant__ AttnArgs a, const int min_units) {
+    using C = SplitCfg<DP, DEEP>;
     constexpr int CH = DP / 8;   // 16-byte chunks of a row
     constexpr int KS = DP / 16;  // k steps of the score product
     constexpr int S = C::kStages;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int64_t before[kThreads + 1];  // units before a thread's sequences
+    __shared__ int before[kThreads];      // units up to a thread's sequences, within its warp
     __shared__ uint32_t live[kWarps][S];      // keys of a stage that are seen and lie in valid pages
 
     ptx::grid_dep_wait();
@@ -149,7 +158,8 @@ __global__ void __launch_bounds__(kThreads, 2) split_kernel(const __grid_constan
     const int per = (a.seqs.batch + kThreads - 1) / kThreads;
     {
         const int b0 = min(a.seqs.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.seqs.batch, b0 + per);
-        int64_t sum = 0;
+        int sum = 0;
+#pragma unroll 1
         for (int b = b0; b < b1; ++b) {
             const Seq sq = load_seq(a.seqs, a.pages.page_shift, b);
             const Units un = units_of(a, sq);
@@ -157,6 +167,7 @@ __global__ void __launch_bounds__(kThreads, 2) split_kernel(const __grid_constan
             // rows of a sequence without any key are zero
             if (blockIdx.x == b % gridDim.x && sq.nq > 0 && un.tiles == 0) {
                 const int chunks = a.pages.dim >> 3;
+#pragma unroll 1
                 for (int i = 0; i < sq.nq * a.heads * chunks; ++i) {
                     const int row = i / chunks, c = i % chunks;
                     *reinterpret_cast<uint4*>(a.out + (sq.t0 + row / a.heads) * a.o_token + (row % a.heads) * a.o_head +
@@ -166,47 +177,42 @@ __global__ void __launch_bounds__(kThreads, 2) split_kernel(const __grid_constan
         }
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const int64_t o = __shfl_up_sync(0xffffffffu, sum, d);
+            const int o = __shfl_up_sync(0xffffffffu, sum, d);
             if (lane >= d) sum += o;
         }
-        before[threadIdx.x + 1] = sum;
-        if (threadIdx.x == 0) before[0] = 0;
+        before[threadIdx.x] = sum;
     }
     __syncthreads();
-    int64_t sums[kWarps + 1] = {0};  // units before each warp's sequences
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) sums[w + 1] = sums[w] + before[(w + 1) * 32];
-    auto before_of = [&](int i) {  // units before thread i's sequences
-        int64_t x = i ? before[i] : 0;
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w)
-            if (i > w * 32) x += before[w * 32];
-        return x;
-    };
-
     // ---- this warp's range
     const int worker = blockIdx.x * kWarps + warp, workers = gridDim.x * kWarps;
-    const int64_t total = sums[kWarps];
-    const int64_t share = max(static_cast<int64_t>(min_units), (total + workers - 1) / workers);
-    const int64_t begin = min(total, worker * share), end = min(total, begin + share);
+    int warp_end[kWarps];  // units up to each warp's sequences
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) warp_end[w] = total += before[w * 32 + 31];
+    const int share = max(min_units, (total + workers - 1) / workers);
+    // (a worker behind the last unit may lie behind 31 bits)
+    const int begin = static_cast<int>(min(static_cast<int64_t>(total), static_cast<int64_t>(worker) * share));
+    const int end = min(total, begin + min(share, total - begin));
     int* desc = reinterpret_cast<int*>(a.ws + static_cast<size_t>(workers) * 2 * piece_floats(DP)) + worker * kDescInts;
     if (a.ws && lane == 0) desc[0] = 0;
     if (begin >= end) return;
-    int seq_lo = 0, seq_hi = kThreads;  // before_of(seq_lo) <= begin < before_of(seq_hi)
-    while (seq_hi - seq_lo > 1) {
-        const int mid = (seq_lo + seq_hi) >> 1;
-        if (before_of(mid) <= begin) {
-            seq_lo = mid;
-        } else {
-            seq_hi = mid;
-        }
+    // the thread whose sequences hold `begin`: how many end at or before it
+    int holder = 0, off = begin, warp_start = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        const bool past = warp_start + before[w * 32 + lane] <= begin;
+        holder += __popc(__ballot_sync(0xffffffffu, past));
+        warp_start = warp_end[w];
     }
-    int64_t off = begin - before_of(seq_lo);
-    int b_first = seq_lo * per;
-    for (;; ++b_first) {
-        const int64_t n = units_of(a, load_seq(a.seqs, a.pages.page_shift, b_first)).units;
-        if (off < n) break;
-        off -= n;
+    if (holder > 0) off -= before[holder - 1] + (holder > 32 ? warp_end[(holder - 1) / 32 - 1] : 0);
+    int b_first = holder * per;
+    if (per > 1) {
+#pragma unroll 1
+        for (;; ++b_first) {
+            const int n = units_of(a, load_seq(a.seqs, a.pages.page_shift, b_first)).units;
+            if (off < n) break;
+            off -= n;
+        }
     }
     Cursor at(a, b_first, off);
     Cursor ld = at;  // loads run ahead
@@ -216,10 +222,20 @@ __global__ void __launch_bounds__(kThreads, 2) split_kernel(const __grid_constan
     const int slot_mask = (1 << a.pages.page_shift) - 1;
 
     // ---- loads: lanes 0..15 find the rows of a tile, all copy chunks
-    int64_t ld_left = end - begin;
+    int ld_left = end - begin;
     int ld_stage = 0;
     // offset of this lane's key of the loading cursor's tile, -1: none; moves the cursor on
     auto find = [&]() -> int64_t {
+        if (ld.tile < 0) {  // an item begins
+            ld_left += ld.tile;
+            ld.tile = 0;
+            if (ld_left > 0) {  // its query rows on their way to L2
+                const int row = ld.rt * kRows + (lane & 15), token = row / a.group;
+                if (row < ld.sq.nq * a.group && (lane >> 4) * 64 < a.pages.dim)
+                    prefetch_l2(a.q + (ld.sq.t0 + token) * a.q_token + (ld.h * a.group + row - token * a.group) * a.q_head +
+                                (lane >> 4) * 64);
+            }
+        }
         if (ld_left <= 0) return -1;
         --ld_left;
         const int key = ld.kt.first(ld.tile) + (lane & 15);
@@ -250,27 +266,40 @@ __global__ void __launch_bounds__(kThreads, 2) split_kernel(const __grid_constan
         ld_stage = ld_stage + 1 == S ? 0 : ld_stage + 1;
         cp_async_commit();
     };
-#pragma unroll 1
-    for (int i = 0; i < S - 1; ++i) issue(find());  // past the range: a stage of nothing
-    int64_t next = find();
-    int stage = 0;
 
-    int64_t done = begin;
+    // ---- one loop over the tiles: what an item begins and ends with inside it, so that its code
+    // is there once (fetching instructions is a good part of a small call)
+    int done = begin;
+    int64_t next = -1;
+    int stage = 1 % S;  // the first stage holds nothing
+    int tile0 = 0, tile1 = 0;  // of the piece at hand
+    int rows = 0, r0 = 0, r1 = 0, p0 = 0, p1 = 0, p_min = 0, p_max = 0;
+    uint32_t qf[KS][4];  // query rows g and g + 8 of the row tile, as A fragments
+    float o[DP / 8][4], m0 = 0.f, m1 = 0.f, l0 = 0.f, l1 = 0.f;
+    bool begins = true;
 #pragma unroll 1
-    while (done < end) {
-        // ---- a piece: tiles [tile0, tile1) of the item at `at`
-        const int tile0 = at.tile;
-        const int tile1 = static_cast<int>(min(static_cast<int64_t>(at.un.tiles), tile0 + (end - done)));
-        const int h = at.h, rows = at.sq.nq * a.group;
-        const int r0 = at.rt * kRows + g, r1 = r0 + 8;
-        const int i0 = r0 / a.group, i1 = r1 / a.group;
-        const int p0 = r0 < rows ? at.sq.p0 + i0 : -1, p1 = r1 < rows ? at.sq.p0 + i1 : -1;
-        const int64_t out0 = (at.sq.t0 + i0) * a.o_token + (h * a.group + r0 - i0 * a.group) * a.o_head;
-        const int64_t out1 = (at.sq.t0 + i1) * a.o_token + (h * a.group + r1 - i1 * a.group) * a.o_head;
-        uint32_t qf[KS][4];  // query rows g and g + 8 of the row tile, as A fragments
-        {
-            const uint16_t* q0 = a.q + (at.sq.t0 + i0) * a.q_token + (h * a.group + r0 - i0 * a.group) * a.q_head;
-            const uint16_t* q1 = a.q + (at.sq.t0 + i1) * a.q_token + (h * a.group + r1 - i1 * a.group) * a.q_head;
+    for (int step = 0;; ++step) {
+        issue(next);
+        next = find();
+        if (step < S) continue;
+        if (begins) {
+            // ---- a piece: tiles [tile0, tile1) of the item at `at`
+            if (at.tile < 0) {
+                done -= at.tile;
+                at.tile = 0;
+            }
+            if (done >= end) break;
+            begins = false;
+            tile0 = at.tile;
+            tile1 = min(at.un.tiles, tile0 + (end - done));
+            rows = at.sq.nq * a.group;
+            r0 = at.rt * kRows + g;
+            r1 = r0 + 8;
+            const int i0 = r0 / a.group, i1 = r1 / a.group;
+            p0 = r0 < rows ? at.sq.p0 + i0 : -1;
+            p1 = r1 < rows ? at.sq.p0 + i1 : -1;
+            const uint16_t* q0 = a.q + (at.sq.t0 + i0) * a.q_token + (at.h * a.group + r0 - i0 * a.group) * a.q_head;
+            const uint16_t* q1 = a.q + (at.sq.t0 + i1) * a.q_token + (at.h * a.group + r1 - i1 * a.group) * a.q_head;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -280,23 +309,19 @@ __global__ void __launch_bounds__(kThreads, 2) split_kernel(const __grid_constan
                     qf[ks][2 * e] = r0 < rows && in ? *reinterpret_cast<const uint32_t*>(q0 + d) : 0u;
                     qf[ks][2 * e + 1] = r1 < rows && in ? *reinterpret_cast<const uint32_t*>(q1 + d) : 0u;
                 }
-        }
-        // positions of the row tile's first and last row, for the whole-tile test
-        const int row_last = min(rows, at.rt * kRows + kRows) - 1;
-        const int p_min = at.sq.p0 + (at.rt * kRows) / a.group, p_max = at.sq.p0 + row_last / a.group;
-
-        float o[DP / 8][4];
+            // positions of the row tile's first and last row, for the whole-tile test
+            p_min = at.sq.p0 + (at.rt * kRows) / a.group;
+            p_max = at.sq.p0 + (min(rows, at.rt * kRows + kRows) - 1) / a.group;
 #pragma unroll
-        for (int j = 0; j < DP / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-#pragma unroll 1
-        for (int i = tile0; i < tile1; ++i) {
-            issue(next);
-            next = find();
+            for (int j = 0; j < DP / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+            m0 = m1 = -INFINITY;
+            l0 = l1 = 0.f;
+        }
+        {
             cp_async_wait<S - 1>();
             __syncwarp();
             const uint32_t kt_s = ring + stage * C::kStageBytes, vt_s = kt_s + kTile * DP * 2;
-            const int key0 = at.kt.first(i);
+            const int key0 = at.kt.first(at.tile);
             const uint32_t alive = live[warp][stage];
             stage = stage + 1 == S ? 0 : stage + 1;
             if (alive != 0) {
@@ -380,7 +405,13 @@ __global__ void __launch_bounds__(kThreads, 2) split_kernel(const __grid_constan
             }
             __syncwarp();  // the stage may be filled again
         }
+        if (++at.tile < tile1) continue;
+
         // ---- the piece's rows: the result, or a part of it
+        const int h = at.h;
+        const int i0 = r0 / a.group, i1 = r1 / a.group;
+        const int64_t out0 = (at.sq.t0 + i0) * a.o_token + (h * a.group + r0 - i0 * a.group) * a.o_head;
+        const int64_t out1 = (at.sq.t0 + i1) * a.o_token + (h * a.group + r1 - i1 * a.group) * a.o_head;
         l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
         l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
@@ -388,13 +419,9 @@ __global__ void __launch_bounds__(kThreads, 2) split_kernel(const __grid_constan
         const bool part = tile1 - tile0 < at.un.tiles;
         float* ws = part ? a.ws + (static_cast<size_t>(worker) * 2 + (tile0 == 0 ? 1 : 0)) * piece_floats(DP) : nullptr;
         if (part && tile0 > 0 && lane == 0) {
-            const int64_t item = done - tile0;
-            desc[1] = at.b;
-            desc[2] = h;
-            desc[3] = at.rt;
-            desc[4] = static_cast<int>(item / share);
-            desc[5] = static_cast<int>((item + at.un.tiles - 1) / share);
-            desc[0] = 1;
+            const int item = done - tile0;  // of its first tile
+            reinterpret_cast<int4*>(desc)[0] = make_int4(1, at.b, at.h, at.rt);
+            reinterpret_cast<int4*>(desc)[1] = make_int4(item / share, (item + at.un.tiles - 1) / share, at.sq.t0, rows);
         }
         float sum0 = 0.f, sum1 = 0.f;  // 0 if all are finite
 #pragma unroll
@@ -451,73 +478,103 @@ __global__ void __launch_bounds__(kThreads, 2) split_kernel(const __grid_constan
             }
         }
         done += tile1 - tile0;
-        if (done < end) at.next_item(a);
+        if (done >= end) break;
+        at.next_item(a);
+        begins = true;
     }
     cp_async_wait_all();
 }
 
 // One CTA per worker that continues an item: the first such of an item, or as many as it has
 // rows, take a share of its rows and add the pieces in worker order, a warp a row or several
-// when there are many pieces.
-constexpr int kJoinWarps = 8;
+// when there are many pieces. A warp has eight pieces in flight at once: latency is all there
+// is to it.
+constexpr int kJoinWarps = 8, kJoinPieces = 8;
 
 template <int DP, bool BF16>
 __global__ void __launch_bounds__(kJoinWarps * 32) split_join_kernel(const __grid_constant__ AttnArgs a) {
     constexpr int E = DP / 32;
-    __shared__ float sums[kJoinWarps][DP + 1];
+    __shared__ float sums[kJoinWarps][DP + 2];
     ptx::grid_dep_wait();
     const int worker = blockIdx.x + 1, workers = gridDim.x + 1;
-    const int* desc =
-        reinterpret_cast<const int*>(a.ws + static_cast<size_t>(workers) * 2 * piece_floats(DP)) + worker * kDescInts;
-    if (desc[0] == 0) return;
-    const int b = desc[1], h = desc[2], rt = desc[3], first = desc[4], last = desc[5];
+    const int4* desc =
+        reinterpret_cast<const int4*>(a.ws + static_cast<size_t>(workers) * 2 * piece_floats(DP)) + worker * (kDescInts / 4);
+    const int4 d0 = desc[0], d1 = desc[1];
+    if (d0.x == 0) return;
+    const int h = d0.z, rt = d0.w, first = d1.x, last = d1.y, t0 = d1.z;
     const int pieces = last - first + 1, mine = worker - first - 1;
-    const Seq sq = load_seq(a.seqs, a.pages.page_shift, b);
-    const int rows = min(kRows, sq.nq * a.group - rt * kRows);
+    const int rows = min(kRows, d1.w - rt * kRows);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int per_row = pieces >= 32 ? 8 : pieces >= 16 ? 4 : pieces >= 8 ? 2 : 1;  // warps
+    const int per_row = pieces > 4 * kJoinPieces ? 8 : pieces > 2 * kJoinPieces ? 4 : pieces > kJoinPieces ? 2 : 1;  // warps
     const int at_once = kJoinWarps / per_row, sub = warp % per_row;
+#pragma unroll 1
     for (int q = 0; mine + q * (pieces - 1) < rows; q += at_once) {
         const int r = mine + (q + warp / per_row) * (pieces - 1);
-        float x[E] = {}, l = 0.f;
+        float x[E] = {}, m = -INFINITY, l = 0.f;
         if (r < rows) {
-            auto piece = [&](int c) {
-                return a.ws + (static_cast<size_t>(c) * 2 + (c == first ? 1 : 0)) * piece_floats(DP);
-            };
-            float m = -INFINITY;
-            for (int c = first + lane; c <= last; c += 32) m = fmaxf(m, piece(c)[r]);
+#pragma unroll 1
+            for (int c0 = first + sub * kJoinPieces; c0 <= last; c0 += per_row * kJoinPieces) {
+                float v[kJoinPieces][E];
 #pragma unroll
-            for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-            const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll 4
-            for (int c = first + sub; c <= last; c += per_row) {
-                const float* w = piece(c);
-                const float f = exp2_approx(w[r] - base);
-                const float lc = w[kRows + r];
-                float v[E];
-                if constexpr (E == 4) {
-                    const float4 u = *reinterpret_cast<const float4*>(w + 2 * kRows + r * DP + lane * 4);
-                    v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
-                } else {
-                    const float2 u = *reinterpret_cast<const float2*>(w + 2 * kRows + r * DP + lane * 2);
-                    v[0] = u.x, v[1] = u.y;
+                for (int i = 0; i < kJoinPieces; ++i) {
+                    const int c = min(c0 + i, last);
+                    const float* w = a.ws + (static_cast<size_t>(c) * 2 + (c == first ? 1 : 0)) * piece_floats(DP) + 2 * kRows +
+                                     r * DP + lane * E;
+                    if constexpr (E == 4) {
+                        const float4 u = *reinterpret_cast<const float4*>(w);
+                        v[i][0] = u.x, v[i][1] = u.y, v[i][2] = u.z, v[i][3] = u.w;
+                    } else {
+                        const float2 u = *reinterpret_cast<const float2*>(w);
+                        v[i][0] = u.x, v[i][1] = u.y;
+                    }
                 }
-                l += lc * f;
-                // a piece in which the row saw nothing adds nothing
+                // maximum and sum of piece c0 + (lane & 7)
+                const int c = c0 + (lane & (kJoinPieces - 1));
+                const float* w = a.ws + (static_cast<size_t>(min(c, last)) * 2 + (c == first ? 1 : 0)) * piece_floats(DP) + r;
+                const float mc = c <= last ? w[0] : -INFINITY, lc = c <= last ? w[kRows] : 0.f;
+                float m2 = fmaxf(m, mc);
 #pragma unroll
-                for (int e = 0; e < E; ++e) x[e] += f == 0.f ? 0.f : f * v[e];
+                for (int d = kJoinPieces / 2; d; d >>= 1) m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, d));
+                const float base = m2 == -INFINITY ? 0.f : m2;
+                const float old = m == -INFINITY ? 0.f : exp2_approx(m - base), f = exp2_approx(mc - base);
+                m = m2;
+                float sum = lc * f;
+#pragma unroll
+                for (int d = kJoinPieces / 2; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                l = l * old + sum;
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[e] = old == 0.f ? 0.f : x[e] * old;
+#pragma unroll
+                for (int i = 0; i < kJoinPieces; ++i) {
+                    const float fi = __shfl_sync(0xffffffffu, f, i);
+                    // a piece in which the row saw nothing adds nothing
+#pragma unroll
+                    for (int e = 0; e < E; ++e) x[e] += fi == 0.f ? 0.f : fi * v[i][e];
+                }
             }
         }
         if (per_row > 1) {
 #pragma unroll
             for (int e = 0; e < E; ++e) sums[warp][lane * E + e] = x[e];
-            if (lane == 0) sums[warp][DP] = l;
+            if (lane == 0) {
+                sums[warp][DP] = m;
+                sums[warp][DP + 1] = l;
+            }
             __syncthreads();
             if (sub == 0 && r < rows) {
-                for (int w = warp + 1; w < warp + per_row; ++w) {
+                float top = m;
+                for (int w = warp + 1; w < warp + per_row; ++w) top = fmaxf(top, sums[w][DP]);
+                const float base = top == -INFINITY ? 0.f : top;
+                const float f = exp2_approx(m - base);
+                l *= f;
 #pragma unroll
-                    for (int e = 0; e < E; ++e) x[e] += sums[w][lane * E + e];
-                    l += sums[w][DP];
+                for (int e = 0; e < E; ++e) x[e] = f == 0.f ? 0.f : x[e] * f;
+#pragma unroll 1
+                for (int w = warp + 1; w < warp + per_row; ++w) {
+                    const float fw = exp2_approx(sums[w][DP] - base);
+                    l += sums[w][DP + 1] * fw;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) x[e] += fw == 0.f ? 0.f : fw * sums[w][lane * E + e];
                 }
             }
             __syncthreads();
@@ -525,17 +582,17 @@ __global__ void __launch_bounds__(kJoinWarps * 32) split_join_kernel(const __gri
         if (sub == 0 && r < rows && lane * E < a.pages.dim) {
             const float inv = l == 0.f ? 0.f : 1.f / l;
             const int row = rt * kRows + r, token = row / a.group;
-            uint16_t* out = a.out + (sq.t0 + token) * a.o_token + (h * a.group + row - token * a.group) * a.o_head + lane * E;
+            uint16_t* out = a.out + (t0 + token) * a.o_token + (h * a.group + row - token * a.group) * a.o_head + lane * E;
 #pragma unroll
             for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(out + e) = pack2<BF16>(x[e] * inv, x[e + 1] * inv);
         }
     }
 }
 
-template <int DP, bool BF16>
+template <int DP, bool BF16, bool DEEP>
 cudaError_t launch_split_t(const AttnArgs& a, const SplitPlan& p, cudaStream_t s) {
-    using C = SplitCfg<DP>;
-    auto kern = split_kernel<DP, BF16>;
+    using C = SplitCfg<DP, DEEP>;
+    auto kern = split_kernel<DP, BF16, DEEP>;
     static std::atomic<uint64_t> ready{0};
     cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), C::kSmem, ready);
     if (e != cudaSuccess) return e;
@@ -557,22 +614,29 @@ cudaError_t launch_split_t(const AttnArgs& a, const SplitPlan& p, cudaStream_t s
     return cudaLaunchKernelEx(&cfg, split_join_kernel<DP, BF16>, a);
 }
 
-}  // namespace
-
-SplitPlan plan_split(const AttnArgs& a, int num_sms) {
-    SplitPlan p;
-    p.min_units = 4;
-    // what the tables cover bounds the work; the lengths are on the device
+// The most units that one sequence can have: what the tables cover bounds its length, which is
+// on the device.
+int64_t most_units(const AttnArgs& a) {
     const int64_t covered = static_cast<int64_t>(a.seqs.width) << a.pages.page_shift;
     int64_t tiles = (covered + kTile - 1) / kTile;
     if (a.window)
         tiles = std::min<int64_t>(tiles, (int64_t{a.sinks} + kTile - 1) / kTile +
                                              (int64_t{a.window} + a.seqs.max_q + 2 * kTile - 2) / kTile);
-    const int64_t items = static_cast<int64_t>(a.seqs.batch) * a.pages.heads_kv *
-                          ((static_cast<int64_t>(a.seqs.max_q) * a.group + kRows - 1) / kRows);
+    return (tiles + kItemUnits) * a.pages.heads_kv * ((static_cast<int64_t>(a.seqs.max_q) * a.group + kRows - 1) / kRows);
+}
+constexpr int64_t kMostUnits = (int64_t{1} << 31) - (int64_t{1} << 20);
+
+}  // namespace
+
+bool split_fits(const AttnArgs& a) { return most_units(a) <= kMostUnits; }
+
+SplitPlan plan_split(const AttnArgs& a, int num_sms) {
+    SplitPlan p;
+    p.min_units = 4;
     const int64_t each = int64_t{kWarps} * p.min_units;
-    const int64_t most = std::max<int64_t>(1, (items * tiles + each - 1) / each);
+    const int64_t most = std::max<int64_t>(1, (a.seqs.batch * most_units(a) + each - 1) / each);
     p.ctas = static_cast<int>(std::min<int64_t>(2 * num_sms, most));
+    p.deep = p.ctas <= num_sms;
     return p;
 }
 
@@ -581,9 +645,33 @@ size_t split_workspace_bytes(const SplitPlan& p, int dim) {
     return static_cast<size_t>(p.ctas) * kWarps * (2 * piece_floats(dp) * sizeof(float) + kDescInts * sizeof(int));
 }
 
-cudaError_t launch_split(const AttnArgs& a, const SplitPlan& p, bool bf16, cudaStream_t s) {
-    if (a.pages.dim <= 64) return bf16 ? launch_split_t<64, true>(a, p, s) : launch_split_t<64, false>(a, p, s);
-    return bf16 ? launch_split_t<128, true>(a, p, s) : launch_split_t<128, false>(a, p, s);
+cudaError_t launch_split(const AttnArgs& all, const SplitPlan& p, bool bf16, cudaStream_t s) {
+    // as many sequences a launch as have units that fit 31 bits: all of them but for tables of
+    // many millions of tokens
+    const int most = static_cast<int>(std::min<int64_t>(all.seqs.batch, kMostUnits / most_units(all)));
+    for (int b = 0; b < all.seqs.batch; b += most) {
+        AttnArgs a = all;
+        a.seqs.batch = std::min(most, all.seqs.batch - b);
+        a.seqs.tables += b * a.seqs.table_stride;
+        a.seqs.lens += b;
+        if (a.seqs.cu_q) {
+            a.seqs.cu_q += b;
+        } else {
+            a.q += b * a.q_token;
+            a.out += b * a.o_token;
+            a.seqs.tokens = a.seqs.batch;
+        }
+        cudaError_t e;
+        if (a.pages.dim <= 64) {
+            e = p.deep ? (bf16 ? launch_split_t<64, true, true>(a, p, s) : launch_split_t<64, false, true>(a, p, s))
+                       : (bf16 ? launch_split_t<64, true, false>(a, p, s) : launch_split_t<64, false, false>(a, p, s));
+        } else {
+            e = p.deep ? (bf16 ? launch_split_t<128, true, true>(a, p, s) : launch_split_t<128, false, true>(a, p, s))
+                       : (bf16 ? launch_split_t<128, true, false>(a, p, s) : launch_split_t<128, false, false>(a, p, s));
+        }
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 }  // namespace w4a16

@@ -58,7 +58,9 @@ cudaError_t launch_append(const AppendArgs& a, bool bf16, cudaStream_t s);
 struct SplitPlan {
     int ctas;       // CTAs that share the work, four workers each
     int min_units;  // least 16-key tiles per worker
+    bool deep;      // one CTA an SM, with deeper rings
 };
+bool split_fits(const AttnArgs& a);  // the units of a sequence are countable
 SplitPlan plan_split(const AttnArgs& a, int num_sms);
 size_t split_workspace_bytes(const SplitPlan& p, int dim);
 cudaError_t launch_split(const AttnArgs& a, const SplitPlan& p, bool bf16, cudaStream_t s);

@@ -206,6 +206,7 @@ size_t w4a16_paged_attention_workspace_size(const w4a16_pages* pages, const w4a1
     if (takes_prompt(attn_args(pages, seqs, heads, window, sinks))) return 0;
     const int sms = sm_count(pages->device);
     if (sms == 0) return 0;
+    if (!split_fits(attn_args(pages, seqs, heads, window, sinks))) return 0;
     return split_workspace_bytes(plan_split(attn_args(pages, seqs, heads, window, sinks), sms), pages->head_dim);
 }
 
@@ -235,6 +236,8 @@ int w4a16_paged_attention(const w4a16_pages* pages, const w4a16_seqs* seqs, cons
         const cudaError_t e = launch_prompt(a, bf16, sms, static_cast<cudaStream_t>(stream));
         return e == cudaSuccess ? W4A16_OK : cuda_error(e, "paged attention launch");
     }
+    if (!split_fits(a))
+        return report_error(W4A16_ERR_UNSUPPORTED, "tables of %d pages for %d key-value heads", seqs->table_width, pages->heads_kv);
     const SplitPlan p = plan_split(a, sms);
     const size_t need = split_workspace_bytes(p, pages->head_dim);
     if (workspace_bytes < need || (need > 0 && !workspace_dev))
