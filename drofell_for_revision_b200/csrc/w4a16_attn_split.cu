@@ -224,6 +224,9 @@ __global__ void __launch_bounds__(kThreads, DEEP ? 1 : 2) split_kernel(const __g
     // ---- loads: lanes 0..15 find the rows of a tile, all copy chunks
     int ld_left = end - begin;
     int ld_stage = 0;
+    // page ids of the loading cursor's sequence, a lane each from `page0` on: one read of the table
+    // for 32 pages
+    int pages = -1, page0 = 0, page_b = -1;
     // offset of this lane's key of the loading cursor's tile, -1: none; moves the cursor on
     auto find = [&]() -> int64_t {
         if (ld.tile < 0) {  // an item begins
@@ -238,30 +241,37 @@ __global__ void __launch_bounds__(kThreads, DEEP ? 1 : 2) split_kernel(const __g
         }
         if (ld_left <= 0) return -1;
         --ld_left;
-        const int key = ld.kt.first(ld.tile) + (lane & 15);
+        const int key0 = ld.kt.first(ld.tile), key = key0 + (lane & 15), keys = ld.sq.p0 + ld.sq.nq;
         const int lo = a.window ? max(0, max(ld.sq.p0, 0) + 1 - a.window) : 0;  // first key of the earliest window
-        const int32_t* table = a.seqs.tables + ld.b * a.seqs.table_stride;
+        const bool seen = key < keys && (key >= lo || key < a.sinks);           // by any row
         const int64_t head = ld.h * a.pages.stride_head;
-        const bool seen = key < ld.sq.p0 + ld.sq.nq && (key >= lo || key < a.sinks);  // by any row
+        const int want = key0 >> a.pages.page_shift, want2 = (min(key0 + kTile, keys) - 1) >> a.pages.page_shift;
+        if (ld.b != page_b || want < page0 || want2 >= page0 + 32) {
+            page_b = ld.b;
+            page0 = want;
+            const int i = page0 + lane;
+            pages = i <= (keys - 1) >> a.pages.page_shift ? a.seqs.tables[ld.b * a.seqs.table_stride + i] : -1;
+        }
+        const int page = __shfl_sync(0xffffffffu, pages, (key >> a.pages.page_shift) - page0);
         if (++ld.tile == ld.un.tiles && ld_left > 0) ld.next_item(a);
-        if (!seen) return -1;
-        const int page = table[key >> a.pages.page_shift];
-        if (page < 0 || page >= a.pages.num_pages) return -1;
+        if (!seen || page < 0 || page >= a.pages.num_pages) return -1;
         return page * a.pages.stride_page + (key & slot_mask) * a.pages.stride_token + head;
     };
     auto issue = [&](int64_t row_off) {
         const uint32_t ok = __ballot_sync(0xffffffffu, row_off >= 0) & 0xffffu;
         if (lane == 0) live[warp][ld_stage] = ok;
-        const uint32_t dst = ring + ld_stage * C::kStageBytes;
+        if (ok) {  // a tile of no key is not read either
+            const uint32_t dst = ring + ld_stage * C::kStageBytes;
 #pragma unroll
-        for (int j0 = 0; j0 < kTile * CH; j0 += 32) {
-            const int j = j0 + lane, r = j / CH, c = j % CH;
-            const int64_t ro = __shfl_sync(0xffffffffu, row_off, r);
-            const bool in = ro >= 0 && c * 8 < a.pages.dim;
-            const int64_t o = in ? ro + c * 8 : 0;
-            const uint32_t n16 = in ? 16u : 0u;
-            cp_async16(dst + chunk_at<DP>(r, c), a.pages.k + o, n16);
-            cp_async16(dst + kTile * DP * 2 + chunk_at<DP>(r, c), a.pages.v + o, n16);
+            for (int j0 = 0; j0 < kTile * CH; j0 += 32) {
+                const int j = j0 + lane, r = j / CH, c = j % CH;
+                const int64_t ro = __shfl_sync(0xffffffffu, row_off, r);
+                const bool in = ro >= 0 && c * 8 < a.pages.dim;
+                const int64_t o = in ? ro + c * 8 : 0;
+                const uint32_t n16 = in ? 16u : 0u;
+                cp_async16(dst + chunk_at<DP>(r, c), a.pages.k + o, n16);
+                cp_async16(dst + kTile * DP * 2 + chunk_at<DP>(r, c), a.pages.v + o, n16);
+            }
         }
         ld_stage = ld_stage + 1 == S ? 0 : ld_stage + 1;
         cp_async_commit();
@@ -632,7 +642,7 @@ bool split_fits(const AttnArgs& a) { return most_units(a) <= kMostUnits; }
 
 SplitPlan plan_split(const AttnArgs& a, int num_sms) {
     SplitPlan p;
-    p.min_units = 4;
+    p.min_units = 2;  // one sequence of 777 tokens: 10.8 us at 1, 10.1 at 2, 10.3 at 3, 11.2 at 4
     const int64_t each = int64_t{kWarps} * p.min_units;
     const int64_t most = std::max<int64_t>(1, (a.seqs.batch * most_units(a) + each - 1) / each);
     p.ctas = static_cast<int>(std::min<int64_t>(2 * num_sms, most));
