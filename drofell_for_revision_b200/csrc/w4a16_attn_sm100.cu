@@ -208,6 +208,7 @@ struct Item {
     int b, h, row0;   // sequence, head, first row
     int rows;         // of the sequence
     int t0, p0;       // as Seq
+    int j0, j1;       // key tiles: all of them, or a part (the results are then parts too)
 };
 
 // What the warps derive from an item: positions, key tiles, which tiles matter to whom.
@@ -241,16 +242,50 @@ struct View {
     }
 };
 
-// Items of sequence b: its row pairs, those that see most keys first, over the heads.
-__device__ __forceinline__ int64_t items_of(const AttnArgs& a, int b) {
-    const Seq s = load_seq(a.seqs, a.pages.page_shift, b);
-    return static_cast<int64_t>((s.nq * a.group + 2 * kTileRows - 1) / (2 * kTileRows)) * a.pages.heads_kv;
+// Below so many rounds of the CTAs over the items, the last one's are cut along their keys:
+// with more, the time lost in it is small beside the others. A piece has at least four tiles.
+constexpr int kSplitRounds = 4, kPieceTiles = 4;
+
+// Whether items may be cut: few items, and long enough for two pieces as far as the host knows.
+int64_t most_tiles(const AttnArgs& a) {
+    const int64_t covered = static_cast<int64_t>(a.seqs.width) << a.pages.page_shift;
+    int64_t tiles = (covered + kTileKeys - 1) / kTileKeys;
+    if (a.window)
+        tiles = std::min<int64_t>(tiles, (int64_t{a.sinks} + kTileKeys - 1) / kTileKeys +
+                                             (int64_t{a.window} + 2 * kTileRows / a.group + 2 * kTileKeys) / kTileKeys);
+    return tiles;
+}
+bool prompt_may_split(const AttnArgs& a, int num_sms) {
+    return most_items(a) < int64_t{kSplitRounds} * num_sms && most_tiles(a) >= 2 * kPieceTiles;
+}
+int prompt_ctas(const AttnArgs& a, int num_sms) {
+    const int64_t pieces = prompt_may_split(a, num_sms) ? most_tiles(a) / kPieceTiles : 1;
+    return static_cast<int>(std::min<int64_t>(num_sms, most_items(a) * pieces));
+}
+
+// Workspace of cut items: of each CTA m[256], l[256], o[256][DP] of the one piece it can have,
+// then {it has one, first CTA and number of the item's pieces, 0, row0, rows, t0, head}.
+constexpr int part_floats(int dp) { return 2 * kTileRows * (dp + 2); }
+template <int DP>
+__device__ __forceinline__ float* part_slot(const AttnArgs& a, int cta) {
+    return a.ws + static_cast<size_t>(cta) * part_floats(DP);
+}
+template <int DP>
+__device__ __forceinline__ int* part_desc(const AttnArgs& a, int ctas, int cta) {
+    return reinterpret_cast<int*>(a.ws + static_cast<size_t>(ctas) * part_floats(DP)) + cta * 8;
+}
+
+// Items of a sequence: its row pairs, those that see most keys first, over the heads. The host
+// has made sure that all of a call fit 31 bits.
+__device__ __forceinline__ int items_of(const AttnArgs& a, const Seq& s) {
+    return (s.nq * a.group + 2 * kTileRows - 1) / (2 * kTileRows) * a.pages.heads_kv;
 }
 
 template <int DP, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                  const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ AttnArgs a, const int q_by_tma) {
+                  const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ AttnArgs a, const int q_by_tma,
+                  const int may_split) {
     using C = Cfg<DP>;
     constexpr int CH = DP / 8;
     constexpr int SL = C::kSlots;
@@ -274,16 +309,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     int* before = reinterpret_cast<int*>(smem + C::kListOff);       // [kThreads + 1] items before a thread's sequences
 
     ptx::grid_dep_wait();
+    if (may_split) ptx::grid_dep_launch_dependents();  // the join, which waits for all of this
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     // ---- how many items come before each thread's share of the sequences
     const int per = (a.seqs.batch + kThreads - 1) / kThreads;
     {
         const int b0 = min(a.seqs.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.seqs.batch, b0 + per);
-        int64_t mine = 0;
-        for (int b = b0; b < b1; ++b) mine += items_of(a, b);
-        // the host has made sure that the items of all sequences fit 31 bits
-        int sum = static_cast<int>(mine);
+        int sum = 0;
+#pragma unroll 1
+        for (int b = b0; b < b1; ++b) sum += items_of(a, load_seq(a.seqs, a.pages.page_shift, b));
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int o = __shfl_up_sync(0xffffffffu, sum, d);
@@ -293,6 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (threadIdx.x == 0) before[0] = 0;
     }
     if (threadIdx.x == 0) {
+        if (may_split) part_desc<DP>(a, gridDim.x, blockIdx.x)[0] = 0;
         for (int s = 0; s < SL; ++s) {
             ptx::mbar_init(&full[s], 1);
             ptx::mbar_init(&empty[s], 2);
@@ -321,16 +357,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     ptx::tc_fence_before();
     __syncthreads();
-    if (warp == kLoadWarp) {  // the warps' sums into one running sum
-        int base = 0;
-#pragma unroll 1
-        for (int w = 0; w < kThreads / 32; ++w) {
-            const int x = before[w * 32 + lane + 1] + base;
-            __syncwarp();
-            before[w * 32 + lane + 1] = x;
-            base = __shfl_sync(0xffffffffu, x, 31);
-        }
-    }
     ptx::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     int* err = &g_attention_error;
@@ -347,6 +373,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         it.rows = posted[s * 8 + 3];
         it.t0 = posted[s * 8 + 4];
         it.p0 = posted[s * 8 + 5];
+        it.j0 = posted[s * 8 + 6];
+        it.j1 = posted[s * 8 + 7];
         if (whole_warp) __syncwarp();
         if (!whole_warp || lane == 0) ptx::mbar_arrive(&iempty[s]);
         return it.b >= 0;
@@ -359,36 +387,48 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int page_size = 1 << a.pages.page_shift;
             const int box = min(page_size, kTileKeys);
             const int boxes = kTileKeys / box;  // per tile, at most 16: one a lane
+            int total = 0;  // of all sequences; the warps' sums become one running sum
+#pragma unroll 1
+            for (int x = 0; x < kThreads && x * per < a.seqs.batch; x += 32) {
+                const int y = before[x + lane + 1] + total;
+                __syncwarp();
+                before[x + lane + 1] = y;
+                total = __shfl_sync(0xffffffffu, y, 31);
+            }
             __syncwarp();
-            const int total = before[kThreads];
             const int ctas = gridDim.x;
             int i = 0, q_loads = 0;  // tiles of K and V, row pairs of Q so far
             bool ok = true;
 #pragma unroll 1
             for (int k = 0; ok; ++k) {
                 // rounds of the CTAs run forth and back over the items, whose work falls along a
-                // sequence: a CTA's shares even out
-                const int64_t at = static_cast<int64_t>(k) * ctas + ((k & 1) ? ctas - 1 - static_cast<int>(blockIdx.x) : blockIdx.x);
+                // sequence: a CTA's shares even out. Where there are few rounds, the items of the last,
+                // incomplete one are cut along their keys, among all CTAs.
+                int64_t at = static_cast<int64_t>(k) * ctas + ((k & 1) ? ctas - 1 - static_cast<int>(blockIdx.x) : blockIdx.x);
+                int pieces = 1, piece = 0;
+                const int rounds = total / ctas, rest_items = total - rounds * ctas;
+                if (may_split && rounds < kSplitRounds && k >= rounds) {
+                    pieces = rest_items > 0 ? ctas / rest_items : 1;
+                    piece = static_cast<int>(blockIdx.x) % pieces;
+                    at = static_cast<int64_t>(rounds) * ctas + static_cast<int>(blockIdx.x) / pieces;
+                    if (k > rounds) at = total;
+                }
                 Item it;
                 it.b = -1;
-                it.h = it.row0 = it.rows = it.t0 = it.p0 = 0;
+                it.h = it.row0 = it.rows = it.t0 = it.p0 = it.j0 = it.j1 = 0;
                 if (at < total) {
-                    int lo = 0, hi = kThreads;  // before[lo] <= at < before[hi]
-                    while (hi - lo > 1) {
-                        const int mid = (lo + hi) >> 1;
-                        if (before[mid] <= at) {
-                            lo = mid;
-                        } else {
-                            hi = mid;
-                        }
-                    }
-                    int rest = static_cast<int>(at) - before[lo], b = lo * per;
-                    for (;; ++b) {
-                        const int n = static_cast<int>(items_of(a, b));
-                        if (rest < n) break;
+                    // the thread whose sequences hold it: how many end at or before it
+                    int holder = 0;
+#pragma unroll 1
+                    for (int x = 0; x < kThreads && x * per < a.seqs.batch; x += 32)
+                        holder += __popc(__ballot_sync(0xffffffffu, before[x + lane + 1] <= at));
+                    int rest = static_cast<int>(at) - before[holder], b = holder * per;
+                    Seq sq = load_seq(a.seqs, a.pages.page_shift, b);
+#pragma unroll 1
+                    for (int n; rest >= (n = items_of(a, sq));) {
                         rest -= n;
+                        sq = load_seq(a.seqs, a.pages.page_shift, ++b);
                     }
-                    const Seq sq = load_seq(a.seqs, a.pages.page_shift, b);
                     const int pairs = (sq.nq * a.group + 2 * kTileRows - 1) / (2 * kTileRows);
                     it.b = b;
                     it.row0 = (pairs - 1 - rest / a.pages.heads_kv) * 2 * kTileRows;
@@ -396,6 +436,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                     it.rows = sq.nq * a.group;
                     it.t0 = sq.t0;
                     it.p0 = sq.p0;
+                    const int n = View(it, a).kt.count;
+                    pieces = min(pieces, max(1, n / kPieceTiles));
+                    if (piece < pieces) {
+                        it.j0 = static_cast<int>(static_cast<int64_t>(n) * piece / pieces);
+                        it.j1 = static_cast<int>(static_cast<int64_t>(n) * (piece + 1) / pieces);
+                        if (pieces > 1 && lane == 0) {
+                            int4* d = reinterpret_cast<int4*>(part_desc<DP>(a, ctas, blockIdx.x));
+                            d[1] = make_int4(it.row0, it.rows, it.t0, it.h);
+                            d[0] = make_int4(1, blockIdx.x - piece, pieces, 0);
+                        }
+                    } else {
+                        it.b = -1;
+                    }
                 }
                 const int s = k & 1;
                 if (k >= 2) ok = warp_wait(&iempty[s], ((k >> 1) - 1) & 1, err, kErrLoad);
@@ -406,23 +459,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                     posted[s * 8 + 3] = it.rows;
                     posted[s * 8 + 4] = it.t0;
                     posted[s * 8 + 5] = it.p0;
+                    posted[s * 8 + 6] = it.j0;
+                    posted[s * 8 + 7] = it.j1;
                     ptx::mbar_arrive(&ifull[s]);
                 }
                 if (it.b < 0 || !ok) break;
                 const View vw(it, a);
-                const int n = vw.kt.count;
                 const int32_t* table = a.seqs.tables + it.b * a.seqs.table_stride;
                 auto page_of = [&](int j) {  // this lane's page of key tile j
                     int page = a.pages.num_pages;  // behind the cache's end: zeros
-                    if (j < n && lane < boxes) {
+                    if (j < it.j1 && lane < boxes) {
                         const int key = vw.kt.first(j) + lane * box;
                         if (key <= vw.last) page = table[key >> a.pages.page_shift];
                     }
                     return page;
                 };
-                int page = page_of(0);
+                int page = page_of(it.j0);
 #pragma unroll 1
-                for (int j = 0; j < n && ok; ++j) {
+                for (int j = it.j0; j < it.j1 && ok; ++j) {
                     const int key = vw.kt.first(j) + lane * box;
                     const int next = page_of(j + 1);
                     const bool none = page < 0 || page >= a.pages.num_pages;
@@ -447,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                     page = next;
-                    if (j == 0 && ok && q_by_tma) {
+                    if (j == it.j0 && ok && q_by_tma) {
                         // after the first keys: the rows of the last item may still be in use
                         if (k > 0) ok = warp_wait(qempty, (k - 1) & 1, err, kErrLoad);
                         if (ok && lane == 0) {
@@ -461,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
                 // an item without keys takes no Q: its phases pass all the same
-                if (n == 0 && ok && q_by_tma) {
+                if (it.j0 == it.j1 && ok && q_by_tma) {
                     if (k > 0) ok = warp_wait(qempty, (k - 1) & 1, err, kErrLoad);
                     if (ok && lane == 0) ptx::mbar_arrive(qfull);
                     if (ok) ++q_loads;
@@ -480,7 +534,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
             for (int k = 0; ok && next_item(k, it, true); ++k) {
                 const View vw(it, a);
-                const int n = vw.kt.count;
                 if (!q_by_tma) {
                     if (k > 0) ok = warp_wait(qempty, (k - 1) & 1, err, kErrMma);
                     if (!ok) break;
@@ -491,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     int r = lane / CH, token = (it.row0 + r) / a.group, g = it.row0 + r - token * a.group;
 #pragma unroll 2
                     for (; r < 2 * kTileRows; r += kStep) {
-                        const bool in = c * 8 < a.pages.dim && r < left && n > 0;
+                        const bool in = c * 8 < a.pages.dim && r < left && it.j0 < it.j1;
                         const uint16_t* src =
                             in ? a.q + (it.t0 + token) * a.q_token + (it.h * a.group + g) * a.q_head + c * 8 : a.q;
                         cp_async16(dst + (r >> 7) * C::kTileBytes + (c >> 3) * kBlock + (r & 127) * 128 +
@@ -511,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // asked for by both MMA threads, one tile at a time (a barrier's parity tells only two
                 // phases apart: a warp that skips tiles cannot wait on `full`)
 #pragma unroll 1
-                for (int j = 0; j < n && ok; ++j, i += 2) {
+                for (int j = it.j0; j < it.j1 && ok; ++j, i += 2) {
                     const int k0 = vw.kt.first(j);
                     if (!vw.cut(k0)) continue;
                     ok = warp_wait(dirty, asked++ & 1, err, kErrMma);
@@ -547,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
             for (int k = 0; ok && next_item(k, it, false); ++k) {
                 const View vw(it, a);
-                const int n = vw.kt.count;
+                const int n = it.j1 - it.j0;  // j counts from the item's first tile
                 ok = wait(qfull, k & 1, err, kErrMma);
                 bool first = true;
                 // step j: P V of tile j - 1, then the scores of tile j
@@ -555,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int j = 0; j <= n && ok; ++j, i += 2) {
                     const int iv = i - 1;                            // of V_{j-1}; K_j is i
                     const int sk = i % SL, sv = (iv + SL) % SL;
-                    const int k0 = vw.kt.first(j), v0 = vw.kt.first(j - 1);
+                    const int k0 = vw.kt.first(it.j0 + j), v0 = vw.kt.first(it.j0 + j - 1);
                     if (j > 0) {
                         if (vw.cut(v0)) ok = wait(clean, cleaned++ & 1, err, kErrMma);
                         if (ok) ok = wait(&full[sv], (iv / SL) & 1, err, kErrMma);
@@ -629,14 +682,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int k = 0; ok && next_item(k, it, true); ++k) {
             const View vw(it, a);
-            const int n = vw.kt.count;
+            const bool part = it.j1 - it.j0 < vw.kt.count;
             const int row = it.row0 + t * kTileRows + tid;
             const bool live_row = row < it.rows;
             const int p = live_row ? max(-1, it.p0 + row / a.group) : -1;
             float m = -INFINITY, l = 0.f;  // m in units of the unscaled score
             bool first = true;
 #pragma unroll 1
-            for (int j = 0; j < n; ++j, ++i) {
+            for (int j = it.j0; j < it.j1; ++j, ++i) {
                 const int k0 = vw.kt.first(j);
                 if (!vw.active(t, k0)) continue;
                 if (!warp_wait(&sfull[t], seen & 1, err, kErrSoftmax)) {
@@ -651,18 +704,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // is still being found; only a row that outgrew it by 2^8 has them taken once more.
                 uint32_t s[kTileKeys];
                 float part;
+                bool masked = false;
                 for (;;) {
-                    tmem_ld32(ts, s);
-                    tmem_ld32(ts + 32, s + 32);
-                    ptx::tmem_ld_wait();
-                    tmem_ld32(ts + 64, s + 64);
-                    tmem_ld32(ts + 96, s + 96);
-                    if (!whole) {
-                        ptx::tmem_ld_wait();
-                        // a bit a key, 32 at a time: up to the row's own, in its window or among the sinks,
-                        // on pages that are pages
+                    if (__builtin_expect(!whole && !masked, 0)) {
+                        // into the scores where they lie, 32 keys at a time: a bit a key, up to the row's own,
+                        // in its window or among the sinks, on pages that are pages
+                        masked = true;
                         const int hi = p - k0, lo = a.window ? hi - a.window : -1, sink = a.window ? a.sinks - k0 : 0;
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < kTileKeys; c += 32) {
                             uint32_t in = first_bits(hi + 1 - c) & (~first_bits(lo + 1 - c) | first_bits(sink - c));
                             if (no_page != 0) {
@@ -670,13 +719,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 for (int e = 0; e < 32; e += 8)
                                     if ((no_page >> ((c + e) >> step_shift)) & 1) in &= ~(0xffu << e);
                             }
+                            tmem_ld32(ts + c, s);
+                            ptx::tmem_ld_wait();
 #pragma unroll
                             for (int e = 0; e < 32; ++e)
-                                if (!((in >> e) & 1)) s[c + e] = 0xff800000u;
+                                if (!((in >> e) & 1)) s[e] = 0xff800000u;
+                            tmem_st32(ts + c, s);
                         }
+                        ptx::tmem_st_wait();
                     }
+                    tmem_ld32(ts, s);
+                    tmem_ld32(ts + 32, s + 32);
+                    ptx::tmem_ld_wait();
+                    tmem_ld32(ts + 64, s + 64);
+                    tmem_ld32(ts + 96, s + 96);
                     float top = largest(s);
-                    if (first) {
+                    if (__builtin_expect(first, 0)) {
                         ptx::tmem_ld_wait();
                         m = fmaxf(top, largest(s + 64));
                     }
@@ -685,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ptx::tmem_ld_wait();
                     top = fmaxf(top, largest(s + 64));
                     const bool grow = (top - m) * sc > kSlack || (m == -INFINITY && top > m);
-                    if (!__any_sync(0xffffffffu, grow)) break;
+                    if (__builtin_expect(!__any_sync(0xffffffffu, grow), 1)) break;
                     const float f = grow ? exp2_approx((m - top) * sc) : 1.f;
                     if (grow) m = top;
                     l *= f;
@@ -710,8 +768,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (ok) ok = warp_wait(&ofull[t], k & 1, err, kErrEnd);
             if (!ok) break;
             ptx::tc_fence_after();
-            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const float inv = part ? 1.f : l == 0.f ? 0.f : 1.f / l;
             const int64_t o_off = (it.t0 + row / a.group) * a.o_token + (it.h * a.group + row % a.group) * a.o_head;
+            float* slot = part ? part_slot<DP>(a, blockIdx.x) : nullptr;
+            const int pr = t * kTileRows + tid;  // row of the part
+            if (part) {
+                slot[pr] = m == -INFINITY ? m : m * sc;
+                slot[2 * kTileRows + pr] = l;
+            }
             bool odd = false;
 #pragma unroll 1
             for (int c = 0; c < DP; c += 32) {
@@ -734,7 +798,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 const float2 z = of_pair(nan);
                 odd |= !(z.x + z.y == 0.f);
-                if (live_row) {
+                if (part) {
+                    float* dst = slot + 4 * kTileRows + pr * DP + c;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8)
+                        if (live_row)
+                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + e), "r"(o[e]),
+                                         "r"(o[e + 1]), "r"(o[e + 2]), "r"(o[e + 3]), "r"(o[e + 4]), "r"(o[e + 5]), "r"(o[e + 6]),
+                                         "r"(o[e + 7])
+                                         : "memory");
+                } else if (live_row) {
                     if (wide) {  // whole 32-byte sectors a thread: half the requests
 #pragma unroll
                         for (int e = 0; e < 16; e += 8)
@@ -758,9 +831,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                 again &= again - 1;
                 __syncwarp();
                 const int token = r / a.group, head = it.h * a.group + r - token * a.group;
-                careful_row<kTileKeys, BF16>(a, it.b, it.h, (it.t0 + token) * a.q_token + head * a.q_head, it.p0 + token, vw.kt,
-                                             0, n)
-                    .template store<BF16>(a, (it.t0 + token) * a.o_token + head * a.o_head);
+                const RowSum x = careful_row<kTileKeys, BF16>(a, it.b, it.h, (it.t0 + token) * a.q_token + head * a.q_head,
+                                                              it.p0 + token, vw.kt, it.j0, it.j1);
+                if (part) {
+                    const int rr = r - it.row0;
+                    if (lane == 0) {
+                        slot[rr] = x.m;
+                        slot[2 * kTileRows + rr] = x.l;
+                    }
+                    if (lane * 4 < DP)
+                        *reinterpret_cast<float4*>(slot + 4 * kTileRows + rr * DP + lane * 4) =
+                            make_float4(x.o[0], x.o[1], x.o[2], x.o[3]);
+                } else {
+                    x.store<BF16>(a, (it.t0 + token) * a.o_token + head * a.o_head);
+                }
             }
         }
     }
@@ -773,6 +857,54 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
+// The pieces of the cut items, added in key order: of an item's 256 rows every CTA of its
+// pieces (and kJoinParts of them) takes a share, a warp a row.
+constexpr int kJoinWarps = 8, kJoinParts = 4;
+
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(kJoinWarps * 32) prompt_join_kernel(const __grid_constant__ AttnArgs a) {
+    constexpr int E = DP / 32;
+    ptx::grid_dep_wait();
+    const int ctas = gridDim.x;
+    const int4* d = reinterpret_cast<const int4*>(part_desc<DP>(a, ctas, blockIdx.x));
+    const int4 d0 = d[0];
+    if (d0.x == 0) return;
+    const int4 d1 = d[1];
+    const int first = d0.y, pieces = d0.z, row0 = d1.x, rows = d1.y, t0 = d1.z, h = d1.w;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int share = (static_cast<int>(blockIdx.x) - first) * kJoinParts + blockIdx.y;
+    for (int r = share * kJoinWarps + warp; r < min(2 * kTileRows, rows - row0); r += pieces * kJoinParts * kJoinWarps) {
+        float m = -INFINITY;
+        for (int c = lane; c < pieces; c += 32) m = fmaxf(m, part_slot<DP>(a, first + c)[r]);
+#pragma unroll
+        for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+        const float base = m == -INFINITY ? 0.f : m;
+        float o[E] = {}, l = 0.f;
+#pragma unroll 4
+        for (int c = 0; c < pieces; ++c) {
+            const float* s = part_slot<DP>(a, first + c);
+            const float f = exp2_approx(s[r] - base);
+            l += f * s[2 * kTileRows + r];
+            float v[E];
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                const float2 u = *reinterpret_cast<const float2*>(s + 4 * kTileRows + r * DP + lane * E + e);
+                v[e] = u.x, v[e + 1] = u.y;
+            }
+            // a piece in which the row saw nothing adds nothing
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += f == 0.f ? 0.f : f * v[e];
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int row = row0 + r, token = row / a.group;
+        uint16_t* out = a.out + (t0 + token) * a.o_token + (h * a.group + row - token * a.group) * a.o_head + lane * E;
+        if (lane * E < a.pages.dim) {
+#pragma unroll
+            for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(out + e) = pack2<BF16>(o[e] * inv, o[e + 1] * inv);
+        }
+    }
+}
+
 template <int DP, bool BF16>
 cudaError_t launch_prompt_t(const AttnArgs& a, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const CUtensorMap& tm_q,
                             bool q_by_tma, int num_sms, cudaStream_t s) {
@@ -781,7 +913,7 @@ cudaError_t launch_prompt_t(const AttnArgs& a, const CUtensorMap& tm_k, const CU
     cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), Cfg<DP>::kSmem, ready);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(num_sms, most_items(a))));
+    cfg.gridDim = dim3(prompt_ctas(a, num_sms));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = Cfg<DP>::kSmem;
     cfg.stream = s;
@@ -790,12 +922,23 @@ cudaError_t launch_prompt_t(const AttnArgs& a, const CUtensorMap& tm_k, const CU
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, tm_k, tm_v, tm_q, a, q_by_tma ? 1 : 0);
+    const bool may_split = prompt_may_split(a, num_sms);
+    e = cudaLaunchKernelEx(&cfg, kern, tm_k, tm_v, tm_q, a, q_by_tma ? 1 : 0, may_split ? 1 : 0);
+    if (e != cudaSuccess || !may_split) return e;
+    cfg.gridDim.y = kJoinParts;
+    cfg.blockDim = dim3(kJoinWarps * 32);
+    cfg.dynamicSmemBytes = 0;
+    return cudaLaunchKernelEx(&cfg, prompt_join_kernel<DP, BF16>, a);
 }
 
 }  // namespace
 
 bool prompt_fits(const AttnArgs& a) { return most_items(a) <= (1 << 30); }
+
+size_t prompt_workspace_bytes(const AttnArgs& a, int num_sms) {
+    if (!prompt_may_split(a, num_sms)) return 0;
+    return static_cast<size_t>(prompt_ctas(a, num_sms)) * (part_floats(a.pages.dim <= 64 ? 64 : 128) * sizeof(float) + 32);
+}
 
 cudaError_t launch_prompt(const AttnArgs& a, bool bf16, int num_sms, cudaStream_t s) {
     const PageView& p = a.pages;

@@ -67,6 +67,7 @@ cudaError_t launch_split(const AttnArgs& a, const SplitPlan& p, bool bf16, cudaS
 
 // Attention of prompts on the tensor cores (w4a16_attn_sm100.cu).
 bool prompt_fits(const AttnArgs& a);
+size_t prompt_workspace_bytes(const AttnArgs& a, int num_sms);
 cudaError_t launch_prompt(const AttnArgs& a, bool bf16, int num_sms, cudaStream_t s);
 // The current device's error word of its bounded waits, then cleared. Synchronises `s`.
 cudaError_t read_attention_error(int* out, cudaStream_t s);

@@ -289,7 +289,8 @@ W4A16_API int w4a16_append_kv(const w4a16_pages* pages, const w4a16_seqs* seqs, 
  * `sinks` ones. heads is a multiple of heads_kv; query head i reads key-value head
  * i / (heads / heads_kv). Rows that see nothing are 0. Softmax statistics and sums in
  * fp32. No host synchronisation and no allocation: capturable. Calls that may overlap on
- * the GPU need workspaces of their own. */
+ * the GPU need workspaces of their own; a workspace is 32-byte aligned, its contents mean
+ * nothing before and after a call. */
 W4A16_API int w4a16_paged_attention(const w4a16_pages* pages, const w4a16_seqs* seqs, const w4a16_rows* q,
                                     const w4a16_rows* out, int heads, float scale, int window, int sinks,
                                     void* workspace_dev, size_t workspace_bytes, void* stream);

@@ -160,6 +160,33 @@ def test_long_chunk(window, sinks):
     check_attention(Batch([5000, 2049], [1500, 2049], 8, 4, 128, 64, torch.bfloat16, seed=13), window, sinks)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,heads_kv,dim,lens,new,window,sinks", [
+    (8, 8, 128, [4099], [65], 0, 0),            # few rows on a long context: keys cut among all SMs
+    (16, 1, 64, [9000, 130], [129, 7], 0, 0),
+    (5, 1, 128, [3000, 2500], [100, 2500], 0, 0),  # a group that does not divide a row tile
+    (4, 2, 128, [6000], [300], 1500, 4),
+    (2, 1, 96, [2100], [2100], 700, 0),         # rows that see nothing of a piece
+    (32, 8, 64, [33000], [40], 0, 0),
+])
+def test_chunk_on_a_long_context(dtype, heads, heads_kv, dim, lens, new, window, sinks):
+    check_attention(Batch(lens, new, heads, heads_kv, dim, 32, dtype, seed=43), window, sinks)
+
+
+def test_many_row_tiles():
+    """More row pairs than a few rounds of the SMs take, and uneven sequences among them."""
+    check_attention(Batch([4100, 1, 900], [4000, 1, 700], 40, 40, 64, 64, torch.float16, seed=47))
+
+
+def test_many_prompts():
+    """More prompts than the threads that count them, some of no new token."""
+    g = torch.Generator().manual_seed(2)
+    new = torch.randint(0, 40, (300,), generator=g).tolist()
+    new[7] = 180
+    lens = [n + int(torch.randint(0, 90, (1,), generator=g)) for n in new]
+    check_attention(Batch(lens, new, 4, 2, 64, 16, torch.bfloat16, seed=53))
+
+
 def test_many_sequences():
     """More sequences than a CTA has threads, among them empty ones."""
     g = torch.Generator().manual_seed(1)
@@ -215,10 +242,11 @@ def test_unwritten_slots_may_hold_anything(value, new):
 
 
 @pytest.mark.parametrize("value", [math.nan, math.inf])
-@pytest.mark.parametrize("new,window", [(4, 0), (4, 20), (140, 0), (140, 64)])
-def test_a_value_reaches_only_the_rows_that_see_it(value, new, window):
-    bt = Batch([new + 60], [new], 4, 2, 128, 16, torch.float16, seed=23)
-    for j in (new + 57, 61, 60 + new // 2):
+@pytest.mark.parametrize("new,old,window", [(4, 60, 0), (4, 60, 20), (4, 900, 0), (140, 60, 0), (140, 60, 64),
+                                            (140, 2000, 0)])
+def test_a_value_reaches_only_the_rows_that_see_it(value, new, old, window):
+    bt = Batch([new + old], [new], 4, 2, 128, 16, torch.float16, seed=23)
+    for j in (new + old - 3, old + 1, old + new // 2):
         bt.v[int(bt.tables[0, j // 16]), :, j % 16, 5] = value
     check_attention(bt, window)
 
