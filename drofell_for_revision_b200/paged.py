@@ -25,7 +25,7 @@ from typing import Dict, Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
 
-from . import _capi
+from . import _capi, exllama
 
 PageIds = Union[Sequence[int], torch.Tensor]
 
@@ -74,6 +74,34 @@ def device_error(device: Optional[torch.device] = None) -> int:
     v = ctypes.c_int(0)
     _capi.check(_capi.lib().w4a16_paged_error(index, _capi.stream_ptr(index), ctypes.byref(v)))
     return v.value
+
+
+def attention_forward(layernorm: torch.Tensor, norm_epsilon: float, q_proj: int, k_proj: int, v_proj: int, o_proj: int,
+                      x: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor,
+                      lens: torch.Tensor, rope: Optional[torch.Tensor] = None, cu_q: Optional[torch.Tensor] = None,
+                      max_q: int = 1, window: int = 0, sinks: int = 0, interleaved: bool = False,
+                      output: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The attention block of a decoder layer, beside ``exllama.mlp_forward_v2``: RMSNorm and the
+    q, k, v projections (``attention_forward_qkv_stage_v2``), k and v into the pages, attention
+    over them, the o projection. x [rows, hidden] fp16, one row per new token; the projections
+    are q4 handles (``q4_matrix.cuda_q4``). Returns [rows, hidden] without the residual."""
+    hq, hk, hv, ho = (exllama._handle(h) for h in (q_proj, k_proj, v_proj, o_proj))
+    if x.dim() != 2 or x.shape[1] != hq.K:
+        raise RuntimeError(f"x must be [rows, {hq.K}]")
+    dim, rows = k_pages.shape[-1], x.shape[0]
+    heads, heads_kv = hq.N // dim, hk.N // dim
+    if hq.N % dim or hk.N % dim or hv.N != hk.N or ho.K != hq.N:
+        raise RuntimeError(f"projections of {hq.N}, {hk.N}, {hv.N} columns and {ho.K} rows for heads of {dim}")
+    rms = torch.empty_like(x)
+    q, k, v = (torch.empty((rows, h.N), dtype=x.dtype, device=x.device) for h in (hq, hk, hv))
+    _capi.qkv_forward(hq, hk, hv, layernorm, norm_epsilon, x, rms, q, k, v)
+    q = q.view(rows, heads, dim)
+    append_kv(k_pages, v_pages, k.view(rows, heads_kv, dim), v.view(rows, heads_kv, dim), tables, lens, cu_q=cu_q, q=q,
+              rope=rope, interleaved=interleaved, q_out=q)
+    mixed = attention(q, k_pages, v_pages, tables, lens, cu_q=cu_q, max_q=max_q, window=window, sinks=sinks)
+    if output is None:
+        output = torch.empty((rows, ho.N), dtype=x.dtype, device=x.device)
+    return ho.gemm(mixed.view(rows, ho.K), output)
 
 
 def _ids(x: PageIds) -> torch.Tensor:
