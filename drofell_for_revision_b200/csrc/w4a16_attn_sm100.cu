@@ -825,27 +825,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-            uint32_t again = __ballot_sync(0xffffffffu, odd && live_row);
-            while (again) {
-                const int r = row - lane + __ffs(again) - 1;
-                again &= again - 1;
-                __syncwarp();
-                const int token = r / a.group, head = it.h * a.group + r - token * a.group;
-                const RowSum x = careful_row<kTileKeys, BF16>(a, it.b, it.h, (it.t0 + token) * a.q_token + head * a.q_head,
-                                                              it.p0 + token, vw.kt, it.j0, it.j1);
-                if (part) {
-                    const int rr = r - it.row0;
-                    if (lane == 0) {
-                        slot[rr] = x.m;
-                        slot[2 * kTileRows + rr] = x.l;
-                    }
-                    if (lane * 4 < DP)
-                        *reinterpret_cast<float4*>(slot + 4 * kTileRows + rr * DP + lane * 4) =
-                            make_float4(x.o[0], x.o[1], x.o[2], x.o[3]);
-                } else {
-                    x.store<BF16>(a, (it.t0 + token) * a.o_token + head * a.o_head);
-                }
-            }
+            // rows whose sums are not finite while their sums of weights are
+            const uint32_t bad = __ballot_sync(0xffffffffu, odd && live_row && l == l);
+            if (bad)
+                settle_rows<kTileKeys, DP, BF16>(a, it.b, it.h, it.t0, it.p0, row - lane, bad, vw.kt, it.j0, it.j1, slot,
+                                                 2 * kTileRows, pr - lane);
         }
     }
 

@@ -463,29 +463,15 @@ __global__ void __launch_bounds__(kThreads, DEEP ? 1 : 2) split_kernel(const __g
                     *reinterpret_cast<uint32_t*>(a.out + out1 + d) = pack2<BF16>(o[j][2] * inv1, o[j][3] * inv1);
             }
         }
-        // A value that a row does not see must not reach it as 0 x inf or 0 x NaN, nor an infinite
-        // one as (w - rounded w) x inf. Any such product leaves a sum that is not finite: the row is
-        // then taken once more, key by key.
-        const uint32_t odd0 = __ballot_sync(0xffffffffu, !(sum0 == 0.f)), odd1 = __ballot_sync(0xffffffffu, !(sum1 == 0.f));
+        // bits: rows of the row tile whose sums are not finite while their sums of weights are
+        const uint32_t odd0 = __ballot_sync(0xffffffffu, !(sum0 == 0.f) && r0 < rows && l0 == l0);
+        const uint32_t odd1 = __ballot_sync(0xffffffffu, !(sum1 == 0.f) && r1 < rows && l1 == l1);
         if (odd0 | odd1) {
-            const int rt = at.rt;
+            uint32_t bad = 0;
 #pragma unroll 1
-            for (int r = 0; r < kRows; ++r) {
-                const int row = rt * kRows + r, token = row / a.group, head = h * a.group + row - token * a.group;
-                if (row >= rows || (((r < 8 ? odd0 : odd1) >> ((r & 7) * 4)) & 15u) == 0) continue;
-                const RowSum x = careful_row<kTile, BF16>(a, at.b, h, (at.sq.t0 + token) * a.q_token + head * a.q_head,
-                                                          at.sq.p0 + token, at.kt, tile0, tile1);
-                if (part) {
-                    if (lane == 0) {
-                        ws[r] = x.m;
-                        ws[kRows + r] = x.l;
-                    }
-                    if (lane * 4 < DP)
-                        *reinterpret_cast<float4*>(ws + 2 * kRows + r * DP + lane * 4) = make_float4(x.o[0], x.o[1], x.o[2], x.o[3]);
-                } else {
-                    x.store<BF16>(a, (at.sq.t0 + token) * a.o_token + head * a.o_head);
-                }
-            }
+            for (int r = 0; r < kRows; ++r)
+                if (((r < 8 ? odd0 : odd1) >> ((r & 7) * 4)) & 15u) bad |= 1u << r;
+            settle_rows<kTile, DP, BF16>(a, at.b, h, at.sq.t0, at.sq.p0, at.rt * kRows, bad, at.kt, tile0, tile1, ws, kRows, 0);
         }
         done += tile1 - tile0;
         if (done >= end) break;

@@ -64,6 +64,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
         b = lo;
     }
     const Seq sq = load_seq(a.seqs, a.pages.page_shift, b);
+    if (t < sq.t0 || t - sq.t0 >= sq.nq) return;  // offsets that do not ascend
     const int pos = sq.p0 + (t - sq.t0);
     int page = -1;
     if (pos >= 0) page = a.seqs.tables[b * a.seqs.table_stride + (pos >> a.pages.page_shift)];

@@ -103,9 +103,8 @@ struct RowSum {
     }
 };
 
-// One row over key tiles [i0, i1), key by key and each key by selection: for rows whose sums
-// are not finite because a product took in a value that the row does not see. A warp a row,
-// lanes over the head's dimensions. Slow, and as rare as infinities and NaN are.
+// One row over key tiles [i0, i1), key by key and each key by selection. A warp a row, lanes
+// over the head's dimensions. Slow: see settle_rows.
 template <int TILE, bool BF16>
 __device__ __noinline__ RowSum careful_row(const AttnArgs& a, int b, int h, int64_t q_off, int p, const KeyTiles<TILE> kt,
                                            int i0, int i1) {
@@ -148,6 +147,106 @@ __device__ __noinline__ RowSum careful_row(const AttnArgs& a, int b, int h, int6
         }
     }
     return r;
+}
+
+// Rows whose weighted sums are not finite although their sums of weights are, a bit each from
+// row `first_row` on: either a value that the row sees is not finite, and so the result, or a
+// product took one in that it does not see (0 x inf, 0 x NaN), or split an infinite one's
+// weight in two parts (inf - inf). The infinities and NaN among the values that the rows see are
+// looked for, once for the keys that all of them see; they decide their dimensions. Only a row
+// with others that are not finite is computed anew. The rows' results (part: their parts, with
+// `part_rows` rows to an array, the first of them `part_row`) are read back and set right.
+template <int TILE, int DP, bool BF16>
+__device__ __noinline__ void settle_rows(const AttnArgs& a, int b, int h, int t0, int p0, int first_row, uint32_t bad,
+                                         const KeyTiles<TILE> kt, int i0, int i1, float* part, int part_rows, int part_row) {
+    const int lane = threadIdx.x & 31, d = lane * 4;
+    const bool in = d < a.pages.dim;
+    __syncwarp();
+    int p_min = 0x7fffffff, p_max = -1;
+    for (uint32_t left = bad; left; left &= left - 1) {
+        const int p = max(-1, p0 + (first_row + __ffs(left) - 1) / a.group);
+        p_min = min(p_min, p);
+        p_max = max(p_max, p);
+    }
+    auto all_see = [&](int k0, int k1) {  // keys k0 .. k1, by every one of the rows
+        return k1 <= p_min && (a.window == 0 || p_max - k0 < a.window || k1 < a.sinks);
+    };
+    const int32_t* table = a.seqs.tables + b * a.seqs.table_stride;
+    // what key j's values are not: bits 0-3 NaN, 4-7 +inf, 8-11 -inf
+    auto kinds = [&](int j) {
+        const int page = table[j >> a.pages.page_shift];
+        if (page < 0 || page >= a.pages.num_pages || !in) return 0u;
+        const uint2 r = *reinterpret_cast<const uint2*>(a.pages.v + page * a.pages.stride_page + h * a.pages.stride_head +
+                                                        (j & ((1 << a.pages.page_shift) - 1)) * a.pages.stride_token + d);
+        const float2 u = unpack2<BF16>(r.x), v = unpack2<BF16>(r.y);
+        const float x[4] = {u.x, u.y, v.x, v.y};
+        uint32_t f = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f |= (x[e] != x[e] ? 1u : x[e] == INFINITY ? 16u : x[e] == -INFINITY ? 256u : 0u) << e;
+        return f;
+    };
+    uint32_t shared = 0;
+#pragma unroll 1
+    for (int i = i0; i < i1; ++i) {
+        const int k0 = kt.first(i);
+        if (!all_see(k0, k0 + TILE - 1)) continue;
+#pragma unroll 4
+        for (int c = 0; c < TILE; ++c) shared |= kinds(k0 + c);
+    }
+#pragma unroll 1
+    for (; bad; bad &= bad - 1) {
+        const int bit = __ffs(bad) - 1, row = first_row + bit, token = row / a.group;
+        const int head = h * a.group + row - token * a.group, p = max(-1, p0 + token);
+        uint32_t f = shared;
+#pragma unroll 1
+        for (int i = i0; i < i1; ++i) {
+            const int k0 = kt.first(i);
+            if (all_see(k0, k0 + TILE - 1) || k0 > p) continue;
+#pragma unroll 1
+            for (int c = 0; c < TILE; ++c)
+                if (visible(k0 + c, p, a.window, a.sinks)) f |= kinds(k0 + c);
+        }
+        const int64_t o_off = static_cast<int64_t>(t0 + token) * a.o_token + head * a.o_head + d;
+        float* slot = part ? part + 2 * part_rows + (part_row + bit) * DP + d : nullptr;
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        if (in && part) {
+            const float4 v = *reinterpret_cast<const float4*>(slot);
+            x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+        } else if (in) {
+            const uint2 r = *reinterpret_cast<const uint2*>(a.out + o_off);
+            const float2 u = unpack2<BF16>(r.x), v = unpack2<BF16>(r.y);
+            x[0] = u.x, x[1] = u.y, x[2] = v.x, x[3] = v.y;
+        }
+        bool anew = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t k = (f >> e) & 0x111u;
+            if (k == 0) {
+                anew |= !(x[e] * 0.f == 0.f);
+            } else {
+                x[e] = k == 16u ? INFINITY : k == 256u ? -INFINITY : NAN;
+            }
+        }
+        if (__any_sync(0xffffffffu, anew)) {
+            const RowSum r = careful_row<TILE, BF16>(a, b, h, static_cast<int64_t>(t0 + token) * a.q_token + head * a.q_head, p, kt,
+                                                     i0, i1);
+            if (part == nullptr) {
+                r.store<BF16>(a, o_off - d);
+                continue;
+            }
+            if (lane == 0) {
+                part[part_row + bit] = r.m;
+                part[part_rows + part_row + bit] = r.l;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = r.o[e];
+        }
+        if (in && part) {
+            *reinterpret_cast<float4*>(slot) = make_float4(x[0], x[1], x[2], x[3]);
+        } else if (in) {
+            *reinterpret_cast<uint2*>(a.out + o_off) = make_uint2(pack2<BF16>(x[0], x[1]), pack2<BF16>(x[2], x[3]));
+        }
+    }
 }
 
 }  // namespace w4a16

@@ -226,6 +226,7 @@ int w4a16_paged_attention(const w4a16_pages* pages, const w4a16_seqs* seqs, cons
     rc = check_rows(q, "q");
     if (rc == W4A16_OK) rc = check_rows(out, "out");
     if (rc != W4A16_OK) return rc;
+    if (q->dev == out->dev) return report_error(W4A16_ERR_INVALID, "out must not be q");
     AttnArgs a = attn_args(pages, seqs, heads, window, sinks);
     a.q = static_cast<const uint16_t*>(q->dev);
     a.q_token = q->stride_token, a.q_head = q->stride_head;

@@ -287,7 +287,7 @@ W4A16_API int w4a16_append_kv(const w4a16_pages* pages, const w4a16_seqs* seqs, 
 /* out = softmax(scale q k^T) v (scale > 0) of every new token over the visible tokens of its sequence:
  * not after it, and with window > 0 the last `window` ones (itself counted) and the first
  * `sinks` ones. heads is a multiple of heads_kv; query head i reads key-value head
- * i / (heads / heads_kv). Rows that see nothing are 0. Softmax statistics and sums in
+ * i / (heads / heads_kv); out must not overlap q. Rows that see nothing are 0. Softmax statistics and sums in
  * fp32. No host synchronisation and no allocation: capturable. Calls that may overlap on
  * the GPU need workspaces of their own; a workspace is 32-byte aligned, its contents mean
  * nothing before and after a call. */

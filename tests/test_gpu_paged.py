@@ -110,7 +110,7 @@ def check_attention(bt, window=0, sinks=0, scale=None, out=None, hide=None):
     finite = torch.isfinite(want)
     assert torch.equal(torch.isnan(got), torch.isnan(want))
     assert torch.equal(got.double()[~finite & ~torch.isnan(want)], want[~finite & ~torch.isnan(want)])
-    top = max(1.0, float(bt.v[torch.isfinite(bt.v)].abs().max()))
+    top = max(1.0, float(torch.nan_to_num(bt.v, 0.0, 0.0, 0.0).abs().max()))
     room = half * want.abs() + half * spread + 1e-5 * top
     bad = finite & ((got.double() - want).abs() > room)
     assert not bad.any(), float(((got.double() - want).abs() / room)[finite].max())
@@ -148,7 +148,7 @@ def test_few_tokens(dtype, window, sinks):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("heads,heads_kv,dim,page", [(4, 4, 128, 16), (16, 2, 128, 128), (14, 2, 64, 8), (6, 2, 96, 64),
-                                                     (7, 1, 80, 256)])
+                                                     (7, 1, 80, 256), (3, 3, 8, 32), (6, 2, 40, 16), (4, 1, 120, 8)])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (50, 3), (300, 200)])
 def test_prompts(dtype, heads, heads_kv, dim, page, window, sinks):
     check_attention(Batch([1, 130, 128, 77, 700, 513], [1, 130, 128, 40, 333, 1], heads, heads_kv, dim, page, dtype,
@@ -249,6 +249,53 @@ def test_a_value_reaches_only_the_rows_that_see_it(value, new, old, window):
     for j in (new + old - 3, old + 1, old + new // 2):
         bt.v[int(bt.tables[0, j // 16]), :, j % 16, 5] = value
     check_attention(bt, window)
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("what", ["q", "k", "v", "some v"])
+@pytest.mark.parametrize("new,old", [(1, 3000), (4, 200), (150, 2000), (700, 0)])
+def test_data_that_is_not_finite(value, what, new, old):
+    """Results that are not finite by right come out so, and as fast as others within reason (a
+    poisoned batch must not look like a hang)."""
+    bt = Batch([new + old, 50], [new, 1], 8, 2, 128, 32, torch.bfloat16, seed=59)
+    if what == "q":
+        bt.q[0, 0] = value
+    elif what == "k":
+        bt.k.fill_(value)
+    elif what == "v":
+        bt.v.fill_(value)
+    else:
+        bt.v[:, 1, :, 3] = value
+        bt.v[::2, 0, 5, 7] = -value
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    paged.attention(bt.q, bt.k, bt.v, bt.tables, bt.lens, cu_q=bt.cu_q, max_q=bt.max_q)
+    start.record()
+    got = paged.attention(bt.q, bt.k, bt.v, bt.tables, bt.lens, cu_q=bt.cu_q, max_q=bt.max_q)
+    end.record()
+    torch.cuda.synchronize()
+    assert start.elapsed_time(end) < 200
+    if what in ("q", "k"):
+        # scores are then NaN or infinite: no weights to speak of, but rows of other queries stand
+        assert torch.isnan(got[0, 0]).all() if value != value else True
+        if what == "q":
+            assert torch.isfinite(got[:, 1:]).all()
+        elif value != value:
+            assert torch.isnan(got).all()
+    else:
+        check_attention(bt)
+
+
+def test_offsets_that_do_not_ascend():
+    """Row offsets of any values: no access out of range, other sequences stand."""
+    bt = Batch([60, 90, 40], [3, 5, 4], 4, 2, 64, 16, torch.float16, seed=61)
+    kn = torch.randn(12, 2, 64, device=DEV).half()
+    for cu in ([0, 9, 2, 12], [-5, 3, 8, 1 << 30], [7, 3, -1, 4], [12, 12, 12, 12], [1 << 30, 5, 5, -(1 << 31)]):
+        cu_q = torch.tensor(cu, dtype=torch.int32, device=DEV)
+        paged.append_kv(bt.k, bt.v, kn, kn, bt.tables, bt.lens, cu_q=cu_q, q=bt.q)
+        for max_q in (5, 40, 300):
+            assert paged.attention(bt.q, bt.k, bt.v, bt.tables, bt.lens, cu_q=cu_q, max_q=max_q).shape == bt.q.shape
+    torch.cuda.synchronize()
+    check_attention(Batch([60, 90, 40], [3, 5, 4], 4, 2, 64, 16, torch.float16, seed=61))
 
 
 def test_pages_that_are_no_pages():

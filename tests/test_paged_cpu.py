@@ -33,8 +33,8 @@ def rows(**kw):
 
 def attention(p=None, s=None, q=None, out=None, heads=4, scale=0.1, window=0, sinks=0, ws=None, n=0):
     ref = lambda x: ctypes.byref(x) if x is not None else None  # noqa: E731
-    return _capi.lib().w4a16_paged_attention(ref(p or pages()), ref(s or seqs()), ref(q or rows()), ref(out or rows()),
-                                             heads, scale, window, sinks, ws, n, None)
+    return _capi.lib().w4a16_paged_attention(ref(p or pages()), ref(s or seqs()), ref(q or rows()),
+                                             ref(out or rows(dev=2 * FAKE)), heads, scale, window, sinks, ws, n, None)
 
 
 def append(p=None, s=None, k=None, v=None, q=None, q_out=None, heads=4, rope=None, positions=0, dim=0, inter=0):
@@ -76,6 +76,7 @@ def test_attention_arguments_are_checked():
     assert attention(q=rows(dev=None)) == INVALID
     assert attention(out=rows(stride_head=4)) == INVALID
     assert attention(out=rows(dev=FAKE + 2)) == INVALID
+    assert attention(out=rows(dev=FAKE)) == INVALID  # q itself
     assert attention(s=seqs(cu_q_dev=FAKE, max_q=(1 << 31) - 1, tokens=5)) == UNSUPPORTED
     assert _capi.lib().w4a16_paged_error(0, None, None) == INVALID
     # nothing to do: no CUDA call
