@@ -43,6 +43,7 @@ constexpr int kLoadWarp = 8, kCleanWarp = 9, kMmaWarp = 10;  // kMmaWarp + t: ro
 // 384 * 168 that the CTA was launched with.
 constexpr int kLaunchRegs = 168, kSoftmaxRegs = 208, kOtherRegs = 88;
 static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "more registers than launched with");
+constexpr int kPostInts = 17;      // of an item and its view
 constexpr int kBlock = 128 * 128;  // bytes of a [128 rows x 64] operand block, 128-byte swizzle
 constexpr uint32_t kWaitLimit = 1u << 18;  // x ~10 us sleeps: a few seconds
 constexpr float kSlack = 8.f;              // log2 of the growth that O tolerates without rescaling
@@ -57,7 +58,8 @@ struct Cfg {
     static constexpr int kSlots = DP == 128 ? 5 : 8;     // K and V tiles in turn
     static constexpr int kKvOff = 2 * kTileBytes;
     static constexpr int kBarOff = kKvOff + kSlots * kTileBytes;
-    static constexpr int kListOff = kBarOff + 384;           // barriers and posted items before it
+    static constexpr int kListOff = kBarOff + 512;           // barriers and posted items before it
+    static_assert((2 * kSlots + 18) * 8 + 4 + 8 * 4 + 2 * kPostInts * 4 <= kListOff - kBarOff, "barriers and posted items");
     static constexpr int kSmem = kListOff + (kThreads + 1) * 4 + 1020;  // and alignment
     static_assert(kSmem <= 227 * 1024, "shared memory budget");
     // TMEM columns: S of both row tiles (P in their first 64), O of both
@@ -218,6 +220,7 @@ struct View {
     int first_seen;        // first key of the earliest window
     int window, sinks;
     KeyTiles<kTileKeys> kt;
+    __device__ __forceinline__ View() : kt(0, -1, 0, 0) {}
     __device__ __forceinline__ View(const Item& it, const AttnArgs& a)
         : last(it.p0 + (min(it.rows, it.row0 + 2 * kTileRows) - 1) / a.group),
           first_seen(a.window ? max(0, max(it.p0 + it.row0 / a.group, 0) + 1 - a.window) : 0),
@@ -305,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* turn = iempty + 2;    // [2] a row tile's turn at the tensor cores
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + 2);
     volatile uint32_t* bad = tmem_slot + 1;                         // [8] boxes of tile j % 8 whose page id is no page
-    volatile int* posted = reinterpret_cast<volatile int*>(bad + 8);  // [2][8] items; b = -1: no more
+    volatile int* posted = reinterpret_cast<volatile int*>(bad + 8);  // [2][kPostInts] items; b = -1: no more
     int* before = reinterpret_cast<int*>(smem + C::kListOff);       // [kThreads + 1] items before a thread's sequences
 
     ptx::grid_dep_wait();
@@ -361,20 +364,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = *tmem_slot;
     int* err = &g_attention_error;
 
-    // Item k of this CTA as the loading warp posted it; false: there is none (or a wait gave up).
-    auto next_item = [&](int k, Item& it, bool whole_warp) {
+    // Item k of this CTA and its view as the loading warp posted them; false: there is none (or a
+    // wait gave up).
+    auto next_item = [&](int k, Item& it, View& vw, bool whole_warp) {
         const int s = k & 1, parity = (k >> 1) & 1;
         bool ok = wait(&ifull[s], parity, err, kErrLoad);
         if (whole_warp) ok = __all_sync(0xffffffffu, ok);
         if (!ok) return false;
-        it.b = posted[s * 8];
-        it.h = posted[s * 8 + 1];
-        it.row0 = posted[s * 8 + 2];
-        it.rows = posted[s * 8 + 3];
-        it.t0 = posted[s * 8 + 4];
-        it.p0 = posted[s * 8 + 5];
-        it.j0 = posted[s * 8 + 6];
-        it.j1 = posted[s * 8 + 7];
+        volatile int* x = posted + s * kPostInts;
+        it.b = x[0], it.h = x[1], it.row0 = x[2], it.rows = x[3], it.t0 = x[4], it.p0 = x[5], it.j0 = x[6], it.j1 = x[7];
+        vw.p_lo[0] = x[8], vw.p_lo[1] = x[9], vw.p_hi[0] = x[10], vw.p_hi[1] = x[11];
+        vw.last = x[12], vw.first_seen = x[13], vw.window = a.window, vw.sinks = a.sinks;
+        vw.kt.sink_tiles = x[14], vw.kt.win_tile = x[15], vw.kt.count = x[16];
         if (whole_warp) __syncwarp();
         if (!whole_warp || lane == 0) ptx::mbar_arrive(&iempty[s]);
         return it.b >= 0;
@@ -414,6 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (k > rounds) at = total;
                 }
                 Item it;
+                View vw;
                 it.b = -1;
                 it.h = it.row0 = it.rows = it.t0 = it.p0 = it.j0 = it.j1 = 0;
                 if (at < total) {
@@ -436,7 +438,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     it.rows = sq.nq * a.group;
                     it.t0 = sq.t0;
                     it.p0 = sq.p0;
-                    const int n = View(it, a).kt.count;
+                    vw = View(it, a);
+                    const int n = vw.kt.count;
                     pieces = min(pieces, max(1, n / kPieceTiles));
                     if (piece < pieces) {
                         it.j0 = static_cast<int>(static_cast<int64_t>(n) * piece / pieces);
@@ -453,18 +456,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int s = k & 1;
                 if (k >= 2) ok = warp_wait(&iempty[s], ((k >> 1) - 1) & 1, err, kErrLoad);
                 if (lane == 0) {
-                    posted[s * 8] = ok ? it.b : -1;
-                    posted[s * 8 + 1] = it.h;
-                    posted[s * 8 + 2] = it.row0;
-                    posted[s * 8 + 3] = it.rows;
-                    posted[s * 8 + 4] = it.t0;
-                    posted[s * 8 + 5] = it.p0;
-                    posted[s * 8 + 6] = it.j0;
-                    posted[s * 8 + 7] = it.j1;
+                    volatile int* x = posted + s * kPostInts;
+                    x[0] = ok ? it.b : -1, x[1] = it.h, x[2] = it.row0, x[3] = it.rows, x[4] = it.t0, x[5] = it.p0;
+                    x[6] = it.j0, x[7] = it.j1, x[8] = vw.p_lo[0], x[9] = vw.p_lo[1], x[10] = vw.p_hi[0], x[11] = vw.p_hi[1];
+                    x[12] = vw.last, x[13] = vw.first_seen;
+                    x[14] = vw.kt.sink_tiles, x[15] = vw.kt.win_tile, x[16] = vw.kt.count;
                     ptx::mbar_arrive(&ifull[s]);
                 }
                 if (it.b < 0 || !ok) break;
-                const View vw(it, a);
                 const int32_t* table = a.seqs.tables + it.b * a.seqs.table_stride;
                 auto page_of = [&](int j) {  // this lane's page of key tile j
                     int page = a.pages.num_pages;  // behind the cache's end: zeros
@@ -531,9 +530,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             int i = 0, asked = 0;
             bool ok = true;
             Item it;
+            View vw;
 #pragma unroll 1
-            for (int k = 0; ok && next_item(k, it, true); ++k) {
-                const View vw(it, a);
+            for (int k = 0; ok && next_item(k, it, vw, true); ++k) {
                 if (!q_by_tma) {
                     if (k > 0) ok = warp_wait(qempty, (k - 1) & 1, err, kErrMma);
                     if (!ok) break;
@@ -597,12 +596,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 return x < 0 || wait(&turn[t], x & 1, err, kErrMma);
             };
             Item it;
+            View vw;
 #pragma unroll 1
-            for (int k = 0; ok && next_item(k, it, false); ++k) {
-                const View vw(it, a);
+            for (int k = 0; ok && next_item(k, it, vw, false); ++k) {
                 const int n = it.j1 - it.j0;  // j counts from the item's first tile
                 ok = wait(qfull, k & 1, err, kErrMma);
-                bool first = true;
+                bool first = true, ended = false;
                 // step j: P V of tile j - 1, then the scores of tile j
 #pragma unroll 1
                 for (int j = 0; j <= n && ok; ++j, i += 2) {
@@ -634,6 +633,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                         half_product(1);
                         ++done;
                         first = false;
+                        // the row tile's last product: its epilogue need not wait for the other's
+                        if (j < n && k0 > vw.p_hi[t]) {
+                            ptx::umma_commit(&ofull[t]);
+                            ended = true;
+                        }
                     } else if (ok) {
                         ok = my_turn();
                     }
@@ -663,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 i -= 2;  // step n has no K
                 if (n == 0) ptx::umma_commit(qempty);
-                ptx::umma_commit(&ofull[t]);
+                if (!ended) ptx::umma_commit(&ofull[t]);
             }
         }
         __syncwarp();
@@ -679,9 +683,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         int i = 0, seen = 0;  // tiles of keys; scores taken
         bool ok = true;
         Item it;
+        View vw;
 #pragma unroll 1
-        for (int k = 0; ok && next_item(k, it, true); ++k) {
-            const View vw(it, a);
+        for (int k = 0; ok && next_item(k, it, vw, true); ++k) {
             const bool part = it.j1 - it.j0 < vw.kt.count;
             const int row = it.row0 + t * kTileRows + tid;
             const bool live_row = row < it.rows;
