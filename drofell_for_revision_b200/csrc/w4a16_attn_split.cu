@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, DEEP ? 1 : 2) split_kernel(const __g
 // rows, take a share of its rows and add the pieces in worker order, a warp a row or several
 // when there are many pieces. A warp has eight pieces in flight at once: latency is all there
 // is to it.
-constexpr int kJoinWarps = 8, kJoinPieces = 8;
+constexpr int kJoinWarps = 4, kJoinPieces = 8;
 
 template <int DP, bool BF16>
 __global__ void __launch_bounds__(kJoinWarps * 32) split_join_kernel(const __grid_constant__ AttnArgs a) {
@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) split_join_kernel(const __gri
     const int pieces = last - first + 1, mine = worker - first - 1;
     const int rows = min(kRows, d1.w - rt * kRows);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int per_row = pieces > 4 * kJoinPieces ? 8 : pieces > 2 * kJoinPieces ? 4 : pieces > kJoinPieces ? 2 : 1;  // warps
+    const int per_row = pieces > 2 * kJoinPieces ? 4 : pieces > kJoinPieces ? 2 : 1;  // warps
     const int at_once = kJoinWarps / per_row, sub = warp % per_row;
 #pragma unroll 1
     for (int q = 0; mine + q * (pieces - 1) < rows; q += at_once) {
