@@ -8,7 +8,8 @@
 namespace w4a16 {
 namespace {
 
-constexpr int kAppendThreads = 128;  // 5 prompts of 5020 tokens: 17.0 us, 19.7 at 256
+constexpr int kAppendHeads = 2;  // read ahead: the same prompts 17.5 us, 18.5 at 1, 18.6 at 3
+constexpr int kAppendThreads = 128;  // 5 prompts, 5020 tokens, 64 + 8 + 8 heads: 18.6 us, 21 at 256
 
 // (x_a, x_b) -> (x_a c - x_b s, x_b c + x_a s): one pair of 8-element chunks, or the four
 // pairs inside each chunk when interleaved. fp32, rounded once.
@@ -47,6 +48,27 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     const int slot = threadIdx.x % slots;
     const int rows = kAppendThreads / slots;
     if (threadIdx.x >= rows * slots) return;
+    const bool pair = slot < half;
+    const int c0 = (pair ? slot : slot + half) * 8, c1 = (slot + half) * 8;
+
+    // a few heads at a time, read before anything is known of where they go
+    const int heads_q = a.q ? a.heads : 0, hkv = a.pages.heads_kv, all = heads_q + 2 * hkv;
+    const int stride = rows * gridDim.y;
+    uint4 x[kAppendHeads], y[kAppendHeads];
+    auto load = [&](int r) {
+#pragma unroll
+        for (int i = 0; i < kAppendHeads; ++i) {
+            const int at = r + i * stride;
+            if (at >= all) break;
+            const uint16_t* src = at < heads_q ? a.q + t * a.q_token + at * a.q_head
+                                  : at < heads_q + hkv ? a.k + t * a.k_token + (at - heads_q) * a.k_head
+                                                       : a.v + t * a.v_token + (at - heads_q - hkv) * a.v_head;
+            x[i] = *reinterpret_cast<const uint4*>(src + c0);
+            if (pair) y[i] = *reinterpret_cast<const uint4*>(src + c1);
+        }
+    };
+    int r = blockIdx.y * rows + threadIdx.x / slots;
+    load(r);
 
     // the token's sequence: the last one that begins at or before row t
     int b = t;
@@ -68,58 +90,45 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     const int pos = sq.p0 + (t - sq.t0);
     int page = -1;
     if (pos >= 0) page = a.seqs.tables[b * a.seqs.table_stride + (pos >> a.pages.page_shift)];
-    const bool store = page >= 0 && page < a.pages.num_pages;  // a token of no valid page is not stored
-    const int64_t cache = store ? page * a.pages.stride_page +
-                                      (pos & ((1 << a.pages.page_shift) - 1)) * a.pages.stride_token
-                                : 0;
 
-    const bool pair = slot < half;
     const bool turn = a.rope && pos >= 0 && (pair || (a.interleaved && slot * 8 < a.rope_dim));
-    const int c0 = (pair ? slot : slot + half) * 8, c1 = (slot + half) * 8;
     float c[8], s[8];
     if (turn) {
         const float* row = a.rope + static_cast<int64_t>(pos) * a.rope_dim;
         const int n = pair ? 8 : 4, first = pair ? slot * 8 : slot * 4;
         for (int i = 0; i < 8; i += 4) {
             if (i < n) {
-                const float4 x = *reinterpret_cast<const float4*>(row + first + i);
-                const float4 y = *reinterpret_cast<const float4*>(row + (a.rope_dim >> 1) + first + i);
-                c[i] = x.x, c[i + 1] = x.y, c[i + 2] = x.z, c[i + 3] = x.w;
-                s[i] = y.x, s[i + 1] = y.y, s[i + 2] = y.z, s[i + 3] = y.w;
+                const float4 u = *reinterpret_cast<const float4*>(row + first + i);
+                const float4 w = *reinterpret_cast<const float4*>(row + (a.rope_dim >> 1) + first + i);
+                c[i] = u.x, c[i + 1] = u.y, c[i + 2] = u.z, c[i + 3] = u.w;
+                s[i] = w.x, s[i + 1] = w.y, s[i + 2] = w.z, s[i + 3] = w.w;
             }
         }
     }
-
-    const int heads_q = a.q ? a.heads : 0;
-    const int all = heads_q + 2 * a.pages.heads_kv;
-    for (int r = blockIdx.y * rows + threadIdx.x / slots; r < all; r += rows * gridDim.y) {
-        const uint16_t* src;
-        uint16_t* dst;
-        bool rot = turn;
-        if (r < heads_q) {
-            src = a.q + t * a.q_token + r * a.q_head;
-            dst = a.q_out + t * a.qo_token + r * a.qo_head;
-        } else if (!store) {
-            break;  // the k and v heads come last
-        } else if (r < heads_q + a.pages.heads_kv) {
-            const int h = r - heads_q;
-            src = a.k + t * a.k_token + h * a.k_head;
-            dst = a.k_out + cache + h * a.pages.stride_head;
-        } else {
-            const int h = r - heads_q - a.pages.heads_kv;
-            src = a.v + t * a.v_token + h * a.v_head;
-            dst = a.v_out + cache + h * a.pages.stride_head;
-            rot = false;
+    const bool store = page >= 0 && page < a.pages.num_pages;  // a token of no valid page is not stored
+    const int64_t cache = store ? page * a.pages.stride_page +
+                                      (pos & ((1 << a.pages.page_shift) - 1)) * a.pages.stride_token
+                                : 0;
+    const int end = store ? all : heads_q;  // the k and v heads come last
+    while (r < end) {
+#pragma unroll
+        for (int i = 0; i < kAppendHeads; ++i) {
+            const int at = r + i * stride;
+            if (at >= end) break;
+            uint16_t* dst = at < heads_q ? a.q_out + t * a.qo_token + at * a.qo_head
+                            : at < heads_q + hkv ? a.k_out + cache + (at - heads_q) * a.pages.stride_head
+                                                 : a.v_out + cache + (at - heads_q - hkv) * a.pages.stride_head;
+            const bool rot = turn && at < heads_q + hkv;
+            if (pair) {
+                if (rot) rotate_halves<BF16>(x[i], y[i], c, s);
+                *reinterpret_cast<uint4*>(dst + c1) = y[i];
+            } else if (rot) {
+                rotate_pairs<BF16>(x[i], c, s);
+            }
+            *reinterpret_cast<uint4*>(dst + c0) = x[i];
         }
-        uint4 x = *reinterpret_cast<const uint4*>(src + c0);
-        if (pair) {
-            uint4 y = *reinterpret_cast<const uint4*>(src + c1);
-            if (rot) rotate_halves<BF16>(x, y, c, s);
-            *reinterpret_cast<uint4*>(dst + c1) = y;
-        } else if (rot) {
-            rotate_pairs<BF16>(x, c, s);
-        }
-        *reinterpret_cast<uint4*>(dst + c0) = x;
+        r += kAppendHeads * stride;
+        if (r < end) load(r);
     }
 }
 
