@@ -591,12 +591,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!vw.cut(k0)) continue;
                     ok = warp_wait(dirty, asked++ & 1, err, kErrMma);
                     const uint32_t v = ptx::smem_u32(smem + C::kKvOff + ((i + 1) % SL) * C::kTileBytes);
-#pragma unroll 1
-                    for (int x = lane; ok && x < kTileKeys * CH; x += 32) {
-                        const int r = x / CH, c = x % CH, key = k0 + r;
-                        if (key > vw.last || (key < vw.first_seen && key >= a.sinks))
-                            ptx::st_shared_v4(v + (c >> 3) * kBlock + r * 128 + (c & 7) * 16, make_uint4(0, 0, 0, 0));
-                    }
+                    // rows [r, r1) of the tile: behind the last key, then between the sinks and the window
+                    auto zero = [&](int r, int r1) {
+#pragma unroll 4
+                        for (r += lane / CH; r < r1; r += 32 / CH)
+                            ptx::st_shared_v4(v + (lane % CH >> 3) * kBlock + r * 128 + (lane & 7) * 16, make_uint4(0, 0, 0, 0));
+                    };
+                    if (ok) zero(max(0, vw.last + 1 - k0), kTileKeys);
+                    if (ok) zero(max(0, a.sinks - k0), min(kTileKeys, vw.first_seen - k0));
                     ptx::fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) ptx::mbar_arrive(clean);
