@@ -423,125 +423,139 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int ctas = gridDim.x;
             int i = 0, q_loads = 0;  // tiles of K and V, row pairs of Q so far
             bool ok = true;
-#pragma unroll 1
-            for (int k = 0; ok; ++k) {
-                // rounds of the CTAs run forth and back over the items, whose work falls along a
-                // sequence: a CTA's shares even out. Where there are few rounds, the items of the last,
-                // incomplete one are cut along their keys, among all CTAs.
-                int64_t at = static_cast<int64_t>(k) * ctas + ((k & 1) ? ctas - 1 - static_cast<int>(blockIdx.x) : blockIdx.x);
-                int pieces = 1, piece = 0;
-                const int rounds = total / ctas, rest_items = total - rounds * ctas;
-                if (may_split && rounds < kSplitRounds && k >= rounds) {
-                    pieces = rest_items > 0 ? ctas / rest_items : 1;
-                    piece = static_cast<int>(blockIdx.x) % pieces;
-                    at = static_cast<int64_t>(rounds) * ctas + static_cast<int>(blockIdx.x) / pieces;
-                    if (k > rounds) at = total;
+            Item it, nx;  // the item whose tiles are loaded, and the next
+            View vw, vx;
+            it.b = nx.b = -1;
+            it.j0 = it.j1 = nx.j0 = nx.j1 = 0;
+            auto page_of = [&](const Item& x, const View& v, int j) {  // this lane's page of key tile j
+                int page = a.pages.num_pages;  // behind the cache's end: zeros
+                if (j < x.j1 && lane < boxes) {
+                    const int key = v.kt.first(j) + lane * box;
+                    if (key <= v.last) page = a.seqs.tables[x.b * a.seqs.table_stride + (key >> a.pages.page_shift)];
                 }
-                Item it;
-                View vw;
-                it.b = -1;
-                it.h = it.row0 = it.rows = it.t0 = it.p0 = it.j0 = it.j1 = 0;
-                if (at < total) {
-                    // the thread whose sequences hold it: how many end at or before it
-                    int holder = 0;
+                return page;
+            };
+            int page = 0, nx_page = 0;
+            // item k's tiles; behind its first one and Q, item k + 1 is planned and posted, so that
+            // nobody waits for it (k = -1: only that)
 #pragma unroll 1
-                    for (int x = 0; x < kThreads && x * per < a.seqs.batch; x += 32)
-                        holder += __popc(__ballot_sync(0xffffffffu, before[x + lane + 1] <= at));
-                    int rest = static_cast<int>(at) - before[holder], b = holder * per;
-                    Seq sq = load_seq(a.seqs, a.pages.page_shift, b);
+            for (int k = -1; ok; ++k) {
+                bool planned = false;
 #pragma unroll 1
-                    for (int n; rest >= (n = items_of(a, sq));) {
-                        rest -= n;
-                        sq = load_seq(a.seqs, a.pages.page_shift, ++b);
-                    }
-                    const int pairs = (sq.nq * a.group + 2 * kTileRows - 1) / (2 * kTileRows);
-                    it.b = b;
-                    it.row0 = (pairs - 1 - rest / a.pages.heads_kv) * 2 * kTileRows;
-                    it.h = rest % a.pages.heads_kv;
-                    it.rows = sq.nq * a.group;
-                    it.t0 = sq.t0;
-                    it.p0 = sq.p0;
-                    vw = View(it, a);
-                    const int n = vw.kt.count;
-                    pieces = min(pieces, max(1, n / kPieceTiles));
-                    if (piece < pieces) {
-                        it.j0 = static_cast<int>(static_cast<int64_t>(n) * piece / pieces);
-                        it.j1 = static_cast<int>(static_cast<int64_t>(n) * (piece + 1) / pieces);
-                        if (pieces > 1 && lane == 0) {
-                            int4* d = reinterpret_cast<int4*>(part_desc<DP>(a, ctas, blockIdx.x));
-                            d[1] = make_int4(it.row0, it.rows, it.t0, it.h);
-                            d[0] = make_int4(1, blockIdx.x - piece, pieces, 0);
-                        }
-                    } else {
-                        it.b = -1;
-                    }
-                }
-                const int s = k & 1;
-                if (k >= 2) ok = warp_wait(&iempty[s], ((k >> 1) - 1) & 1, err, kErrLoad);
-                if (lane == 0) {
-                    volatile int* x = posted + s * kPostInts;
-                    x[0] = ok ? it.b : -1, x[1] = it.h, x[2] = it.row0, x[3] = it.rows, x[4] = it.t0, x[5] = it.p0;
-                    x[6] = it.j0, x[7] = it.j1, x[8] = vw.p_lo[0], x[9] = vw.p_lo[1], x[10] = vw.p_hi[0], x[11] = vw.p_hi[1];
-                    x[12] = vw.last, x[13] = vw.first_seen;
-                    x[14] = vw.kt.sink_tiles, x[15] = vw.kt.win_tile, x[16] = vw.kt.count;
-                    ptx::mbar_arrive(&ifull[s]);
-                }
-                if (it.b < 0 || !ok) break;
-                const int32_t* table = a.seqs.tables + it.b * a.seqs.table_stride;
-                auto page_of = [&](int j) {  // this lane's page of key tile j
-                    int page = a.pages.num_pages;  // behind the cache's end: zeros
-                    if (j < it.j1 && lane < boxes) {
+                for (int j = it.j0; ok;) {
+                    if (j < it.j1) {
                         const int key = vw.kt.first(j) + lane * box;
-                        if (key <= vw.last) page = table[key >> a.pages.page_shift];
-                    }
-                    return page;
-                };
-                int page = page_of(it.j0);
+                        const int next = page_of(it, vw, j + 1);
+                        const bool none = page < 0 || page >= a.pages.num_pages;
+                        const uint32_t none_of = __ballot_sync(0xffffffffu, none && lane < boxes && key <= vw.last);
+                        if (none) page = a.pages.num_pages;
 #pragma unroll 1
-                for (int j = it.j0; j < it.j1 && ok; ++j) {
-                    const int key = vw.kt.first(j) + lane * box;
-                    const int next = page_of(j + 1);
-                    const bool none = page < 0 || page >= a.pages.num_pages;
-                    const uint32_t none_of = __ballot_sync(0xffffffffu, none && lane < boxes && key <= vw.last);
-                    if (none) page = a.pages.num_pages;
-#pragma unroll 1
-                    for (int w = 0; w < 2; ++w, ++i) {
-                        const int sl = i % SL;
-                        if (i >= SL) ok = warp_wait(&empty[sl], ((i / SL) - 1) & 1, err, kErrLoad);
-                        if (!ok) break;
-                        if (lane == 0) {
-                            if (w == 0) bad[(i >> 1) & 7] = none_of;
-                            ptx::mbar_arrive_expect_tx(&full[sl], C::kTileBytes);
-                        }
-                        __syncwarp();
-                        if (lane < boxes) {
-                            const uint32_t dst = ptx::smem_u32(smem + C::kKvOff + sl * C::kTileBytes) + lane * box * 128;
+                        for (int w = 0; w < 2; ++w, ++i) {
+                            const int sl = i % SL;
+                            if (i >= SL) ok = warp_wait(&empty[sl], ((i / SL) - 1) & 1, err, kErrLoad);
+                            if (!ok) break;
+                            if (lane == 0) {
+                                if (w == 0) bad[(i >> 1) & 7] = none_of;
+                                ptx::mbar_arrive_expect_tx(&full[sl], C::kTileBytes);
+                            }
+                            __syncwarp();
+                            if (lane < boxes) {
+                                const uint32_t dst = ptx::smem_u32(smem + C::kKvOff + sl * C::kTileBytes) + lane * box * 128;
 #pragma unroll
-                            for (int d = 0; d < C::kBlocks; ++d)
-                                tma_load_4d(dst + d * kBlock, w ? &tm_v : &tm_k, &full[sl], d * 64, key & (page_size - 1), it.h,
-                                            page);
+                                for (int d = 0; d < C::kBlocks; ++d)
+                                    tma_load_4d(dst + d * kBlock, w ? &tm_v : &tm_k, &full[sl], d * 64, key & (page_size - 1), it.h,
+                                                page);
+                            }
                         }
+                        page = next;
+                        ++j;
                     }
-                    page = next;
-                    if (j == it.j0 && ok && q_by_tma) {
-                        // after the first keys: the rows of the last item may still be in use
+                    if (planned) {
+                        if (j >= it.j1) break;
+                        continue;
+                    }
+                    planned = true;
+                    if (k >= 0 && ok && q_by_tma) {
+                        // after the first keys: the rows of the last item may still be in use. An item
+                        // without keys takes no Q, but its phases pass all the same.
                         if (k > 0) ok = warp_wait(qempty, (k - 1) & 1, err, kErrLoad);
-                        if (ok && lane == 0) {
+                        if (ok && lane == 0 && it.j0 < it.j1) {
                             ptx::mbar_arrive_expect_tx(qfull, 2 * C::kTileBytes);
                             const int tokens = kTileRows / a.group, token = it.t0 + it.row0 / a.group;
                             for (int x = 0; x < 2 * C::kBlocks; ++x)
                                 tma_load_3d(ptx::smem_u32(smem) + x * kBlock, &tm_q, qfull, (x % C::kBlocks) * 64, it.h * a.group,
                                             token + (x / C::kBlocks) * tokens);
+                        } else if (ok && lane == 0) {
+                            ptx::mbar_arrive(qfull);
                         }
                         if (ok) ++q_loads;
                     }
+
+                    // ---- item k + 1. Rounds of the CTAs run forth and back over the items, whose work
+                    // falls along a sequence: a CTA's shares even out. Where there are few rounds, the items
+                    // of the last, incomplete one are cut along their keys, among all CTAs.
+                    const int k1 = k + 1, s = k1 & 1;
+                    int64_t at = static_cast<int64_t>(k1) * ctas + (s ? ctas - 1 - static_cast<int>(blockIdx.x) : blockIdx.x);
+                    int pieces = 1, piece = 0;
+                    const int rounds = total / ctas, rest_items = total - rounds * ctas;
+                    if (may_split && rounds < kSplitRounds && k1 >= rounds) {
+                        pieces = rest_items > 0 ? ctas / rest_items : 1;
+                        piece = static_cast<int>(blockIdx.x) % pieces;
+                        at = static_cast<int64_t>(rounds) * ctas + static_cast<int>(blockIdx.x) / pieces;
+                        if (k1 > rounds) at = total;
+                    }
+                    nx.b = -1;
+                    if (at < total) {
+                        // the thread whose sequences hold it: how many end at or before it
+                        int holder = 0;
+#pragma unroll 1
+                        for (int x = 0; x < kThreads && x * per < a.seqs.batch; x += 32)
+                            holder += __popc(__ballot_sync(0xffffffffu, before[x + lane + 1] <= at));
+                        int rest = static_cast<int>(at) - before[holder], b = holder * per;
+                        Seq sq = load_seq(a.seqs, a.pages.page_shift, b);
+#pragma unroll 1
+                        for (int n; rest >= (n = items_of(a, sq));) {
+                            rest -= n;
+                            sq = load_seq(a.seqs, a.pages.page_shift, ++b);
+                        }
+                        const int pairs = (sq.nq * a.group + 2 * kTileRows - 1) / (2 * kTileRows);
+                        nx.b = b;
+                        nx.row0 = (pairs - 1 - rest / a.pages.heads_kv) * 2 * kTileRows;
+                        nx.h = rest % a.pages.heads_kv;
+                        nx.rows = sq.nq * a.group;
+                        nx.t0 = sq.t0;
+                        nx.p0 = sq.p0;
+                        vx = View(nx, a);
+                        const int n = vx.kt.count;
+                        pieces = min(pieces, max(1, n / kPieceTiles));
+                        if (piece < pieces) {
+                            nx.j0 = static_cast<int>(static_cast<int64_t>(n) * piece / pieces);
+                            nx.j1 = static_cast<int>(static_cast<int64_t>(n) * (piece + 1) / pieces);
+                            nx_page = page_of(nx, vx, nx.j0);
+                            if (pieces > 1 && lane == 0) {
+                                int4* d = reinterpret_cast<int4*>(part_desc<DP>(a, ctas, blockIdx.x));
+                                d[1] = make_int4(nx.row0, nx.rows, nx.t0, nx.h);
+                                d[0] = make_int4(1, blockIdx.x - piece, pieces, 0);
+                            }
+                        } else {
+                            nx.b = -1;
+                        }
+                    }
+                    if (ok && k1 >= 2) ok = warp_wait(&iempty[s], ((k1 >> 1) - 1) & 1, err, kErrLoad);
+                    if (lane == 0) {
+                        volatile int* x = posted + s * kPostInts;
+                        x[0] = ok ? nx.b : -1, x[1] = nx.h, x[2] = nx.row0, x[3] = nx.rows, x[4] = nx.t0, x[5] = nx.p0;
+                        x[6] = nx.j0, x[7] = nx.j1, x[8] = vx.p_lo[0], x[9] = vx.p_lo[1], x[10] = vx.p_hi[0], x[11] = vx.p_hi[1];
+                        x[12] = vx.last, x[13] = vx.first_seen;
+                        x[14] = vx.kt.sink_tiles, x[15] = vx.kt.win_tile, x[16] = vx.kt.count;
+                        ptx::mbar_arrive(&ifull[s]);
+                    }
+                    if (j >= it.j1) break;
                 }
-                // an item without keys takes no Q: its phases pass all the same
-                if (it.j0 == it.j1 && ok && q_by_tma) {
-                    if (k > 0) ok = warp_wait(qempty, (k - 1) & 1, err, kErrLoad);
-                    if (ok && lane == 0) ptx::mbar_arrive(qfull);
-                    if (ok) ++q_loads;
-                }
+                if (nx.b < 0) break;
+                it = nx;
+                vw = vx;
+                page = nx_page;
             }
             // no copy may be in flight when the CTA ends
 #pragma unroll 1
