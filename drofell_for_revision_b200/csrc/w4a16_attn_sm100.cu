@@ -14,13 +14,24 @@
 // Rounding P to the 16-bit type (at most half a step each) is what lets the second product
 // run on the tensor cores at their 16-bit rate; l sums the unrounded fp32 values.
 //
+// One persistent CTA per SM goes through its items (256 rows), which all roles learn from the
+// loading warp; the next item's rows and keys are loaded behind the current one's.
+//
 // Warp roles (384 threads): warps 0-3 and 4-7 softmax and epilogue of the two row tiles, one
-// row a thread; warp 8 loads K and V page by page (TMA, lane = page; a page id that is no
-// page reads zeros behind the cache's end); warp 9 puts zeros into V where a tile holds keys
-// that no row sees; warps 10 and 11 issue the MMAs of one row tile each: while one is in its
-// softmax, the tensor cores work for the other. One warp for both left them idle a third of
-// the time: its waits, slowed to some 300 cycles each by the exponentials that share the
-// queue to the shared-memory and special-function units, added up.
+// row a thread; warp 8 plans the items and loads Q, and K and V page by page (TMA, lane =
+// page; a page id that is no page reads zeros behind the cache's end); warp 9 puts zeros into
+// V where a tile holds keys that no row sees; warps 10 and 11 issue the MMAs of one row tile
+// each: while one is in its softmax, the tensor cores work for the other. One warp for both
+// left them idle a third of the time: its waits, slowed to some 300 cycles each by the
+// exponentials that share the queue to the shared-memory and special-function units, added up.
+//
+// What bounds it: the tensor cores and, between them, the chain scores - softmax - product of
+// each row tile, at the clock that the power cap leaves. The MMAs of a step (both row tiles,
+// 128 keys, 128 dimensions) take 2896 cycles by themselves: 16 of M = N = 128 with both
+// operands in shared memory at 107, 16 with P in TMEM at 74. A step takes 3260 of them in a
+// long prompt, and 7 thousand go to an item's beginning and end. One prompt of 8192 tokens, 32
+// heads, bf16: 474 us while the clock is at 1.8 GHz (1160 TFLOP/s over the visible pairs), 575
+// to 590 us (930 to 957) under load for long, at 1.5 GHz.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>

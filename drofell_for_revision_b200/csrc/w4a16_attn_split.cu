@@ -16,6 +16,12 @@
 // waits for another, and the workspace has a fixed size: at most the first and the last piece
 // of a range are parts of an item. Those go to the workspace in fp32 and split_join_kernel
 // adds them in range order (the same result for the same lengths, whatever runs when).
+//
+// Measured (keys and values of 128 dimensions): two sequences of 130001 tokens, 64 heads on 8:
+// 171 to 186 us, 5.7 to 6.2 TB/s; 48 uneven ones of up to 8191: 53 us, 5.0 TB/s; 24 under a
+// window of 1024, 40 heads: 49 us, 5.0 TB/s; one sequence of 777 tokens, 32 heads: 10 us. What
+// is left there: some 4 us until the first keys arrive (length, place, page id, key: four
+// reads that wait for one another) and 4 us for the join's launch and its two reads.
 #include <algorithm>
 #include <atomic>
 
