@@ -10,6 +10,7 @@
 // never freed before w4a16_torch_release: a CUDA graph captured with one still writes
 // into it on replay.
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
@@ -276,28 +277,23 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const
     if (!out_arg.has_value()) outr = w4a16_rows{out.data_ptr(), out.stride(0), out.stride(1)};
     if (tokens == 0) return out;
     // one workspace a call, from torch's allocator on the current stream: calls that overlap
-    // on other streams, and graphs, have their own
+    // on other streams, and graphs, have their own (bare memory: a tensor costs a microsecond)
     const size_t need = w4a16_paged_attention_workspace_size(&p.pages, &p.seqs, static_cast<int>(heads),
                                                              static_cast<int>(window), static_cast<int>(sinks));
-    at::Tensor ws;
-    if (need > 0) ws = at::empty({static_cast<int64_t>(need)}, q.options().dtype(at::kByte));
+    c10::DataPtr ws;
+    if (need > 0) ws = c10::cuda::CUDACachingAllocator::get()->allocate(need);
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(k_pages.device().index()).stream();
     check(w4a16_paged_attention(&p.pages, &p.seqs, &qr, &outr, static_cast<int>(heads), static_cast<float>(scale),
-                                static_cast<int>(window), static_cast<int>(sinks), need > 0 ? ws.data_ptr() : nullptr,
-                                need, stream));
+                                static_cast<int>(window), static_cast<int>(sinks), ws.get(), need, stream));
     return out;
 }
 
-void copy_pages(const at::Tensor& k, const at::Tensor& v, const at::Tensor& src, const at::Tensor& dst) {
+void copy_ids(const at::Tensor& k, const at::Tensor& v, const int32_t* src, const int32_t* dst, int64_t pairs) {
     TORCH_CHECK((k.dim() == 4 || k.dim() == 5) && k.sizes() == v.sizes() && k.strides() == v.strides() &&
                     k.scalar_type() == v.scalar_type(),
                 "k_pages and v_pages must be [(layers,) pages, heads, page size, head dim] of the same type and strides");
     no_grad(k, "k_pages");
     no_grad(v, "v_pages");
-    for (const at::Tensor* t : {&src, &dst})
-        TORCH_CHECK(t->dim() == 1 && t->scalar_type() == at::kInt && t->is_cpu() && t->is_contiguous(),
-                    "src and dst must be lists of page ids on the host");
-    TORCH_CHECK(src.size(0) == dst.size(0), src.size(0), " source pages for ", dst.size(0));
     const int64_t at_page = k.dim() - 4;
     // a page's three dimensions, in whatever order, must fill one block of memory
     int64_t elems = 1, left = 3;
@@ -317,11 +313,11 @@ void copy_pages(const at::Tensor& k, const at::Tensor& v, const at::Tensor& src,
     TORCH_CHECK(k.is_cuda(), "k_pages must be a CUDA tensor (no CPU path exists)");
     on_device(v, k, "v_pages");
     if (k.numel() == 0) {
-        TORCH_CHECK(src.size(0) == 0, "no pages to copy");
+        TORCH_CHECK(pairs == 0, "no pages to copy");
         return;
     }
     const int64_t size = k.element_size(), pages = k.size(at_page), layers = k.dim() == 5 ? k.size(0) : 1;
-    TORCH_CHECK(pages <= 0x7fffffff && layers <= 32767 && src.size(0) <= 0x7fffffff, "sizes must fit 32 bits");
+    TORCH_CHECK(pages <= 0x7fffffff && layers <= 32767 && pairs <= 0x7fffffff, "sizes must fit 32 bits");
     const int64_t stride_page = pages > 1 ? k.stride(at_page) * size : elems * size;
     const int64_t stride_layer = layers > 1 ? k.stride(0) * size : 0;
     TORCH_CHECK(layers == 1 || stride_layer >= (pages - 1) * stride_page + elems * size ||
@@ -329,8 +325,32 @@ void copy_pages(const at::Tensor& k, const at::Tensor& v, const at::Tensor& src,
                 "the layers' pages overlap");
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(k.device().index()).stream();
     check(w4a16_copy_pages(k.data_ptr(), v.data_ptr(), stride_layer, stride_page, static_cast<int>(layers),
-                           static_cast<int>(pages), elems * size, src.data_ptr<int32_t>(), dst.data_ptr<int32_t>(),
-                           static_cast<int>(src.size(0)), k.device().index(), stream));
+                           static_cast<int>(pages), elems * size, src, dst, static_cast<int>(pairs), k.device().index(),
+                           stream));
+}
+
+void copy_pages(const at::Tensor& k, const at::Tensor& v, const at::Tensor& src, const at::Tensor& dst) {
+    for (const at::Tensor* t : {&src, &dst})
+        TORCH_CHECK(t->dim() == 1 && t->scalar_type() == at::kInt && t->is_cpu() && t->is_contiguous(),
+                    "src and dst must be lists of page ids on the host");
+    TORCH_CHECK(src.size(0) == dst.size(0), src.size(0), " source pages for ", dst.size(0));
+    copy_ids(k, v, src.data_ptr<int32_t>(), dst.data_ptr<int32_t>(), src.size(0));
+}
+
+// The ids as Python lists: without the microseconds that two tensors cost.
+void copy_page_lists(const at::Tensor& k, const at::Tensor& v, const std::vector<int64_t>& src,
+                     const std::vector<int64_t>& dst) {
+    TORCH_CHECK(src.size() == dst.size(), src.size(), " source pages for ", dst.size());
+    std::vector<int32_t> ids[2];
+    for (int i = 0; i < 2; ++i) {
+        const std::vector<int64_t>& from = i ? dst : src;
+        ids[i].reserve(from.size());
+        for (const int64_t x : from) {
+            TORCH_CHECK(x >= 0 && x <= 0x7fffffff, "page ids must fit 32 bits, got ", x);
+            ids[i].push_back(static_cast<int32_t>(x));
+        }
+    }
+    copy_ids(k, v, ids[0].data(), ids[1].data(), static_cast<int64_t>(src.size()));
 }
 
 }  // namespace
@@ -346,4 +366,5 @@ PYBIND11_MODULE(_w4a16_torch, m) {
     m.def("append_kv", &append_kv, "store new k and v into pages, rotate q (w4a16_append_kv)");
     m.def("paged_attention", &paged_attention, "attention over pages (w4a16_paged_attention)");
     m.def("copy_pages", &copy_pages, "copy whole pages of every layer (w4a16_copy_pages)");
+    m.def("copy_page_lists", &copy_page_lists, "copy_pages with the ids as lists");
 }

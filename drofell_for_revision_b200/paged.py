@@ -58,7 +58,7 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tab
     """softmax(scale q k^T) v of every new token over its sequence's tokens up to itself;
     with ``window`` over the last ``window`` of them (itself counted) and the sequence's first
     ``sinks``. q [tokens, heads, head dim], heads a multiple of the key-value heads; scale
-    1 / sqrt(head dim) unless given. ``max_q`` is at least the most new tokens of a sequence
+    (positive) 1 / sqrt(head dim) unless given. ``max_q`` is at least the most new tokens of a sequence
     (rows beyond it get no result). Rows that see nothing are 0; rows of no sequence are left
     as they were (undefined in an output that this call makes). ``out`` must not overlap q."""
     if scale is None:
@@ -105,20 +105,25 @@ def attention_forward(layernorm: torch.Tensor, norm_epsilon: float, q_proj: int,
 
 
 def _ids(x: PageIds) -> torch.Tensor:
-    if isinstance(x, torch.Tensor):
-        if x.is_floating_point() or x.is_complex() or x.dtype == torch.bool:
-            raise RuntimeError("page ids must be whole numbers")
-        if x.dtype == torch.int64 and x.numel() and not x.is_cuda and (int(x.min()) < 0 or int(x.max()) >= 1 << 31):
-            raise RuntimeError("page ids must fit 32 bits")
-        return x.to(torch.int32).contiguous() if not x.is_cuda else x
-    return torch.tensor(x, dtype=torch.int32)
+    if not isinstance(x, torch.Tensor):
+        x = torch.tensor(x, dtype=torch.int64)
+    if x.is_floating_point() or x.is_complex() or x.dtype == torch.bool:
+        raise RuntimeError("page ids must be whole numbers")
+    if x.is_cuda:
+        raise RuntimeError("src and dst must be lists of page ids on the host")
+    if x.numel() and (int(x.min()) < 0 or int(x.max()) >= 1 << 31):
+        raise RuntimeError("page ids must fit 32 bits")
+    return x.to(torch.int32).contiguous()
 
 
 def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: PageIds, dst: PageIds) -> None:
     """Copy pages src[i] to dst[i] of K and V [(layers,) pages, heads, page size, head dim], of
     all layers. The ids are host lists, read before the call returns; no page may be written
     twice, or both read and written."""
-    _ext().copy_pages(k_pages, v_pages, _ids(src), _ids(dst))
+    if type(src) is list and type(dst) is list:
+        _ext().copy_page_lists(k_pages, v_pages, src, dst)
+    else:
+        _ext().copy_pages(k_pages, v_pages, _ids(src), _ids(dst))
 
 
 def rope_table(positions: int, dim: int, base: float = 10000.0, device: Optional[torch.device] = None) -> torch.Tensor:

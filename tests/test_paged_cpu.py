@@ -175,8 +175,13 @@ def test_copy_refusals():
         paged.copy_pages(k, k.clone(), [1], [2, 3])
     with pytest.raises(RuntimeError, match="one block"):
         paged.copy_pages(k[..., :32], k.clone()[..., :32], [1], [2])
-    with pytest.raises(RuntimeError, match="32 bits"):
-        paged.copy_pages(k, k.clone(), torch.tensor([1 << 32]), [2])
+    for big in (torch.tensor([1 << 32]), [1 << 32], [-1], torch.tensor([-1])):
+        with pytest.raises(RuntimeError, match="32 bits"):
+            paged.copy_pages(k, k.clone(), big, [2])
+    with pytest.raises((RuntimeError, TypeError)):
+        paged.copy_pages(k, k.clone(), [1.5], [2])
+    with pytest.raises(RuntimeError, match="source pages"):
+        paged.copy_pages(k, k.clone(), (1, 2), torch.tensor([2]))
     with pytest.raises(RuntimeError, match="whole numbers"):
         paged.copy_pages(k, k.clone(), torch.tensor([1.5]), [2])
 
