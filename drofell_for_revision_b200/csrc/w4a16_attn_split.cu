@@ -174,8 +174,8 @@ __global__ void __launch_bounds__(kThreads, DEEP ? 1 : 2) split_kernel(const __g
             if (blockIdx.x == b % gridDim.x && sq.nq > 0 && un.tiles == 0) {
                 const int chunks = a.pages.dim >> 3;
 #pragma unroll 1
-                for (int i = 0; i < sq.nq * a.heads * chunks; ++i) {
-                    const int row = i / chunks, c = i % chunks;
+                for (int64_t i = 0; i < int64_t{sq.nq} * a.heads * chunks; ++i) {
+                    const int64_t row = i / chunks, c = i % chunks;
                     *reinterpret_cast<uint4*>(a.out + (sq.t0 + row / a.heads) * a.o_token + (row % a.heads) * a.o_head +
                                               c * 8) = make_uint4(0, 0, 0, 0);
                 }

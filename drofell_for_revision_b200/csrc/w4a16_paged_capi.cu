@@ -2,6 +2,7 @@
 // the choice of the attention kernel, launches.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <climits>
 #include <cmath>
@@ -71,6 +72,30 @@ int check_rows(const w4a16_rows* r, const char* name) {
     if (r->stride_token < 0 || r->stride_head < 0 || r->stride_token % 8 || r->stride_head % 8 || !aligned16(r->dev))
         return report_error(W4A16_ERR_INVALID, "%s must be 16-byte aligned, its strides non-negative multiples of 8 elements",
                             name);
+    return W4A16_OK;
+}
+
+// Memory that is written holds no element twice: counts and strides of what lies around rows of `dim`.
+struct Extent {
+    int64_t count, stride;
+};
+bool apart(Extent a, Extent b, Extent c, int dim) {
+    Extent e[3] = {a, b, c};
+    std::sort(e, e + 3, [](const Extent& x, const Extent& y) { return x.stride < y.stride; });
+    int64_t taken = dim;
+    for (const Extent& x : e) {
+        if (x.count <= 1) continue;
+        if (x.stride < taken) return false;
+        taken += (x.count - 1) * x.stride;
+    }
+    return true;
+}
+
+int check_written(const w4a16_rows* r, int tokens, int heads, int dim, const char* name) {
+    const int rc = check_rows(r, name);
+    if (rc != W4A16_OK) return rc;
+    if (!apart({tokens, r->stride_token}, {heads, r->stride_head}, {1, 0}, dim))
+        return report_error(W4A16_ERR_INVALID, "%s's rows overlap", name);
     return W4A16_OK;
 }
 
@@ -167,9 +192,12 @@ int w4a16_append_kv(const w4a16_pages* pages, const w4a16_seqs* seqs, const w4a1
     const bool with_q = q && q->dev;
     if (rc == W4A16_OK && with_q) {
         rc = check_rows(q, "q");
-        if (rc == W4A16_OK) rc = check_rows(q_out, "q_out");
         if (rc == W4A16_OK && heads <= 0) rc = report_error(W4A16_ERR_INVALID, "heads=%d", heads);
+        if (rc == W4A16_OK) rc = check_written(q_out, seqs->tokens, heads, pages->head_dim, "q_out");
     }
+    if (rc == W4A16_OK && !apart({pages->num_pages, pages->stride_page}, {pages->heads_kv, pages->stride_head},
+                                 {pages->page_size, pages->stride_token}, pages->head_dim))
+        rc = report_error(W4A16_ERR_INVALID, "pages that overlap");
     if (rc != W4A16_OK) return rc;
     if (rope_dev) {
         if (rope_dim <= 0 || rope_dim > pages->head_dim || rope_dim % (interleaved ? 8 : 16))
@@ -224,7 +252,7 @@ int w4a16_paged_attention(const w4a16_pages* pages, const w4a16_seqs* seqs, cons
         return report_error(W4A16_ERR_INVALID, "scale must be positive and finite");
     if (seqs->batch == 0 || seqs->tokens == 0 || seqs->max_q == 0) return W4A16_OK;
     rc = check_rows(q, "q");
-    if (rc == W4A16_OK) rc = check_rows(out, "out");
+    if (rc == W4A16_OK) rc = check_written(out, seqs->tokens, heads, pages->head_dim, "out");
     if (rc != W4A16_OK) return rc;
     if (q->dev == out->dev) return report_error(W4A16_ERR_INVALID, "out must not be q");
     AttnArgs a = attn_args(pages, seqs, heads, window, sinks);

@@ -97,6 +97,20 @@ def test_append_arguments_are_checked():
     assert append(s=seqs(batch=0, tokens=0)) == OK
 
 
+@pytest.mark.parametrize("kw", [dict(stride_token=0), dict(stride_head=0), dict(stride_token=384), dict(stride_head=64),
+                                dict(stride_token=128, stride_head=128)])
+def test_rows_that_are_written_must_not_overlap(kw):
+    assert attention(out=rows(dev=2 * FAKE, **kw)) == INVALID
+    assert append(q=rows(), q_out=rows(**kw)) == INVALID
+    assert b"overlap" in _capi.lib().w4a16_last_error()
+
+
+def test_pages_that_are_written_must_not_overlap():
+    for kw in (dict(stride_page=2048), dict(stride_head=1024), dict(stride_token=64)):
+        assert append(p=pages(**kw)) == INVALID
+        assert b"overlap" in _capi.lib().w4a16_last_error()
+
+
 def copy(src, dst, k=FAKE, stride_layer=1 << 20, stride_page=4096, layers=2, num=10, size=4096):
     n = len(src)
     arr = lambda x: (ctypes.c_int * n)(*x)  # noqa: E731
