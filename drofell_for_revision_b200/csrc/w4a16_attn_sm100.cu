@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* qempty = qfull + 1;   // and all scores of them are made
     uint64_t* sfull = qempty + 1;   // [2] S of a row tile is complete (and all products before it)
     uint64_t* pfull = sfull + 2;    // [2][2] half of P is written (the first: O rescaled)
-    uint64_t* ofull = pfull + 4;    // [2] all products of a row tile are complete
+    uint64_t* ofull = pfull + 4;    // [2] all products of a row tile are complete, of an item that has some for it
     uint64_t* dirty = ofull + 2;    // V of a tile that the mask cuts is loaded
     uint64_t* clean = dirty + 1;    // and holds zeros where no row sees
     uint64_t* ifull = clean + 1;    // [2] an item is posted
@@ -717,7 +717,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 i -= 2;  // step n has no K
                 if (n == 0) ptx::umma_commit(qempty);
-                if (!ended) ptx::umma_commit(&ofull[t]);
+                // only an item that has a product for this row tile is signalled: such a one waits for the
+                // softmax warps, others could run two phases ahead of them, which a parity does not tell apart
+                if (!ended && !first) ptx::umma_commit(&ofull[t]);
             }
         }
         __syncwarp();
@@ -730,7 +732,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int step_shift = min(a.pages.page_shift, 7);
         const float sc = a.scale_log2;
         const bool wide = ((reinterpret_cast<uintptr_t>(a.out) & 31) | ((a.o_token | a.o_head | a.pages.dim) & 15)) == 0;
-        int i = 0, seen = 0;  // tiles of keys; scores taken
+        int i = 0, seen = 0, ends = 0;  // tiles of keys; scores taken; items with any
         bool ok = true;
         Item it;
         View vw;
@@ -819,7 +821,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 first = false;
             }
             // ------------------------------------------------ epilogue
-            if (ok) ok = warp_wait(&ofull[t], k & 1, err, kErrEnd);
+            if (ok && !first) ok = warp_wait(&ofull[t], ends++ & 1, err, kErrEnd);
             if (!ok) break;
             ptx::tc_fence_after();
             const float inv = part ? 1.f : l == 0.f ? 0.f : 1.f / l;

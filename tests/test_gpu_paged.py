@@ -251,6 +251,20 @@ def test_a_value_reaches_only_the_rows_that_see_it(value, new, old, window):
     check_attention(bt, window)
 
 
+@pytest.mark.parametrize("heads,dim,seed", [(2, 64, 0), (2, 128, 1), (6, 128, 2)])
+def test_row_tiles_without_keys_among_others(heads, dim, seed):
+    """Long runs of items in which a row tile, or both, has nothing to do, behind ones whose values
+    that are not finite take it long: who has nothing to do must not run ahead."""
+    g = torch.Generator().manual_seed(seed)
+    kinds = [(200, 200), (50, 50), (0, 40), (30, 100), (160, 1), (0, 200)]
+    pick = torch.randint(0, len(kinds), (1000,), generator=g).tolist()
+    bt = Batch([kinds[i][0] for i in pick], [kinds[i][1] for i in pick], heads, 2, dim, 16, torch.bfloat16, seed=seed)
+    for b, i in enumerate(pick):
+        if i == 0:
+            bt.v[int(bt.tables[b, 9]), :, 6, 5] = (math.nan, math.inf)[b & 1]
+    check_attention(bt)
+
+
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("what", ["q", "k", "v", "some v"])
 @pytest.mark.parametrize("new,old", [(1, 3000), (4, 200), (150, 2000), (700, 0)])
