@@ -60,7 +60,8 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tab
     ``sinks``. q [tokens, heads, head dim], heads a multiple of the key-value heads; scale
     (positive) 1 / sqrt(head dim) unless given. ``max_q`` is at least the most new tokens of a sequence
     (rows beyond it get no result). Rows that see nothing are 0; rows of no sequence are left
-    as they were (undefined in an output that this call makes). ``out`` must not overlap q."""
+    as they were (undefined in an output that this call makes). ``out`` must not overlap q
+    or hold an element twice."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     return _ext().paged_attention(q, k_pages, v_pages, tables, lens, cu_q, max_q, scale, window, sinks, out)

@@ -278,8 +278,9 @@ typedef struct w4a16_rows {
  * width * page_size. Dimensions i and i + rope_dim / 2 rotate together, with interleaved
  * 2 i and 2 i + 1; those past rope_dim pass through. rope_dim is a multiple of 16 (8 when
  * interleaved). fp32 arithmetic, rounded once. Pages that two sequences share must not be
- * written to. Tokens of a negative position (more new tokens than the length) are not
- * stored, their q passes unrotated. */
+ * written to; pages, or rows of q_out, that overlap in memory are refused. Tokens of a
+ * negative position (more new tokens than the length) are not stored, their q passes
+ * unrotated. */
 W4A16_API int w4a16_append_kv(const w4a16_pages* pages, const w4a16_seqs* seqs, const w4a16_rows* k,
                               const w4a16_rows* v, const w4a16_rows* q, const w4a16_rows* q_out, int heads,
                               const float* rope_dev, int rope_positions, int rope_dim, int interleaved, void* stream);
@@ -287,10 +288,10 @@ W4A16_API int w4a16_append_kv(const w4a16_pages* pages, const w4a16_seqs* seqs, 
 /* out = softmax(scale q k^T) v (scale > 0) of every new token over the visible tokens of its sequence:
  * not after it, and with window > 0 the last `window` ones (itself counted) and the first
  * `sinks` ones. heads is a multiple of heads_kv; query head i reads key-value head
- * i / (heads / heads_kv); out must not overlap q. Rows that see nothing are 0. Softmax statistics and sums in
- * fp32. No host synchronisation and no allocation: capturable. Calls that may overlap on
- * the GPU need workspaces of their own; a workspace is 32-byte aligned, its contents mean
- * nothing before and after a call. */
+ * i / (heads / heads_kv); out must not overlap q or itself. Rows that see nothing are 0.
+ * Softmax statistics and sums in fp32. No host synchronisation and no allocation: capturable.
+ * Calls that may overlap on the GPU need workspaces of their own; a workspace is 32-byte
+ * aligned, its contents mean nothing before and after a call. */
 W4A16_API int w4a16_paged_attention(const w4a16_pages* pages, const w4a16_seqs* seqs, const w4a16_rows* q,
                                     const w4a16_rows* out, int heads, float scale, int window, int sinks,
                                     void* workspace_dev, size_t workspace_bytes, void* stream);
