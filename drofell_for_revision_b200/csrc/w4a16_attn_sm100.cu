@@ -8,11 +8,13 @@
 //   S = Q K^T (tcgen05, fp32 in TMEM), P = 2^(scale S - m) rounded to 16 bits, O += P V.
 // P replaces S in TMEM and is the A operand of the second product, read from there; V, whose
 // rows are keys, is an MN-major B operand. O stays in TMEM; it is rescaled only when a row's
-// maximum grew by more than 2^8 (P up to 256 keeps every bit; l and O share the factor), so
+// maximum grew by more than 2^8 (l and O share the factor; P stays in the type's range), so
 // that the usual tile costs no round trip of O.
 //
 // Rounding P to the 16-bit type (at most half a step each) is what lets the second product
-// run on the tensor cores at their 16-bit rate; l sums the unrounded fp32 values.
+// run on the tensor cores at their 16-bit rate; l sums the unrounded fp32 values. In fp16 P and l
+// are taken times 2^7: steps end at 2^-24, so that a weight of less than 2^-21 of the maximum
+// at hand loses bits, but n keys lose less than n 2^-32 of the whole.
 //
 // One persistent CTA per SM goes through its items (256 rows), which all roles learn from the
 // loading warp; the next item's rows and keys are loaded behind the current one's.
@@ -58,6 +60,7 @@ constexpr int kPostInts = 17;      // of an item and its view
 constexpr int kBlock = 128 * 128;  // bytes of a [128 rows x 64] operand block, 128-byte swizzle
 constexpr uint32_t kWaitLimit = 1u << 18;  // x ~10 us sleeps: a few seconds
 constexpr float kSlack = 8.f;              // log2 of the growth that O tolerates without rescaling
+static_assert(kSlack + kWeightBias<false, kTileKeys> < 16.f, "fp16 weights that overflow");
 
 enum : int { kErrLoad = 1, kErrMma = 2, kErrSoftmax = 3, kErrEnd = 4 };
 __device__ int g_attention_error;
@@ -152,7 +155,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// 2^x of two values on the FMA units, x <= 8: 2^round(x) by the exponent bits, 2^f for f in
+// 2^x of two values on the FMA units, x <= 15: 2^round(x) by the exponent bits, 2^f for f in
 // [-1/2, 1/2] by the polynomial of degree 4 of least relative error with value 1 at 0
 // (2.8e-6, a hundredth of the 16-bit rounding that follows). Below -126 it runs out through
 // the denormals to exactly 0 at -127, where smaller x (and -inf) are held. NaN stays NaN.
@@ -169,6 +172,11 @@ __device__ __forceinline__ float2 exp2_fma(float2 x) {
     const float2 a = of_pair(y), b = of_pair(r);
     return make_float2(__int_as_float(__float_as_int(a.x) + (__float_as_int(b.x) << 23)),
                        __int_as_float(__float_as_int(a.y) + (__float_as_int(b.y) << 23)));
+}
+// What is taken from a row's scaled scores: its maximum so far, and the weights' factor.
+template <bool BF16>
+__device__ __forceinline__ float base_of(float m, float sc) {
+    return (m == -INFINITY ? 0.f : m * sc) - kWeightBias<BF16, kTileKeys>;
 }
 // 64 of a row's weights, 2^(sc s - base), packed into the first 32 of s; returns their sum.
 // Two pairs of seven are raised on the FMA units, beside the special-function units, which
@@ -794,7 +802,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         ptx::tmem_ld_wait();
                         m = fmaxf(top, largest(s + 64));
                     }
-                    part = weights<BF16>(s, sc, m == -INFINITY ? 0.f : m * sc);
+                    part = weights<BF16>(s, sc, base_of<BF16>(m, sc));
                     if (first) break;
                     ptx::tmem_ld_wait();
                     top = fmaxf(top, largest(s + 64));
@@ -814,7 +822,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
                 put_half(ts, s, &pfull[2 * t]);
-                part += weights<BF16>(s + 64, sc, m == -INFINITY ? 0.f : m * sc);
+                part += weights<BF16>(s + 64, sc, base_of<BF16>(m, sc));
                 put_half(ts + 32, s + 64, &pfull[2 * t + 1]);
                 l += part;
                 ++seen;

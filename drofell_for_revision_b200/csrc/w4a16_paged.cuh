@@ -90,6 +90,15 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
+// Weights enter the value products in 16 bits, taken times 2^kWeightBias; so do the sums of
+// weights, and the factor cancels in their quotient. fp16 holds nothing below 2^-24: without a
+// factor all weights of less than 2^-25 of the largest would be counted in the sum and missing in the
+// product (130000 of them behind a key that outweighs them: an output off by percents). The
+// factors fill fp16's range upwards: the split kernel's weights are at most 1 (its maximum is exact),
+// the prompt kernel's at most 2^8 (key tiles of 128). bf16 has fp32's exponents and needs none.
+template <bool BF16, int TILE>
+constexpr float kWeightBias = BF16 ? 0.f : TILE == 16 ? 15.f : 7.f;
+
 // A row's maximum, sum of weights and weighted sum of values (four dimensions a lane).
 struct RowSum {
     float m, l, o[4];
@@ -139,7 +148,7 @@ __device__ __noinline__ RowSum careful_row(const AttnArgs& a, int b, int h, int6
             for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
             s *= a.scale_log2;
             const float m = fmaxf(r.m, s), base = m == -INFINITY ? 0.f : m;
-            const float f = r.m == m ? 1.f : exp2_approx(r.m - base), w = exp2_approx(s - base);
+            const float f = r.m == m ? 1.f : exp2_approx(r.m - base), w = exp2_approx(s - base + kWeightBias<BF16, TILE>);
             r.m = m;
             r.l = r.l * f + w;
 #pragma unroll

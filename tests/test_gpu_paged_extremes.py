@@ -1,0 +1,88 @@
+"""The paged cache where scores are extreme: weights far below the largest.
+
+Tolerances. As in test_gpu_paged.py an output is off by at most half a step of its own and half a
+step of the weights, (eps / 2) (|out| + sum p |v|) together. What comes on top is counted here:
+ * fp32 accumulation takes one step, at most 2^-23 relative, for every 16 keys of a product, and
+   400 more cover sums inside a tile and the join: (n / 16 + 400) 2^-23 sum p |v|;
+ * a score's error is amplified by the exponential: scores of at most 2^9 (base 2) are off by
+   2^-23 of that in two roundings, 2^-13 sum p |v|, counted only where scores are that large;
+ * fp16 cannot hold a weight below its smallest step: with the weights scaled by 2^7 and the
+   running maximum at most 2^8 behind, half a step is 2^-32 of the largest weight (2^-40 where
+   they are scaled by 2^15 against the exact maximum): n 2^-32 max |v|.
+"""
+import math
+
+import pytest
+import torch
+
+from drofell_for_revision_b200 import paged
+from test_gpu_paged import DEV, Batch, check_attention, exact_attention
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float16, torch.bfloat16]
+
+
+@pytest.fixture(autouse=True)
+def no_wait_gave_up():
+    yield
+    assert paged.device_error(DEV) == 0
+
+
+def attend(bt, scale, **kw):
+    return paged.attention(bt.q, bt.k, bt.v, bt.tables, bt.lens, cu_q=bt.cu_q, max_q=bt.max_q, scale=scale, **kw)
+
+
+def check(bt, scale, n, score_error=0.0, **kw):
+    got = attend(bt, scale, **kw)
+    want, spread = exact_attention(bt, scale, kw.get("window", 0), kw.get("sinks", 0))
+    half = torch.finfo(got.dtype).eps / 2
+    room = half * (want.abs() + spread) + ((n / 16 + 400) * 2.0 ** -23 + score_error) * spread
+    if got.dtype == torch.float16:
+        room = room + n * 2.0 ** -32 * float(bt.v.abs().max()) + 2.0 ** -25  # and half the output's own smallest step
+    over = (got.double() - want).abs() / room
+    assert float(over.max()) <= 1.0
+    return got
+
+
+# ---------------------------------------------------------------- weights far below the largest
+def sinks_first(lens, new, heads, hkv, dim, dtype, low, high):
+    """Sequences whose first key lies `low` to `high` nats above the others, its value 0, theirs of
+    one sign."""
+    bt = Batch(lens, new, heads, hkv, dim, 64, dtype, seed=71)
+    g = torch.Generator(device=DEV).manual_seed(71)
+    bt.q.mul_(0.01)
+    bt.q[..., 0] = 4.0
+    bt.k.mul_(0.01)
+    gap = low + (high - low) * torch.rand(bt.k.shape[:3], device=DEV, generator=g)
+    bt.k[..., 0] = (-gap * math.sqrt(dim) / 4.0).to(dtype)
+    bt.v.copy_((bt.v.abs() * 0.5 + 0.5).to(dtype))
+    first = bt.tables[:, 0].long()
+    bt.k[first, :, 0, 0] = 0.0
+    bt.v[first, :, 0] = 0.0
+    return bt
+
+
+# weights of 17.4 nats below the largest round to 0 on fp16's own grid, those of 16.8 to 17.2 to the
+# step above
+GAPS = [(14.0, 18.0), (17.4, 18.0), (16.8, 17.2)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("low,high", GAPS)
+@pytest.mark.parametrize("n,new", [(40000, 1), (130001, 1), (33000, 64), (3000, 300)])
+def test_one_key_holds_nearly_all_the_weight(dtype, dim, low, high, n, new):
+    bt = sinks_first([n], [new], 4, 1, dim, dtype, low, high)
+    check(bt, 1.0 / math.sqrt(dim), n)
+    # and where all values are 1, so is the result: no weight is counted and not summed
+    bt.v.fill_(1.0)
+    check(bt, 1.0 / math.sqrt(dim), n)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("low,high", GAPS)
+@pytest.mark.parametrize("batch,n,new", [(160, 900, 1), (80, 900, 64)])
+def test_one_key_holds_nearly_all_the_weight_of_many_sequences(dtype, low, high, batch, n, new):
+    """So many that most are not cut into pieces with a maximum of their own."""
+    check(sinks_first([n] * batch, [new] * batch, 8, 8, 64, dtype, low, high), 0.125, n)
