@@ -939,9 +939,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) prompt_join_kernel(const __gr
                 const float2 u = *reinterpret_cast<const float2*>(s + 4 * kTileRows + r * DP + lane * E + e);
                 v[e] = u.x, v[e + 1] = u.y;
             }
-            // a piece in which the row saw nothing adds nothing
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] += f == 0.f ? 0.f : f * v[e];
+            for (int e = 0; e < E; ++e) o[e] += share_of(f, v[e]);
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const int row = row0 + r, token = row / a.group;

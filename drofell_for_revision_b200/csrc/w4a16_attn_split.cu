@@ -548,13 +548,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) split_join_kernel(const __gri
                 for (int d = kJoinPieces / 2; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
                 l = l * old + sum;
 #pragma unroll
-                for (int e = 0; e < E; ++e) x[e] = old == 0.f ? 0.f : x[e] * old;
+                for (int e = 0; e < E; ++e) x[e] = share_of(old, x[e]);
 #pragma unroll
                 for (int i = 0; i < kJoinPieces; ++i) {
                     const float fi = __shfl_sync(0xffffffffu, f, i);
-                    // a piece in which the row saw nothing adds nothing
 #pragma unroll
-                    for (int e = 0; e < E; ++e) x[e] += fi == 0.f ? 0.f : fi * v[i][e];
+                    for (int e = 0; e < E; ++e) x[e] += share_of(fi, v[i][e]);
                 }
             }
         }
@@ -573,13 +572,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) split_join_kernel(const __gri
                 const float f = exp2_approx(m - base);
                 l *= f;
 #pragma unroll
-                for (int e = 0; e < E; ++e) x[e] = f == 0.f ? 0.f : x[e] * f;
+                for (int e = 0; e < E; ++e) x[e] = share_of(f, x[e]);
 #pragma unroll 1
                 for (int w = warp + 1; w < warp + per_row; ++w) {
                     const float fw = exp2_approx(sums[w][DP] - base);
                     l += sums[w][DP + 1] * fw;
 #pragma unroll
-                    for (int e = 0; e < E; ++e) x[e] += fw == 0.f ? 0.f : fw * sums[w][lane * E + e];
+                    for (int e = 0; e < E; ++e) x[e] += share_of(fw, sums[w][lane * E + e]);
                 }
             }
             __syncthreads();

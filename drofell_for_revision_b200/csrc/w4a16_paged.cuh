@@ -99,6 +99,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
 template <bool BF16, int TILE>
 constexpr float kWeightBias = BF16 ? 0.f : TILE == 16 ? 15.f : 7.f;
 
+// f v of a piece's sum v under a factor f of at most 1 that may have run out to 0. No weight is
+// 0, so an infinity or NaN among the values stays one, however small its piece's share.
+__device__ __forceinline__ float share_of(float f, float v) {
+    return f == 0.f ? (v * 0.f == 0.f ? 0.f : v) : f * v;
+}
+
 // A row's maximum, sum of weights and weighted sum of values (four dimensions a lane).
 struct RowSum {
     float m, l, o[4];

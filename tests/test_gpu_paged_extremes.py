@@ -1,4 +1,4 @@
-"""The paged cache where scores are extreme: weights far below the largest.
+"""The paged cache where scores and values are extreme: weights far below the largest, infinite values.
 
 Tolerances. As in test_gpu_paged.py an output is off by at most half a step of its own and half a
 step of the weights, (eps / 2) (|out| + sum p |v|) together. What comes on top is counted here:
@@ -86,3 +86,33 @@ def test_one_key_holds_nearly_all_the_weight(dtype, dim, low, high, n, new):
 def test_one_key_holds_nearly_all_the_weight_of_many_sequences(dtype, low, high, batch, n, new):
     """So many that most are not cut into pieces with a maximum of their own."""
     check(sinks_first([n] * batch, [new] * batch, 8, 8, 64, dtype, low, high), 0.125, n)
+
+
+# ---------------------------------------------------------------- values that are not finite
+def far(lens, new, dtype, j_top, seed):
+    """Sequences whose key j_top is 256 nats above the others: exp2 of the distance is 0 in fp32."""
+    bt = Batch(lens, new, 4, 2, 128, 16, dtype, seed=seed)
+    bt.q.mul_(0.1)
+    bt.q[..., 0] = 16.0
+    bt.k.mul_(0.1)
+    bt.k[..., 0] = 0.0
+    for b in range(len(lens)):
+        bt.k[int(bt.tables[b, j_top // 16]), :, j_top % 16, 0] = 16.0
+    return bt
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("n,new,j_top", [(5000, 1, 10), (5000, 1, 4990), (5000, 200, 3), (300, 1, 299)])
+def test_infinite_values_of_vanishing_weight(dtype, value, n, new, j_top):
+    """A weight is never 0, however far its key lies below the largest: an infinity there is one in
+    the result, whatever pieces the keys were cut into."""
+    bt = far([n, n], [new, new], dtype, j_top, 73)
+    for j, d in ((5, 7), (n // 2, 40), (n - new - 1, 100)):
+        bt.v[int(bt.tables[0, j // 16]), :, j % 16, d] = value
+    want, _ = exact_attention(bt, 1.0, 0, 0)
+    got = attend(bt, 1.0).double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.isinf(got), torch.isinf(want))
+    assert torch.equal(got[torch.isinf(want)], want[torch.isinf(want)])
+    assert not torch.isfinite(want[:new][..., [7, 40, 100]]).any() and torch.isfinite(want[new:]).all()
