@@ -108,14 +108,6 @@ __device__ __forceinline__ float share_of(float f, float v) {
 // A row's maximum, sum of weights and weighted sum of values (four dimensions a lane).
 struct RowSum {
     float m, l, o[4];
-    template <bool BF16>
-    __device__ __forceinline__ void store(const AttnArgs& a, int64_t o_off) const {
-        const int d = (threadIdx.x & 31) * 4;
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        if (d < a.pages.dim)
-            *reinterpret_cast<uint2*>(a.out + o_off + d) =
-                make_uint2(pack2<BF16>(o[0] * inv, o[1] * inv), pack2<BF16>(o[2] * inv, o[3] * inv));
-    }
 };
 
 // One row over key tiles [i0, i1), key by key and each key by selection. A warp a row, lanes
@@ -234,27 +226,23 @@ __device__ __noinline__ void settle_rows(const AttnArgs& a, int b, int h, int t0
         }
         bool anew = false;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint32_t k = (f >> e) & 0x111u;
-            if (k == 0) {
-                anew |= !(x[e] * 0.f == 0.f);
-            } else {
-                x[e] = k == 16u ? INFINITY : k == 256u ? -INFINITY : NAN;
-            }
-        }
+        for (int e = 0; e < 4; ++e) anew |= ((f >> e) & 0x111u) == 0 && !(x[e] * 0.f == 0.f);
         if (__any_sync(0xffffffffu, anew)) {
             const RowSum r = careful_row<TILE, BF16>(a, b, h, static_cast<int64_t>(t0 + token) * a.q_token + head * a.q_head, p, kt,
                                                      i0, i1);
-            if (part == nullptr) {
-                r.store<BF16>(a, o_off - d);
-                continue;
-            }
-            if (lane == 0) {
+            if (part && lane == 0) {
                 part[part_row + bit] = r.m;
                 part[part_rows + part_row + bit] = r.l;
             }
+            const float inv = part ? 1.f : r.l == 0.f ? 0.f : 1.f / r.l;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = r.o[e];
+            for (int e = 0; e < 4; ++e) x[e] = r.o[e] * inv;
+        }
+        // what the row sees of infinities and NaN decides, whichever way the rest was computed
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t k = (f >> e) & 0x111u;
+            if (k) x[e] = k == 16u ? INFINITY : k == 256u ? -INFINITY : NAN;
         }
         if (in && part) {
             *reinterpret_cast<float4*>(slot) = make_float4(x[0], x[1], x[2], x[3]);

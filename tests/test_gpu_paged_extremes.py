@@ -116,3 +116,21 @@ def test_infinite_values_of_vanishing_weight(dtype, value, n, new, j_top):
     assert torch.equal(torch.isinf(got), torch.isinf(want))
     assert torch.equal(got[torch.isinf(want)], want[torch.isinf(want)])
     assert not torch.isfinite(want[:new][..., [7, 40, 100]]).any() and torch.isfinite(want[new:]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("n,new", [(60, 4), (5000, 4), (60, 40), (5000, 200)])
+def test_a_row_computed_anew_keeps_what_it_sees(dtype, value, n, new):
+    """A row that a value it does not see made not finite is computed anew; an infinity that it does
+    see, of vanishing weight, still decides its dimension."""
+    bt = far([n], [new], dtype, 1, 79)
+    page, slot = int(bt.tables[0, 0]), 0
+    bt.v[page, :, slot, 7] = value
+    last = n - 1  # seen by the last row alone
+    bt.v[int(bt.tables[0, last // 16]), :, last % 16, 90] = math.nan
+    want, _ = exact_attention(bt, 1.0, 0, 0)
+    got = attend(bt, 1.0).double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.isinf(got), torch.isinf(want))
+    assert torch.equal(got[torch.isinf(want)], want[torch.isinf(want)])
