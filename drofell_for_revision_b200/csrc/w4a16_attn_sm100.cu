@@ -58,7 +58,7 @@ constexpr int kLaunchRegs = 168, kSoftmaxRegs = 208, kOtherRegs = 88;
 static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "more registers than launched with");
 constexpr int kPostInts = 17;      // of an item and its view
 constexpr int kBlock = 128 * 128;  // bytes of a [128 rows x 64] operand block, 128-byte swizzle
-constexpr uint32_t kWaitLimit = 1u << 18;  // x ~10 us sleeps: a few seconds
+constexpr uint32_t kWaitLimit = 1u << 18;  // x at most 10 us of sleep: up to a few seconds
 constexpr float kSlack = 8.f;              // log2 of the growth that O tolerates without rescaling
 static_assert(kSlack + kWeightBias<false, kTileKeys> < 16.f, "fp16 weights that overflow");
 
@@ -73,7 +73,7 @@ struct Cfg {
     static constexpr int kKvOff = 2 * kTileBytes;
     static constexpr int kBarOff = kKvOff + kSlots * kTileBytes;
     static constexpr int kListOff = kBarOff + 512;           // barriers and posted items before it
-    static_assert((2 * kSlots + 18) * 8 + 4 + 8 * 4 + 2 * kPostInts * 4 <= kListOff - kBarOff, "barriers and posted items");
+    static_assert((2 * kSlots + 18) * 8 + 4 + 10 * 4 + 8 * 4 + 2 * kPostInts * 4 <= kListOff - kBarOff, "barriers and posted items");
     static constexpr int kSmem = kListOff + (kThreads + 1) * 4 + 1020;  // and alignment
     static_assert(kSmem <= 227 * 1024, "shared memory budget");
     // TMEM columns: S of both row tiles (P in their first 64), O of both
@@ -235,6 +235,23 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* e
     return __all_sync(0xffffffffu, wait(bar, parity, err, code));
 }
 
+// As warp_wait, for whoever waits until some tile of an item is reached, however many come before
+// it: gives up when for kWaitLimit polls no tile was loaded either (*loaded did not change). Only where
+// time does not count: the same in every wait cost 4 to 6 % of a prompt.
+__device__ __forceinline__ bool warp_wait_long(uint64_t* bar, uint32_t parity, int* err, int code, const volatile int* loaded) {
+    bool ok = false;
+#pragma unroll 1
+    for (int seen = *loaded, now;; seen = now) {
+#pragma unroll 1
+        for (uint32_t i = 0; i < kWaitLimit && !ok; ++i) ok = ptx::mbar_try_wait_sleep(bar, parity, 10000u);
+        now = *loaded;
+        if (__all_sync(0xffffffffu, ok)) return true;
+        if (__all_sync(0xffffffffu, ok || now == seen)) break;
+    }
+    atomicCAS(err, 0, code);
+    return false;
+}
+
 // The lowest n bits, n held to 0 .. 32.
 __device__ __forceinline__ uint32_t first_bits(int n) {
     return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
@@ -326,6 +343,110 @@ __device__ __forceinline__ int items_of(const AttnArgs& a, const Seq& s) {
     return (s.nq * a.group + 2 * kTileRows - 1) / (2 * kTileRows) * a.pages.heads_kv;
 }
 
+// Item k of this CTA; false: it has none (x.b is then -1). Rounds of the CTAs run forth and back over
+// the items, whose work falls along a sequence: a CTA's shares even out. Where there are few
+// rounds, the items of the last, incomplete one are cut along their keys, among all CTAs. `before`
+// holds the items before each thread's `per` sequences, `total` of all. A whole warp.
+__device__ __forceinline__ bool plan_item(const AttnArgs& a, const int* before, int per, int total, int may_split, int k,
+                                          Item& x, View& v, int& piece, int& pieces) {
+    const int ctas = gridDim.x, lane = threadIdx.x & 31;
+    int64_t at = static_cast<int64_t>(k) * ctas + (k & 1 ? ctas - 1 - static_cast<int>(blockIdx.x) : blockIdx.x);
+    pieces = 1, piece = 0;
+    const int rounds = total / ctas, rest_items = total - rounds * ctas;
+    if (may_split && rounds < kSplitRounds && k >= rounds) {
+        pieces = rest_items > 0 ? ctas / rest_items : 1;
+        piece = static_cast<int>(blockIdx.x) % pieces;
+        at = static_cast<int64_t>(rounds) * ctas + static_cast<int>(blockIdx.x) / pieces;
+        if (k > rounds) at = total;
+    }
+    x.b = -1;
+    if (at >= total) return false;
+    // the thread whose sequences hold it: how many end at or before it
+    int holder = 0;
+#pragma unroll 1
+    for (int y = 0; y < kThreads && y * per < a.seqs.batch; y += 32)
+        holder += __popc(__ballot_sync(0xffffffffu, before[y + lane + 1] <= at));
+    int rest = static_cast<int>(at) - before[holder], b = holder * per;
+    Seq sq = load_seq(a.seqs, a.pages.page_shift, b);
+#pragma unroll 1
+    for (int n; rest >= (n = items_of(a, sq));) {
+        rest -= n;
+        sq = load_seq(a.seqs, a.pages.page_shift, ++b);
+    }
+    const int pairs = (sq.nq * a.group + 2 * kTileRows - 1) / (2 * kTileRows);
+    x.row0 = (pairs - 1 - rest / a.pages.heads_kv) * 2 * kTileRows;
+    x.h = rest % a.pages.heads_kv;
+    x.rows = sq.nq * a.group;
+    x.t0 = sq.t0;
+    x.p0 = sq.p0;
+    v = View(x, a);
+    const int n = v.kt.count;
+    pieces = min(pieces, max(1, n / kPieceTiles));
+    if (piece >= pieces) return false;
+    x.b = b;
+    x.j0 = static_cast<int>(static_cast<int64_t>(n) * piece / pieces);
+    x.j1 = static_cast<int>(static_cast<int64_t>(n) * (piece + 1) / pieces);
+    return true;
+}
+
+// A row that has to be settled is marked until then: in the output, all that is not finite becomes a
+// NaN that no conversion makes; of a part, the sum of weights gets a minus sign.
+template <bool BF16>
+constexpr uint32_t kExponent = BF16 ? 0x7f80u : 0x7c00u;
+template <bool BF16>
+constexpr uint32_t kMark = kExponent<BF16> | 1u;
+
+// The rows of a warp whose bit is set, a lane a row; `l` is its sum of weights if it is part of one.
+// Of item k, which is noted in *items.
+template <bool BF16>
+__device__ __noinline__ void mark_rows(uint32_t rows, uint16_t* row, int dim, float* l, volatile uint32_t* items, int k) {
+    const int lane = threadIdx.x & 31;
+    const bool mine = (rows >> lane) & 1u;
+    if (lane == 0) *items |= 1u << (k & 31);
+    if (mine && l) *l = -*l;
+#pragma unroll 1
+    for (int d = 0; mine && !l && d < dim; d += 2) {
+        uint32_t x = *reinterpret_cast<uint32_t*>(row + d);
+        if ((x & kExponent<BF16>) == kExponent<BF16>) x = (x & 0xffff0000u) | kMark<BF16>;
+        if (((x >> 16) & kExponent<BF16>) == kExponent<BF16>) x = (x & 0xffffu) | (kMark<BF16> << 16);
+        *reinterpret_cast<uint32_t*>(row + d) = x;
+    }
+    __syncwarp();
+}
+
+// Settles the marked rows of a softmax warp: the same 32 of each of the CTA's items k whose bit k % 32
+// is set in `items`. Behind the last item, when nobody waits for a barrier any more: some 25 to 100
+// cycles a row and key can be more than a bounded wait lasts.
+template <int DP, bool BF16>
+__device__ __noinline__ void settle_marked(const AttnArgs& a, const int* before, int total, int may_split, uint32_t items) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first = warp * 32;
+    const int per = (a.seqs.batch + kThreads - 1) / kThreads;
+#pragma unroll 1
+    for (int k = 0; k <= total / static_cast<int>(gridDim.x) + 1; ++k) {
+        Item it;
+        View vw;
+        int piece, pieces;
+        if (((items >> (k & 31)) & 1u) == 0 || !plan_item(a, before, per, total, may_split, k, it, vw, piece, pieces)) continue;
+        const int row = it.row0 + first + lane, token = row / a.group;
+        float* slot = it.j1 - it.j0 < vw.kt.count ? part_slot<DP>(a, blockIdx.x) : nullptr;
+        bool marked = false;
+        if (row < it.rows && slot) {
+            float* l = slot + 2 * kTileRows + first + lane;
+            marked = __float_as_int(*l) < 0 && *l == *l;
+            if (marked) *l = fabsf(*l);
+        } else if (row < it.rows) {
+            const uint16_t* x = a.out + static_cast<int64_t>(it.t0 + token) * a.o_token +
+                                (it.h * a.group + row - token * a.group) * a.o_head;
+#pragma unroll 1
+            for (int d = 0; d < a.pages.dim && !marked; ++d) marked = x[d] == kMark<BF16>;
+        }
+        const uint32_t bad = __ballot_sync(0xffffffffu, marked);
+        if (bad)
+            settle_rows<kTileKeys, DP, BF16>(a, it.b, it.h, it.t0, it.p0, it.row0 + first, bad, vw.kt, it.j0, it.j1, slot,
+                                             2 * kTileRows, first);
+    }
+}
+
 template <int DP, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -349,7 +470,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* iempty = ifull + 2;   // [2] and was read by all
     uint64_t* turn = iempty + 2;    // [2] a row tile's turn at the tensor cores
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + 2);
-    volatile uint32_t* bad = tmem_slot + 1;                         // [8] boxes of tile j % 8 whose page id is no page
+    volatile int* loaded = reinterpret_cast<volatile int*>(tmem_slot + 1);  // tiles of K and V so far
+    volatile int* all_items = loaded + 1;                           // of all sequences
+    volatile uint32_t* to_settle = tmem_slot + 3;  // [8] of each softmax warp: items with marked rows, a bit each by k % 32
+    volatile uint32_t* bad = to_settle + 8;                         // [8] boxes of tile j % 8 whose page id is no page
     volatile int* posted = reinterpret_cast<volatile int*>(bad + 8);  // [2][kPostInts] items; b = -1: no more
     int* before = reinterpret_cast<int*>(smem + C::kListOff);       // [kThreads + 1] items before a thread's sequences
 
@@ -374,6 +498,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (threadIdx.x == 0) {
         if (may_split) part_desc<DP>(a, gridDim.x, blockIdx.x)[0] = 0;
+        *loaded = 0;
+        for (int w = 0; w < 8; ++w) to_settle[w] = 0;
         for (int s = 0; s < SL; ++s) {
             ptx::mbar_init(&full[s], 1);
             ptx::mbar_init(&empty[s], 2);
@@ -439,6 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 total = __shfl_sync(0xffffffffu, y, 31);
             }
             __syncwarp();
+            if (lane == 0) *all_items = total;
             const int ctas = gridDim.x;
             int i = 0, q_loads = 0;  // tiles of K and V, row pairs of Q so far
             bool ok = true;
@@ -486,6 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                 page);
                             }
                         }
+                        if (lane == 0) *loaded = i;
                         page = next;
                         ++j;
                     }
@@ -510,54 +638,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (ok) ++q_loads;
                     }
 
-                    // ---- item k + 1. Rounds of the CTAs run forth and back over the items, whose work
-                    // falls along a sequence: a CTA's shares even out. Where there are few rounds, the items
-                    // of the last, incomplete one are cut along their keys, among all CTAs.
+                    // ---- item k + 1
                     const int k1 = k + 1, s = k1 & 1;
-                    int64_t at = static_cast<int64_t>(k1) * ctas + (s ? ctas - 1 - static_cast<int>(blockIdx.x) : blockIdx.x);
-                    int pieces = 1, piece = 0;
-                    const int rounds = total / ctas, rest_items = total - rounds * ctas;
-                    if (may_split && rounds < kSplitRounds && k1 >= rounds) {
-                        pieces = rest_items > 0 ? ctas / rest_items : 1;
-                        piece = static_cast<int>(blockIdx.x) % pieces;
-                        at = static_cast<int64_t>(rounds) * ctas + static_cast<int>(blockIdx.x) / pieces;
-                        if (k1 > rounds) at = total;
-                    }
+                    int piece = 0, pieces = 1;
                     nx.b = -1;
-                    if (at < total) {
-                        // the thread whose sequences hold it: how many end at or before it
-                        int holder = 0;
-#pragma unroll 1
-                        for (int x = 0; x < kThreads && x * per < a.seqs.batch; x += 32)
-                            holder += __popc(__ballot_sync(0xffffffffu, before[x + lane + 1] <= at));
-                        int rest = static_cast<int>(at) - before[holder], b = holder * per;
-                        Seq sq = load_seq(a.seqs, a.pages.page_shift, b);
-#pragma unroll 1
-                        for (int n; rest >= (n = items_of(a, sq));) {
-                            rest -= n;
-                            sq = load_seq(a.seqs, a.pages.page_shift, ++b);
-                        }
-                        const int pairs = (sq.nq * a.group + 2 * kTileRows - 1) / (2 * kTileRows);
-                        nx.b = b;
-                        nx.row0 = (pairs - 1 - rest / a.pages.heads_kv) * 2 * kTileRows;
-                        nx.h = rest % a.pages.heads_kv;
-                        nx.rows = sq.nq * a.group;
-                        nx.t0 = sq.t0;
-                        nx.p0 = sq.p0;
-                        vx = View(nx, a);
-                        const int n = vx.kt.count;
-                        pieces = min(pieces, max(1, n / kPieceTiles));
-                        if (piece < pieces) {
-                            nx.j0 = static_cast<int>(static_cast<int64_t>(n) * piece / pieces);
-                            nx.j1 = static_cast<int>(static_cast<int64_t>(n) * (piece + 1) / pieces);
-                            nx_page = page_of(nx, vx, nx.j0);
-                            if (pieces > 1 && lane == 0) {
-                                int4* d = reinterpret_cast<int4*>(part_desc<DP>(a, ctas, blockIdx.x));
-                                d[1] = make_int4(nx.row0, nx.rows, nx.t0, nx.h);
-                                d[0] = make_int4(1, blockIdx.x - piece, pieces, 0);
-                            }
-                        } else {
-                            nx.b = -1;
+                    if (plan_item(a, before, per, total, may_split, k1, nx, vx, piece, pieces)) {
+                        nx_page = page_of(nx, vx, nx.j0);
+                        if (pieces > 1 && lane == 0) {
+                            int4* d = reinterpret_cast<int4*>(part_desc<DP>(a, ctas, blockIdx.x));
+                            d[1] = make_int4(nx.row0, nx.rows, nx.t0, nx.h);
+                            d[0] = make_int4(1, blockIdx.x - piece, pieces, 0);
                         }
                     }
                     if (ok && k1 >= 2) ok = warp_wait(&iempty[s], ((k1 >> 1) - 1) & 1, err, kErrLoad);
@@ -590,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
             for (int k = 0; ok && next_item(k, it, vw, true); ++k) {
                 if (!q_by_tma) {
-                    if (k > 0) ok = warp_wait(qempty, (k - 1) & 1, err, kErrMma);
+                    if (k > 0) ok = warp_wait_long(qempty, (k - 1) & 1, err, kErrMma, loaded);
                     if (!ok) break;
                     // 16 bytes a lane and copy, into the swizzled operand layout
                     constexpr int kStep = 32 / CH;  // rows between a lane's chunks
@@ -622,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int j = it.j0; j < it.j1 && ok; ++j, i += 2) {
                     const int k0 = vw.kt.first(j);
                     if (!vw.cut(k0)) continue;
-                    ok = warp_wait(dirty, asked++ & 1, err, kErrMma);
+                    ok = warp_wait_long(dirty, asked++ & 1, err, kErrMma, loaded);
                     const uint32_t v = ptx::smem_u32(smem + C::kKvOff + ((i + 1) % SL) * C::kTileBytes);
                     // rows [r, r1) of the tile: behind the last key, then between the sinks and the window
                     auto zero = [&](int r, int r1) {
@@ -890,11 +980,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             // rows whose sums are not finite while their sums of weights are
-            const uint32_t bad = __ballot_sync(0xffffffffu, odd && live_row && l == l);
-            if (bad)
-                settle_rows<kTileKeys, DP, BF16>(a, it.b, it.h, it.t0, it.p0, row - lane, bad, vw.kt, it.j0, it.j1, slot,
-                                                 2 * kTileRows, pr - lane);
+            // rows whose sums are not finite while their sums of weights are
+            const uint32_t rows = __ballot_sync(0xffffffffu, odd && live_row && l == l);
+            if (rows)
+                mark_rows<BF16>(rows, a.out + o_off, a.pages.dim, part ? slot + 2 * kTileRows + pr : nullptr, to_settle + warp, k);
         }
+        if (ok && to_settle[warp]) settle_marked<DP, BF16>(a, before, *all_items, may_split, to_settle[warp]);
     }
 
     ptx::tc_fence_before();

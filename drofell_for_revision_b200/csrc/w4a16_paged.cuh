@@ -110,10 +110,11 @@ struct RowSum {
     float m, l, o[4];
 };
 
-// One row over key tiles [i0, i1), key by key and each key by selection. A warp a row, lanes
-// over the head's dimensions. Slow: see settle_rows.
+// One row over key tiles [i0, i1) of 16, key by key and each key by selection. A warp a row, lanes
+// over the head's dimensions. Slow, but what the split kernel calls takes registers from its loop
+// (the form below: 2 to 3 % of a call).
 template <int TILE, bool BF16>
-__device__ __noinline__ RowSum careful_row(const AttnArgs& a, int b, int h, int64_t q_off, int p, const KeyTiles<TILE> kt,
+__device__ __noinline__ RowSum row_by_keys(const AttnArgs& a, int b, int h, int64_t q_off, int p, const KeyTiles<TILE> kt,
                                            int i0, int i1) {
     const int d = (threadIdx.x & 31) * 4;
     const bool in = d < a.pages.dim;
@@ -156,6 +157,73 @@ __device__ __noinline__ RowSum careful_row(const AttnArgs& a, int b, int h, int6
     return r;
 }
 
+// The same, 32 keys at once: a lane a key for the scores, lanes over the head's dimensions for the
+// values.
+template <int TILE, bool BF16>
+__device__ __noinline__ RowSum row_by_32(const AttnArgs& a, int b, int h, int64_t q_off, int p, const KeyTiles<TILE> kt,
+                                           int i0, int i1) {
+    static_assert(TILE % 32 == 0, "32 keys of a tile at once");
+    const int lane = threadIdx.x & 31, d = lane * 4;
+    RowSum r = {-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
+    const int32_t* table = a.seqs.tables + b * a.seqs.table_stride;
+#pragma unroll 1
+    for (int i = i0; i < i1; ++i) {
+#pragma unroll 1
+        for (int c = 0; c < TILE; c += 32) {
+            const int j = kt.first(i) + c + lane;
+            int page = -1;
+            if (visible(j, p, a.window, a.sinks)) page = table[j >> a.pages.page_shift];
+            const bool seen = page >= 0 && page < a.pages.num_pages;
+            const uint32_t keys = __ballot_sync(0xffffffffu, seen);
+            if (keys == 0) continue;
+            const int64_t at = seen ? page * a.pages.stride_page + h * a.pages.stride_head +
+                                          (j & ((1 << a.pages.page_shift) - 1)) * a.pages.stride_token
+                                    : 0;
+            float s = 0.f;
+            if (seen) {
+#pragma unroll 4
+                for (int x = 0; x < a.pages.dim; x += 8) {
+                    const uint4 qv = *reinterpret_cast<const uint4*>(a.q + q_off + x);
+                    const uint4 kv = *reinterpret_cast<const uint4*>(a.pages.k + at + x);
+                    const uint32_t qw[4] = {qv.x, qv.y, qv.z, qv.w}, kw[4] = {kv.x, kv.y, kv.z, kv.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 u = unpack2<BF16>(qw[e]), w = unpack2<BF16>(kw[e]);
+                        s += u.x * w.x + u.y * w.y;
+                    }
+                }
+            }
+            s = seen ? s * a.scale_log2 : -INFINITY;
+            float m = fmaxf(r.m, s);
+#pragma unroll
+            for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+            const float base = m == -INFINITY ? 0.f : m;
+            const float f = r.m == m ? 1.f : exp2_approx(r.m - base);
+            const float w = seen ? exp2_approx(s - base + kWeightBias<BF16, TILE>) : 0.f;
+            float sum = w;
+#pragma unroll
+            for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            r.m = m;
+            r.l = r.l * f + sum;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r.o[e] = f == 0.f ? 0.f : r.o[e] * f;
+#pragma unroll 8
+            for (int e = 0; e < 32; ++e) {
+                const float we = __shfl_sync(0xffffffffu, w, e);
+                const int64_t o = __shfl_sync(0xffffffffu, at, e);
+                if (((keys >> e) & 1u) == 0 || d >= a.pages.dim) continue;
+                const uint2 vv = *reinterpret_cast<const uint2*>(a.pages.v + o + d);
+                const float2 u = unpack2<BF16>(vv.x), v = unpack2<BF16>(vv.y);
+                r.o[0] += we * u.x;
+                r.o[1] += we * u.y;
+                r.o[2] += we * v.x;
+                r.o[3] += we * v.y;
+            }
+        }
+    }
+    return r;
+}
+
 // Rows whose weighted sums are not finite although their sums of weights are, a bit each from
 // row `first_row` on: either a value that the row sees is not finite, and so the result, or a
 // product took one in that it does not see (0 x inf, 0 x NaN), or split an infinite one's
@@ -163,6 +231,7 @@ __device__ __noinline__ RowSum careful_row(const AttnArgs& a, int b, int h, int6
 // looked for, once for the keys that all of them see; they decide their dimensions. Only a row
 // with others that are not finite is computed anew. The rows' results (part: their parts, with
 // `part_rows` rows to an array, the first of them `part_row`) are read back and set right.
+// This can take long: nobody may wait for it with a limit.
 template <int TILE, int DP, bool BF16>
 __device__ __noinline__ void settle_rows(const AttnArgs& a, int b, int h, int t0, int p0, int first_row, uint32_t bad,
                                          const KeyTiles<TILE> kt, int i0, int i1, float* part, int part_rows, int part_row) {
@@ -209,7 +278,7 @@ __device__ __noinline__ void settle_rows(const AttnArgs& a, int b, int h, int t0
         for (int i = i0; i < i1; ++i) {
             const int k0 = kt.first(i);
             if (all_see(k0, k0 + TILE - 1) || k0 > p) continue;
-#pragma unroll 1
+#pragma unroll 4
             for (int c = 0; c < TILE; ++c)
                 if (visible(k0 + c, p, a.window, a.sinks)) f |= kinds(k0 + c);
         }
@@ -228,8 +297,13 @@ __device__ __noinline__ void settle_rows(const AttnArgs& a, int b, int h, int t0
 #pragma unroll
         for (int e = 0; e < 4; ++e) anew |= ((f >> e) & 0x111u) == 0 && !(x[e] * 0.f == 0.f);
         if (__any_sync(0xffffffffu, anew)) {
-            const RowSum r = careful_row<TILE, BF16>(a, b, h, static_cast<int64_t>(t0 + token) * a.q_token + head * a.q_head, p, kt,
-                                                     i0, i1);
+            const int64_t q_off = static_cast<int64_t>(t0 + token) * a.q_token + head * a.q_head;
+            RowSum r;
+            if constexpr (TILE % 32 == 0) {
+                r = row_by_32<TILE, BF16>(a, b, h, q_off, p, kt, i0, i1);
+            } else {
+                r = row_by_keys<TILE, BF16>(a, b, h, q_off, p, kt, i0, i1);
+            }
             if (part && lane == 0) {
                 part[part_row + bit] = r.m;
                 part[part_rows + part_row + bit] = r.l;

@@ -1,4 +1,4 @@
-"""The paged cache where scores and values are extreme: weights far below the largest, infinite values.
+"""The paged cache where scores and values are extreme: weights far below the largest, infinities and NaN.
 
 Tolerances. As in test_gpu_paged.py an output is off by at most half a step of its own and half a
 step of the weights, (eps / 2) (|out| + sum p |v|) together. What comes on top is counted here:
@@ -134,3 +134,54 @@ def test_a_row_computed_anew_keeps_what_it_sees(dtype, value, n, new):
     assert torch.equal(torch.isnan(got), torch.isnan(want))
     assert torch.equal(torch.isinf(got), torch.isinf(want))
     assert torch.equal(got[torch.isinf(want)], want[torch.isinf(want)])
+
+
+# ---------------------------------------------------------------- long contexts
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_values_that_are_not_finite_at_the_end_of_a_long_context(dtype, value):
+    """The rows just before such a value are computed anew over 200000 keys each while their CTA's other
+    warps, with items of other sequences ahead of them, wait: nobody gives up, and nobody else's rows
+    change. Other sequences enough that no item is cut."""
+    hkv, dim, size, new, n, others = 8, 128, 64, 2048, 200064, 9
+    g = torch.Generator(device=DEV).manual_seed(97)
+    used, few = n // size, 2048 // size
+    k, v = (torch.randn(used + others * few, hkv, size, dim, device=DEV, generator=g, dtype=torch.float32).to(dtype)
+            for _ in range(2))
+    tables = torch.zeros(others + 1, used, dtype=torch.int32, device=DEV)
+    tables[0] = torch.arange(used, device=DEV)
+    tables[1:, :few] = used + torch.arange(others * few, device=DEV).view(others, few)
+    lens = torch.tensor([n] + [2048] * others, dtype=torch.int32, device=DEV)
+    cu = torch.arange(0, (others + 1) * new + 1, new, dtype=torch.int32, device=DEV)
+    q = torch.randn((others + 1) * new, hkv, dim, device=DEV, generator=g).to(dtype)
+    clean = paged.attention(q, k, v, tables, lens, cu_q=cu, max_q=new)
+    at = n - 60  # in the last tile of 128 keys, which begins at n - 128
+    keep = v[at // size, :, at % size].clone()
+    v[at // size, :, at % size] = value
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    got = paged.attention(q, k, v, tables, lens, cu_q=cu, max_q=new)
+    end.record()
+    assert paged.device_error(DEV) == 0
+    assert start.elapsed_time(end) < 10000
+    first, row = new - 128, at - (n - new)  # rows of the tile, the first that sees the value
+    assert (torch.isnan(got[row:new]) if value != value else got[row:new] == value).all()
+    assert torch.equal(got[:first], clean[:first]) and torch.equal(got[new:], clean[new:])
+    v[at // size, :, at % size] = keep
+    half = torch.finfo(dtype).eps / 2
+    for h in (0, 5):
+        kk, vv = (x[:used, h].reshape(-1, dim)[:at].double() for x in (k, v))
+        s = q[first:row, h].double() @ kk.T / math.sqrt(dim)
+        s.masked_fill_(torch.arange(at, device=DEV)[None] > torch.arange(n - 128, at, device=DEV)[:, None], -math.inf)
+        w = torch.softmax(s, -1)
+        want, spread = w @ vv, w @ vv.abs()
+        room = half * (want.abs() + spread) + (n / 16 + 400) * 2.0 ** -23 * spread
+        assert ((got[first:row, h].double() - want).abs() <= room).all()
+
+
+def test_many_items_with_rows_to_settle():
+    """More items a CTA than bits to note them by, a few of them with rows to settle."""
+    bt = Batch([60 + i % 50 for i in range(700)], [40] * 700, 8, 8, 64, 16, torch.float16, seed=101)
+    for b in range(0, 700, 9):
+        bt.v[int(bt.tables[b, 2]), :, b % 16, b % 64] = (math.nan, math.inf, -math.inf)[b % 3]
+    check_attention(bt)
