@@ -163,22 +163,31 @@ __global__ void __launch_bounds__(kThreads, DEEP ? 1 : 2) split_kernel(const __g
     // ---- units before each thread's share of the sequences
     const int per = (a.seqs.batch + kThreads - 1) / kThreads;
     {
-        const int b0 = min(a.seqs.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.seqs.batch, b0 + per);
         int sum = 0;
 #pragma unroll 1
-        for (int b = b0; b < b1; ++b) {
-            const Seq sq = load_seq(a.seqs, a.pages.page_shift, b);
-            const Units un = units_of(a, sq);
-            sum += un.units;
-            // rows of a sequence without any key are zero
-            if (blockIdx.x == b % gridDim.x && sq.nq > 0 && un.tiles == 0) {
-                const int chunks = a.pages.dim >> 3;
+        for (int i = 0; i < per; ++i) {
+            const int b = static_cast<int>(threadIdx.x) * per + i;
+            Seq sq = {0, 0, 0};
+            bool none = false;
+            if (b < a.seqs.batch) {
+                sq = load_seq(a.seqs, a.pages.page_shift, b);
+                const Units un = units_of(a, sq);
+                sum += un.units;
+                none = sq.nq > 0 && un.tiles == 0;
+            }
+            // rows of a sequence without any key are zero: a token a CTA, all lanes over its heads
 #pragma unroll 1
-                for (int64_t i = 0; i < int64_t{sq.nq} * a.heads * chunks; ++i) {
-                    const int64_t row = i / chunks, c = i % chunks;
-                    *reinterpret_cast<uint4*>(a.out + (sq.t0 + row / a.heads) * a.o_token + (row % a.heads) * a.o_head +
-                                              c * 8) = make_uint4(0, 0, 0, 0);
-                }
+            for (uint32_t left = __ballot_sync(0xffffffffu, none); left; left &= left - 1) {
+                const int from = __ffs(left) - 1, grid = gridDim.x;
+                const int t0 = __shfl_sync(0xffffffffu, sq.t0, from), nq = __shfl_sync(0xffffffffu, sq.nq, from);
+                const int first = (static_cast<int>(blockIdx.x) + grid - __shfl_sync(0xffffffffu, b, from) % grid) % grid;
+#pragma unroll 1
+                for (int t = first; t < nq; t += grid)
+#pragma unroll 1
+                    for (int h = lane; h < a.heads; h += 32)
+#pragma unroll 1
+                        for (int d = 0; d < a.pages.dim; d += 8)
+                            *reinterpret_cast<uint4*>(a.out + (t0 + t) * a.o_token + h * a.o_head + d) = make_uint4(0, 0, 0, 0);
             }
         }
 #pragma unroll

@@ -185,3 +185,42 @@ def test_many_items_with_rows_to_settle():
     for b in range(0, 700, 9):
         bt.v[int(bt.tables[b, 2]), :, b % 16, b % 64] = (math.nan, math.inf, -math.inf)[b % 3]
     check_attention(bt)
+
+
+# ---------------------------------------------------------------- sequences without a key
+def graph_time(call, calls=20):
+    """Microseconds a call, of several in one graph."""
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(calls):
+            call()
+    best = math.inf
+    for _ in range(4):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        graph.replay()
+        end.record()
+        torch.cuda.synchronize()
+        best = min(best, start.elapsed_time(end) * 1000 / calls)
+    return best
+
+
+@pytest.mark.parametrize("heads,hkv,dim,new", [(64, 8, 128, 1), (32, 32, 80, 1), (64, 8, 128, 2), (32, 32, 64, 30)])
+@pytest.mark.parametrize("batch", [16, 300])
+def test_empty_slots_of_a_padded_batch(heads, hkv, dim, new, batch):
+    """A fixed batch in which some slots hold no sequence: their rows are 0, the others right, and the
+    call takes no longer than with sequences there, within a factor of two (and 20 us) for noise."""
+    bt = Batch([500] * batch if batch < 100 else [60] * batch, [new] * batch, heads, hkv, dim, 16, torch.float16, seed=103)
+    full = attend(bt, 0.1)
+    base = graph_time(lambda: attend(bt, 0.1, out=full))
+    empty = torch.zeros(batch, dtype=torch.bool)
+    empty[[0, 3, 4, batch - 1]] = True
+    bt.lens.masked_fill_(empty.to(DEV), 0)
+    out = torch.full_like(full, math.nan)
+    attend(bt, 0.1, out=out)
+    assert (out[empty.repeat_interleave(new).to(DEV)] == 0).all()
+    bt.lens_l = [0 if e else n for n, e in zip(bt.lens_l, empty.tolist())]
+    check(bt, 0.1, 500, out=out)
+    took = graph_time(lambda: attend(bt, 0.1, out=out))
+    assert took < 2 * base + 20, (took, base)
