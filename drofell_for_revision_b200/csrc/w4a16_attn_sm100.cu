@@ -396,7 +396,7 @@ constexpr uint32_t kExponent = BF16 ? 0x7f80u : 0x7c00u;
 template <bool BF16>
 constexpr uint32_t kMark = kExponent<BF16> | 1u;
 
-// The rows of a warp whose bit is set, a lane a row; `l` is its sum of weights if it is part of one.
+// Marks the rows of a warp whose bit is set, a lane a row; `l` is the sum of weights if it is a part's.
 // Of item k, which is noted in *items.
 template <bool BF16>
 __device__ __noinline__ void mark_rows(uint32_t rows, uint16_t* row, int dim, float* l, volatile uint32_t* items, int k) {
@@ -414,12 +414,13 @@ __device__ __noinline__ void mark_rows(uint32_t rows, uint16_t* row, int dim, fl
     __syncwarp();
 }
 
-// Settles the marked rows of a softmax warp: the same 32 of each of the CTA's items k whose bit k % 32
-// is set in `items`. Behind the last item, when nobody waits for a barrier any more: some 25 to 100
-// cycles a row and key can be more than a bounded wait lasts.
+// Settles the marked rows of the CTA's items k whose bit k % 32 is set in `items`, 16 rows a softmax
+// warp. Behind the last item, when nobody waits for a barrier with a limit any more: rows that are
+// computed anew can take longer than such a wait lasts (prompts of 2048 tokens, one of them behind
+// 198016 others and with a NaN 60 tokens before its end: 2.9 ms without, 129 with it).
 template <int DP, bool BF16>
 __device__ __noinline__ void settle_marked(const AttnArgs& a, const int* before, int total, int may_split, uint32_t items) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first = warp * 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int per = (a.seqs.batch + kThreads - 1) / kThreads;
 #pragma unroll 1
     for (int k = 0; k <= total / static_cast<int>(gridDim.x) + 1; ++k) {
@@ -427,23 +428,26 @@ __device__ __noinline__ void settle_marked(const AttnArgs& a, const int* before,
         View vw;
         int piece, pieces;
         if (((items >> (k & 31)) & 1u) == 0 || !plan_item(a, before, per, total, may_split, k, it, vw, piece, pieces)) continue;
-        const int row = it.row0 + first + lane, token = row / a.group;
         float* slot = it.j1 - it.j0 < vw.kt.count ? part_slot<DP>(a, blockIdx.x) : nullptr;
-        bool marked = false;
-        if (row < it.rows && slot) {
-            float* l = slot + 2 * kTileRows + first + lane;
-            marked = __float_as_int(*l) < 0 && *l == *l;
-            if (marked) *l = fabsf(*l);
-        } else if (row < it.rows) {
-            const uint16_t* x = a.out + static_cast<int64_t>(it.t0 + token) * a.o_token +
-                                (it.h * a.group + row - token * a.group) * a.o_head;
 #pragma unroll 1
-            for (int d = 0; d < a.pages.dim && !marked; ++d) marked = x[d] == kMark<BF16>;
+        for (int first = warp * 16; first < 2 * kTileRows; first += 128) {
+            const int row = it.row0 + first + lane, token = row / a.group;
+            bool marked = false;
+            if (lane < 16 && row < it.rows && slot) {
+                float* l = slot + 2 * kTileRows + first + lane;
+                marked = __float_as_int(*l) < 0 && *l == *l;
+                if (marked) *l = fabsf(*l);
+            } else if (lane < 16 && row < it.rows) {
+                const uint16_t* x = a.out + static_cast<int64_t>(it.t0 + token) * a.o_token +
+                                    (it.h * a.group + row - token * a.group) * a.o_head;
+#pragma unroll 1
+                for (int d = 0; d < a.pages.dim && !marked; ++d) marked = x[d] == kMark<BF16>;
+            }
+            const uint32_t bad = __ballot_sync(0xffffffffu, marked);
+            if (bad)
+                settle_rows<kTileKeys, DP, BF16>(a, it.b, it.h, it.t0, it.p0, it.row0 + first, bad, vw.kt, it.j0, it.j1, slot,
+                                                 2 * kTileRows, first);
         }
-        const uint32_t bad = __ballot_sync(0xffffffffu, marked);
-        if (bad)
-            settle_rows<kTileKeys, DP, BF16>(a, it.b, it.h, it.t0, it.p0, it.row0 + first, bad, vw.kt, it.j0, it.j1, slot,
-                                             2 * kTileRows, first);
     }
 }
 
@@ -985,7 +989,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (rows)
                 mark_rows<BF16>(rows, a.out + o_off, a.pages.dim, part ? slot + 2 * kTileRows + pr : nullptr, to_settle + warp, k);
         }
-        if (ok && to_settle[warp]) settle_marked<DP, BF16>(a, before, *all_items, may_split, to_settle[warp]);
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // the softmax warps alone
+        uint32_t items = 0;
+        for (int w = 0; w < 8; ++w) items |= to_settle[w];
+        if (items) settle_marked<DP, BF16>(a, before, *all_items, may_split, items);
     }
 
     ptx::tc_fence_before();

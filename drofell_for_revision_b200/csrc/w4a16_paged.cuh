@@ -99,6 +99,23 @@ __device__ __forceinline__ float exp2_approx(float x) {
 template <bool BF16, int TILE>
 constexpr float kWeightBias = BF16 ? 0.f : TILE == 16 ? 15.f : 7.f;
 
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF16) {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    } else {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+}
+
 // f v of a piece's sum v under a factor f of at most 1 that may have run out to 0. No weight is
 // 0, so an infinity or NaN among the values stays one, however small its piece's share.
 __device__ __forceinline__ float share_of(float f, float v) {
@@ -113,9 +130,10 @@ struct RowSum {
 // One row over key tiles [i0, i1) of 16, key by key and each key by selection. A warp a row, lanes
 // over the head's dimensions. Slow, but what the split kernel calls takes registers from its loop
 // (the form below: 2 to 3 % of a call).
-template <int TILE, bool BF16>
-__device__ __noinline__ RowSum row_by_keys(const AttnArgs& a, int b, int h, int64_t q_off, int p, const KeyTiles<TILE> kt,
-                                           int i0, int i1) {
+template <int TILE, int DP, bool BF16>
+__device__ __noinline__ void row_by_keys(const AttnArgs& a, int b, int h, int t0, int p0, int row, const KeyTiles<TILE> kt, int i0,
+                                         int i1, float* part, int part_rows, int part_row) {
+    const int token = row / a.group, head = h * a.group + row - token * a.group, p = max(-1, p0 + token);
     const int d = (threadIdx.x & 31) * 4;
     const bool in = d < a.pages.dim;
     auto load4 = [&](const uint16_t* src, float (&x)[4]) {
@@ -127,7 +145,7 @@ __device__ __noinline__ RowSum row_by_keys(const AttnArgs& a, int b, int h, int6
     };
     RowSum r = {-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
     float q[4];
-    load4(a.q + q_off, q);
+    load4(a.q + static_cast<int64_t>(t0 + token) * a.q_token + head * a.q_head, q);
     const int32_t* table = a.seqs.tables + b * a.seqs.table_stride;
 #pragma unroll 1
     for (int i = i0; i < i1; ++i) {
@@ -154,74 +172,163 @@ __device__ __noinline__ RowSum row_by_keys(const AttnArgs& a, int b, int h, int6
             for (int e = 0; e < 4; ++e) r.o[e] = (f == 0.f ? 0.f : r.o[e] * f) + w * v[e];
         }
     }
-    return r;
+    if (part && (threadIdx.x & 31) == 0) {
+        part[part_row] = r.m;
+        part[part_rows + part_row] = r.l;
+    }
+    const float inv = part ? 1.f : r.l == 0.f ? 0.f : 1.f / r.l;
+    if (in && part) {
+        *reinterpret_cast<float4*>(part + 2 * part_rows + part_row * DP + d) = make_float4(r.o[0], r.o[1], r.o[2], r.o[3]);
+    } else if (in) {
+        *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(t0 + token) * a.o_token + head * a.o_head + d) =
+            make_uint2(pack2<BF16>(r.o[0] * inv, r.o[1] * inv), pack2<BF16>(r.o[2] * inv, r.o[3] * inv));
+    }
 }
 
-// The same, 32 keys at once: a lane a key for the scores, lanes over the head's dimensions for the
-// values.
-template <int TILE, bool BF16>
-__device__ __noinline__ RowSum row_by_32(const AttnArgs& a, int b, int h, int64_t q_off, int p, const KeyTiles<TILE> kt,
-                                           int i0, int i1) {
-    static_assert(TILE % 32 == 0, "32 keys of a tile at once");
-    const int lane = threadIdx.x & 31, d = lane * 4;
-    RowSum r = {-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
-    const int32_t* table = a.seqs.tables + b * a.seqs.table_stride;
-#pragma unroll 1
-    for (int i = i0; i < i1; ++i) {
-#pragma unroll 1
-        for (int c = 0; c < TILE; c += 32) {
-            const int j = kt.first(i) + c + lane;
-            int page = -1;
-            if (visible(j, p, a.window, a.sinks)) page = table[j >> a.pages.page_shift];
-            const bool seen = page >= 0 && page < a.pages.num_pages;
-            const uint32_t keys = __ballot_sync(0xffffffffu, seen);
-            if (keys == 0) continue;
-            const int64_t at = seen ? page * a.pages.stride_page + h * a.pages.stride_head +
-                                          (j & ((1 << a.pages.page_shift) - 1)) * a.pages.stride_token
-                                    : 0;
-            float s = 0.f;
-            if (seen) {
-#pragma unroll 4
-                for (int x = 0; x < a.pages.dim; x += 8) {
-                    const uint4 qv = *reinterpret_cast<const uint4*>(a.q + q_off + x);
-                    const uint4 kv = *reinterpret_cast<const uint4*>(a.pages.k + at + x);
-                    const uint32_t qw[4] = {qv.x, qv.y, qv.z, qv.w}, kw[4] = {kv.x, kv.y, kv.z, kv.w};
+// The same for up to 16 rows from row `row0` of the sequence on (a bit each), over key tiles of 128,
+// 16 keys at a time on mma.sync; values that are not finite count as 0. Operands come from
+// global memory in 16-byte pieces: a product's sum does not care for the order of the dimensions, nor a
+// result for which of its columns they are, as long as both sides agree on it. Loads are made
+// whether they are wanted or not (then from an address that is one): under conditions they wait for
+// one another. 64 dimensions of the values a sweep: what this takes of registers, the prompt
+// kernel's loop does without (with 128, 4 bytes spilled there and 5 % of a prompt). The rows' results
+// (part: their parts) are written.
+template <int DP, bool BF16>
+__device__ __noinline__ void rows_by_tiles(const AttnArgs& a, int b, int h, int t0, int p0, int row0, uint32_t rows,
+                                           const KeyTiles<128> kt, int i0, int i1, float* part, int part_rows, int part_row) {
+    constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
+    const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+    bool valid[2];
+    int p[2];
+    int64_t q_off[2];  // rows g and g + 8
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 u = unpack2<BF16>(qw[e]), w = unpack2<BF16>(kw[e]);
-                        s += u.x * w.x + u.y * w.y;
-                    }
+    for (int e = 0; e < 2; ++e) {
+        const int row = row0 + g + 8 * e, token = row / a.group, head = h * a.group + row - token * a.group;
+        valid[e] = (rows >> (g + 8 * e)) & 1u;
+        p[e] = valid[e] ? max(-1, p0 + token) : -1;
+        q_off[e] = valid[e] ? static_cast<int64_t>(t0 + token) * a.q_token + head * a.q_head : 0;
+    }
+    const int p_max = __reduce_max_sync(0xffffffffu, max(p[0], p[1]));
+    const int32_t* table = a.seqs.tables + b * a.seqs.table_stride;
+    auto load = [&](const uint16_t* x, int64_t off, int d, bool there) {
+        there = there && d < a.pages.dim;
+        const uint4 r = *reinterpret_cast<const uint4*>(x + (there ? off + d : 0));
+        return there ? r : make_uint4(0, 0, 0, 0);
+    };
+#pragma unroll 1
+    for (int d0 = 0; d0 < a.pages.dim; d0 += 64) {
+        float o[8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+#pragma unroll 1
+        for (int u = i0 * 8; u < i1 * 8; ++u) {
+            const int key0 = kt.first(u >> 3) + (u & 7) * 16;
+            if (key0 > p_max) break;
+            const int j = min(key0 + (lane & 15), p_max), page = table[j >> a.pages.page_shift];
+            const int64_t at = page >= 0 && page < a.pages.num_pages
+                                   ? page * a.pages.stride_page + h * a.pages.stride_head +
+                                         (j & ((1 << a.pages.page_shift) - 1)) * a.pages.stride_token
+                                   : -1;  // of key key0 + lane % 16
+            const uint32_t alive = __ballot_sync(0xffffffffu, at >= 0);
+            float s[2][4] = {};
+            {
+                const int64_t k0 = __shfl_sync(0xffffffffu, at, g), k1 = __shfl_sync(0xffffffffu, at, 8 + g);
+                // dimensions 8 tq .. 8 tq + 7 of each 32 for two steps
+#pragma unroll 2
+                for (int d = tq * 8; d < DP; d += 32) {
+                    const uint4 q0 = load(a.q, q_off[0], d, valid[0]), q1 = load(a.q, q_off[1], d, valid[1]);
+                    const uint4 x0 = load(a.pages.k, k0, d, k0 >= 0), x1 = load(a.pages.k, k1, d, k1 >= 0);
+                    const uint32_t u0[4] = {q0.x, q1.x, q0.y, q1.y}, u1[4] = {q0.z, q1.z, q0.w, q1.w};
+                    mma16816<BF16>(s[0], u0, x0.x, x0.y);
+                    mma16816<BF16>(s[0], u1, x0.z, x0.w);
+                    mma16816<BF16>(s[1], u0, x1.x, x1.y);
+                    mma16816<BF16>(s[1], u1, x1.z, x1.w);
                 }
             }
-            s = seen ? s * a.scale_log2 : -INFINITY;
-            float m = fmaxf(r.m, s);
+            // values of keys 2 tq, 2 tq + 1 and 8 further, dimensions d0 + 8 g .. d0 + 8 g + 7: column g of
+            // product j has dimension d0 + 8 g + j
+            uint32_t v[4][4];
 #pragma unroll
-            for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-            const float base = m == -INFINITY ? 0.f : m;
-            const float f = r.m == m ? 1.f : exp2_approx(r.m - base);
-            const float w = seen ? exp2_approx(s - base + kWeightBias<BF16, TILE>) : 0.f;
-            float sum = w;
+            for (int e = 0; e < 4; ++e) {
+                const int64_t key = __shfl_sync(0xffffffffu, at, (e >> 1) * 8 + tq * 2 + (e & 1));
+                const uint4 x = load(a.pages.v, key, d0 + g * 8, key >= 0);
+                v[e][0] = x.x, v[e][1] = x.y, v[e][2] = x.z, v[e][3] = x.w;
+            }
 #pragma unroll
-            for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-            r.m = m;
-            r.l = r.l * f + sum;
+            for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) r.o[e] = f == 0.f ? 0.f : r.o[e] * f;
-#pragma unroll 8
-            for (int e = 0; e < 32; ++e) {
-                const float we = __shfl_sync(0xffffffffu, w, e);
-                const int64_t o = __shfl_sync(0xffffffffu, at, e);
-                if (((keys >> e) & 1u) == 0 || d >= a.pages.dim) continue;
-                const uint2 vv = *reinterpret_cast<const uint2*>(a.pages.v + o + d);
-                const float2 u = unpack2<BF16>(vv.x), v = unpack2<BF16>(vv.y);
-                r.o[0] += we * u.x;
-                r.o[1] += we * u.y;
-                r.o[2] += we * v.x;
-                r.o[3] += we * v.y;
+                for (int e = 0; e < 4; ++e) {
+                    const int c = n * 8 + tq * 2 + (e & 1);
+                    if (((alive >> c) & 1u) == 0 || !visible(key0 + c, p[e >> 1], a.window, a.sinks)) s[n][e] = -INFINITY;
+                }
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                float x = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1])) * a.scale_log2;
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                x = fmaxf(x, m[r]);
+                const float f = x == m[r] ? 1.f : exp2_approx(m[r] - x);
+                m[r] = x;
+                l[r] *= f;
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    o[n][2 * r] *= f;
+                    o[n][2 * r + 1] *= f;
+                }
+                const float base = (x == -INFINITY ? 0.f : x) - kWeightBias<BF16, 128>;
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const float y = exp2_approx(s[n][2 * r] * a.scale_log2 - base);
+                    const float w = exp2_approx(s[n][2 * r + 1] * a.scale_log2 - base);
+                    l[r] += y + w;
+                    hi[2 * n + r] = pack2<BF16>(y, w);
+                    const float2 z = unpack2<BF16>(hi[2 * n + r]);
+                    lo[2 * n + r] = pack2<BF16>(y - z.x, w - z.y);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if ((v[e][i] & kExp) == kExp) v[e][i] &= 0xffff0000u;
+                    if (((v[e][i] >> 16) & kExp) == kExp) v[e][i] &= 0xffffu;
+                }
+                const uint32_t b0 = __byte_perm(v[0][i], v[1][i], 0x5410), b1 = __byte_perm(v[2][i], v[3][i], 0x5410);
+                const uint32_t c0 = __byte_perm(v[0][i], v[1][i], 0x7632), c1 = __byte_perm(v[2][i], v[3][i], 0x7632);
+                mma16816<BF16>(o[2 * i], hi, b0, b1);
+                mma16816<BF16>(o[2 * i], lo, b0, b1);
+                mma16816<BF16>(o[2 * i + 1], hi, c0, c1);
+                mma16816<BF16>(o[2 * i + 1], lo, c0, c1);
             }
         }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            if (!valid[r]) continue;
+            const int row = row0 + g + 8 * r, token = row / a.group, at = part_row + g + 8 * r;
+            uint16_t* out = a.out + static_cast<int64_t>(t0 + token) * a.o_token + (h * a.group + row - token * a.group) * a.o_head;
+            if (part && tq == 0) {
+                part[at] = m[r];
+                part[part_rows + at] = l[r];
+            }
+            const float inv = part ? 1.f : l[r] == 0.f ? 0.f : 1.f / l[r];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    const int d = d0 + (2 * tq + n) * 8 + i;
+                    const float x = o[i][2 * r + n] * inv, y = o[i + 1][2 * r + n] * inv;
+                    if (d >= a.pages.dim) continue;
+                    if (part) {
+                        *reinterpret_cast<float2*>(part + 2 * part_rows + at * DP + d) = make_float2(x, y);
+                    } else {
+                        *reinterpret_cast<uint32_t*>(out + d) = pack2<BF16>(x, y);
+                    }
+                }
+        }
     }
-    return r;
 }
 
 // Rows whose weighted sums are not finite although their sums of weights are, a bit each from
@@ -248,17 +355,31 @@ __device__ __noinline__ void settle_rows(const AttnArgs& a, int b, int h, int t0
         return k1 <= p_min && (a.window == 0 || p_max - k0 < a.window || k1 < a.sinks);
     };
     const int32_t* table = a.seqs.tables + b * a.seqs.table_stride;
-    // what key j's values are not: bits 0-3 NaN, 4-7 +inf, 8-11 -inf
-    auto kinds = [&](int j) {
-        const int page = table[j >> a.pages.page_shift];
-        if (page < 0 || page >= a.pages.num_pages || !in) return 0u;
-        const uint2 r = *reinterpret_cast<const uint2*>(a.pages.v + page * a.pages.stride_page + h * a.pages.stride_head +
-                                                        (j & ((1 << a.pages.page_shift) - 1)) * a.pages.stride_token + d);
-        const float2 u = unpack2<BF16>(r.x), v = unpack2<BF16>(r.y);
-        const float x[4] = {u.x, u.y, v.x, v.y};
-        uint32_t f = 0;
+    // What the values of eight keys from j on (of one page) are not, of those whose bit is set: bits 0-3
+    // NaN, 4-7 +inf, 8-11 -inf. All of them are looked at for an exponent of ones first.
+    auto kinds = [&](int j, uint32_t keys) {
+        constexpr uint32_t kCarry = BF16 ? 0x00800080u : 0x04000400u;
+        const int page = table[keys ? j >> a.pages.page_shift : 0];
+        const bool ok = in && keys && page >= 0 && page < a.pages.num_pages;
+        const uint16_t* v = a.pages.v + (ok ? page * a.pages.stride_page + h * a.pages.stride_head +
+                                                  (j & ((1 << a.pages.page_shift) - 1)) * a.pages.stride_token + d
+                                            : 0);
+        const int64_t step = ok ? a.pages.stride_token : 0;
+        uint2 r[8];
+        uint32_t any = 0, f = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f |= (x[e] != x[e] ? 1u : x[e] == INFINITY ? 16u : x[e] == -INFINITY ? 256u : 0u) << e;
+        for (int c = 0; c < 8; ++c) r[c] = *reinterpret_cast<const uint2*>(v + c * step);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) any |= ((r[c].x & 0x7fff7fffu) + kCarry) | ((r[c].y & 0x7fff7fffu) + kCarry);
+        if (!ok || (any & 0x80008000u) == 0) return 0u;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            const float2 x = unpack2<BF16>(r[c].x), y = unpack2<BF16>(r[c].y);
+            const float z[4] = {x.x, x.y, y.x, y.y};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if ((keys >> c) & 1u) f |= (z[e] != z[e] ? 1u : z[e] == INFINITY ? 16u : z[e] == -INFINITY ? 256u : 0u) << e;
+        }
         return f;
     };
     uint32_t shared = 0;
@@ -266,21 +387,26 @@ __device__ __noinline__ void settle_rows(const AttnArgs& a, int b, int h, int t0
     for (int i = i0; i < i1; ++i) {
         const int k0 = kt.first(i);
         if (!all_see(k0, k0 + TILE - 1)) continue;
-#pragma unroll 4
-        for (int c = 0; c < TILE; ++c) shared |= kinds(k0 + c);
+#pragma unroll 2
+        for (int c = 0; c < TILE; c += 8) shared |= kinds(k0 + c, 0xffu);
+        if (__all_sync(0xffffffffu, !in || (shared & 15u) == 15u)) break;  // all NaN already
     }
-#pragma unroll 1
-    for (; bad; bad &= bad - 1) {
-        const int bit = __ffs(bad) - 1, row = first_row + bit, token = row / a.group;
+    // sets a row's result right; whether it has to be computed anew first
+    auto settle = [&](int bit, bool may_be_anew) {
+        const int row = first_row + bit, token = row / a.group;
         const int head = h * a.group + row - token * a.group, p = max(-1, p0 + token);
         uint32_t f = shared;
 #pragma unroll 1
         for (int i = i0; i < i1; ++i) {
             const int k0 = kt.first(i);
             if (all_see(k0, k0 + TILE - 1) || k0 > p) continue;
-#pragma unroll 4
-            for (int c = 0; c < TILE; ++c)
-                if (visible(k0 + c, p, a.window, a.sinks)) f |= kinds(k0 + c);
+#pragma unroll 1
+            for (int c = k0; c < k0 + TILE; c += 8) {
+                uint32_t keys = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) keys |= static_cast<uint32_t>(visible(c + e, p, a.window, a.sinks)) << e;
+                f |= kinds(c, keys);
+            }
         }
         const int64_t o_off = static_cast<int64_t>(t0 + token) * a.o_token + head * a.o_head + d;
         float* slot = part ? part + 2 * part_rows + (part_row + bit) * DP + d : nullptr;
@@ -295,35 +421,40 @@ __device__ __noinline__ void settle_rows(const AttnArgs& a, int b, int h, int t0
         }
         bool anew = false;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) anew |= ((f >> e) & 0x111u) == 0 && !(x[e] * 0.f == 0.f);
-        if (__any_sync(0xffffffffu, anew)) {
-            const int64_t q_off = static_cast<int64_t>(t0 + token) * a.q_token + head * a.q_head;
-            RowSum r;
-            if constexpr (TILE % 32 == 0) {
-                r = row_by_32<TILE, BF16>(a, b, h, q_off, p, kt, i0, i1);
-            } else {
-                r = row_by_keys<TILE, BF16>(a, b, h, q_off, p, kt, i0, i1);
-            }
-            if (part && lane == 0) {
-                part[part_row + bit] = r.m;
-                part[part_rows + part_row + bit] = r.l;
-            }
-            const float inv = part ? 1.f : r.l == 0.f ? 0.f : 1.f / r.l;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = r.o[e] * inv;
-        }
-        // what the row sees of infinities and NaN decides, whichever way the rest was computed
-#pragma unroll
         for (int e = 0; e < 4; ++e) {
             const uint32_t k = (f >> e) & 0x111u;
             if (k) x[e] = k == 16u ? INFINITY : k == 256u ? -INFINITY : NAN;
+            anew |= k == 0 && !(x[e] * 0.f == 0.f);
         }
+        if (may_be_anew && __any_sync(0xffffffffu, anew)) return true;
         if (in && part) {
             *reinterpret_cast<float4*>(slot) = make_float4(x[0], x[1], x[2], x[3]);
         } else if (in) {
             *reinterpret_cast<uint2*>(a.out + o_off) = make_uint2(pack2<BF16>(x[0], x[1]), pack2<BF16>(x[2], x[3]));
         }
+        return false;
+    };
+    uint32_t anew = 0;
+#pragma unroll 1
+    for (uint32_t left = bad; left; left &= left - 1)
+        if (settle(__ffs(left) - 1, true)) anew |= left & -left;
+    if (anew == 0) return;
+    if constexpr (TILE == 128) {
+#pragma unroll 1
+        for (int r = 0; r < 32; r += 16)
+            if ((anew >> r) & 0xffffu)
+                rows_by_tiles<DP, BF16>(a, b, h, t0, p0, first_row + r, (anew >> r) & 0xffffu, kt, i0, i1, part, part_rows,
+                                        part_row + r);
+    } else {
+#pragma unroll 1
+        for (uint32_t left = anew; left; left &= left - 1)
+            row_by_keys<TILE, DP, BF16>(a, b, h, t0, p0, first_row + __ffs(left) - 1, kt, i0, i1, part, part_rows,
+                                        part_row + __ffs(left) - 1);
     }
+    __syncwarp();
+    // what a row sees of infinities and NaN decides, whichever way the rest was computed
+#pragma unroll 1
+    for (; anew; anew &= anew - 1) settle(__ffs(anew) - 1, false);
 }
 
 }  // namespace w4a16

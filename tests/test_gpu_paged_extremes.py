@@ -224,3 +224,32 @@ def test_empty_slots_of_a_padded_batch(heads, hkv, dim, new, batch):
     check(bt, 0.1, 500, out=out)
     took = graph_time(lambda: attend(bt, 0.1, out=out))
     assert took < 2 * base + 20, (took, base)
+
+
+# ---------------------------------------------------------------- rows computed anew
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,hkv,dim", [(4, 4, 128), (8, 1, 64), (6, 2, 128), (10, 2, 80), (4, 4, 120), (12, 4, 8)])
+@pytest.mark.parametrize("n,new,window,sinks", [(2600, 260, 0, 0), (700, 700, 0, 0), (2600, 300, 500, 4), (300, 130, 33, 70)])
+def test_rows_computed_anew(dtype, heads, hkv, dim, n, new, window, sinks):
+    """Values that are not finite all along the new tokens and at the edges of what windows show: most
+    rows have some in their tiles that they do not see, and compute everything else anew. Some
+    pages are no pages."""
+    bt = Batch([n, 40], [new, 20], heads, hkv, dim, 16, dtype, seed=107)
+    hide = [torch.zeros(n, dtype=torch.bool), torch.zeros(40, dtype=torch.bool)]
+    for j in range(max(0, n - new - 3), n, 37):
+        bt.v[int(bt.tables[0, j // 16]), :, j % 16, j % dim] = (math.nan, math.inf, -math.inf)[j % 3]
+    for j in range(5, max(6, n - new - window), 97):
+        bt.v[int(bt.tables[0, j // 16]), :, j % 16, (j // 7) % dim] = math.inf
+    good, bt.tables = bt.tables, bt.tables.clone()
+    bt.tables[0, 3], bt.tables[0, (n - new) // 16] = -1, bt.k.shape[0]
+    for at in (3, (n - new) // 16):
+        hide[0][at * 16:at * 16 + 16] = True
+    got = attend(bt, 1 / math.sqrt(dim), window=window, sinks=sinks)
+    bt.tables = good
+    want, spread = exact_attention(bt, 1 / math.sqrt(dim), window, sinks, hide)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isinf(got), torch.isinf(want))
+    finite = torch.isfinite(want)
+    assert torch.equal(got[torch.isinf(want)].double(), want[torch.isinf(want)])
+    room = torch.finfo(dtype).eps / 2 * (want.abs() + spread) + (n / 16 + 400) * 2.0 ** -23 * spread + n * 2.0 ** -32 * 8 + 2.0 ** -25
+    assert ((got.double() - want).abs() <= room)[finite].all()
+    assert finite.any() and not finite.all()
