@@ -53,17 +53,20 @@ def append_kv(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, v: 
 
 
 def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor,
-              cu_q: Optional[torch.Tensor] = None, max_q: int = 1, scale: Optional[float] = None, window: int = 0,
+              cu_q: Optional[torch.Tensor] = None, max_q: Optional[int] = None, scale: Optional[float] = None, window: int = 0,
               sinks: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """softmax(scale q k^T) v of every new token over its sequence's tokens up to itself;
     with ``window`` over the last ``window`` of them (itself counted) and the sequence's first
     ``sinks``. q [tokens, heads, head dim], heads a multiple of the key-value heads; scale
-    (positive) 1 / sqrt(head dim) unless given. ``max_q`` is at least the most new tokens of a sequence
-    (rows beyond it get no result). Rows that see nothing are 0; rows of no sequence are left
-    as they were (undefined in an output that this call makes). ``out`` must not overlap q
-    or hold an element twice."""
+    (positive) 1 / sqrt(head dim) unless given. ``max_q`` is at least the most new tokens of a
+    sequence: rows beyond it get no result. Left out, it is the number of rows (1 without
+    ``cu_q``); given, it lets the call choose its kernel and cut its work by what is there. Rows
+    that see nothing are 0; rows of no sequence are left as they were (undefined in an output
+    that this call makes). ``out`` must not overlap q or hold an element twice."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
+    if max_q is None:
+        max_q = 1 if cu_q is None else q.shape[0]
     return _ext().paged_attention(q, k_pages, v_pages, tables, lens, cu_q, max_q, scale, window, sinks, out)
 
 
@@ -80,7 +83,7 @@ def device_error(device: Optional[torch.device] = None) -> int:
 def attention_forward(layernorm: torch.Tensor, norm_epsilon: float, q_proj: int, k_proj: int, v_proj: int, o_proj: int,
                       x: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor,
                       lens: torch.Tensor, rope: Optional[torch.Tensor] = None, cu_q: Optional[torch.Tensor] = None,
-                      max_q: int = 1, window: int = 0, sinks: int = 0, interleaved: bool = False,
+                      max_q: Optional[int] = None, window: int = 0, sinks: int = 0, interleaved: bool = False,
                       output: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The attention block of a decoder layer, beside ``exllama.mlp_forward_v2``: RMSNorm and the
     q, k, v projections (``attention_forward_qkv_stage_v2``), k and v into the pages, attention

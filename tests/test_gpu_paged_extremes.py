@@ -253,3 +253,15 @@ def test_rows_computed_anew(dtype, heads, hkv, dim, n, new, window, sinks):
     room = torch.finfo(dtype).eps / 2 * (want.abs() + spread) + (n / 16 + 400) * 2.0 ** -23 * spread + n * 2.0 ** -32 * 8 + 2.0 ** -25
     assert ((got.double() - want).abs() <= room)[finite].all()
     assert finite.any() and not finite.all()
+
+
+# ---------------------------------------------------------------- arguments left out
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 1, 2], [40, 7, 0], [300, 1, 150]])
+def test_max_q_may_be_left_out(new):
+    """With row offsets and no max_q every row of a sequence gets its result."""
+    bt = Batch([n + 50 for n in new], new, 8, 2, 64, 16, torch.float16, seed=109)
+    cu = torch.tensor(bt.cu_l, dtype=torch.int32, device=DEV)
+    out = torch.full_like(bt.q, math.nan)
+    paged.attention(bt.q, bt.k, bt.v, bt.tables, bt.lens, cu_q=cu, out=out)
+    want, spread = exact_attention(bt, 0.125, 0, 0)
+    assert ((out.double() - want).abs() <= 2.0 ** -11 * (want.abs() + spread) + 1e-5 * float(bt.v.abs().max())).all()
