@@ -99,6 +99,58 @@ int check_written(const w4a16_rows* r, int tokens, int heads, int dim, const cha
     return W4A16_OK;
 }
 
+// Two sets of runs of `size` bytes (or elements), their first runs `delta` apart: a run of the one and
+// one of the other lie sum x_i stride_i + delta apart, lo_i <= x_i <= hi_i. Whether any two share
+// memory: strides in falling order, and of each only the x that the others can still make up for.
+struct Apart {
+    int64_t stride, lo, hi;
+};
+bool share(int64_t delta, const Apart* d, int n, int64_t size) {
+    if (n == 0) return delta < size && -delta < size;
+    int64_t reach = size - 1;  // of the other strides
+    for (int i = 1; i < n; ++i) reach += d[i].stride * std::max(-d[i].lo, d[i].hi);
+    if (d->stride == 0) return share(delta, d + 1, n - 1, size);
+    const auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0 ? 1 : 0); };
+    const int64_t first = std::max(d->lo, -floor_div(delta + reach, d->stride));
+    const int64_t last = std::min(d->hi, floor_div(reach - delta, d->stride));
+    for (int64_t x = first; x <= last; ++x)
+        if (share(delta + x * d->stride, d + 1, n - 1, size)) return true;
+    return false;
+}
+
+// Whether two sets of runs with the same strides share memory; addresses and strides in bytes.
+bool share_alike(const void* a, const void* b, Extent x, Extent y, Extent z, int64_t size) {
+    Extent e[3] = {x, y, z};
+    std::sort(e, e + 3, [](const Extent& u, const Extent& w) { return u.stride > w.stride; });
+    Apart d[3];
+    int n = 0;
+    for (const Extent& u : e)
+        if (u.count > 1) d[n++] = {u.stride, 1 - u.count, u.count - 1};
+    return share(static_cast<int64_t>(reinterpret_cast<intptr_t>(a) - reinterpret_cast<intptr_t>(b)), d, n, size);
+}
+
+// Whether rows share memory. Views of one buffer (a q/k/v product, say) have their strides in common.
+// Where they do not, and their ranges meet, rows count as sharing it: which of them do would
+// have to be searched for.
+bool rows_share(const w4a16_rows* a, int heads_a, const w4a16_rows* b, int heads_b, int tokens, int dim) {
+    const auto span = [&](const w4a16_rows* r, int heads) {
+        return ((tokens - 1) * r->stride_token + (heads - 1) * r->stride_head + dim) * 2;
+    };
+    const intptr_t pa = reinterpret_cast<intptr_t>(a->dev), pb = reinterpret_cast<intptr_t>(b->dev);
+    if (pa + span(a, heads_a) <= pb || pb + span(b, heads_b) <= pa) return false;
+    if ((tokens > 1 && a->stride_token != b->stride_token) || (pa - pb) % 2) return true;
+    Apart d[3] = {{tokens > 1 ? a->stride_token : 0, 1 - int64_t{tokens}, int64_t{tokens} - 1}};
+    int n = 1;
+    if (heads_a > 1 && heads_b > 1 && a->stride_head == b->stride_head) {
+        d[n++] = {a->stride_head, 1 - int64_t{heads_b}, int64_t{heads_a} - 1};
+    } else {
+        d[n++] = {heads_a > 1 ? a->stride_head : 0, 0, int64_t{heads_a} - 1};
+        d[n++] = {heads_b > 1 ? b->stride_head : 0, 1 - int64_t{heads_b}, 0};
+    }
+    std::sort(d, d + n, [](const Apart& x, const Apart& y) { return x.stride > y.stride; });
+    return share((pa - pb) / 2, d, n, dim);
+}
+
 PageView page_view(const w4a16_pages* p) {
     PageView v;
     v.k = static_cast<const uint16_t*>(p->k_dev);
@@ -208,6 +260,19 @@ int w4a16_append_kv(const w4a16_pages* pages, const w4a16_seqs* seqs, const w4a1
             return report_error(W4A16_ERR_INVALID, "a rope table of %d positions for tables of %lld tokens", rope_positions,
                                 static_cast<long long>(seqs->table_width) * pages->page_size);
     }
+    if (share_alike(pages->k_dev, pages->v_dev, {pages->num_pages, pages->stride_page * 2},
+                    {pages->heads_kv, pages->stride_head * 2}, {pages->page_size, pages->stride_token * 2},
+                    int64_t{pages->head_dim} * 2))
+        return report_error(W4A16_ERR_INVALID, "K and V pages that overlap");
+    if (with_q) {
+        const int hkv = pages->heads_kv, dim = pages->head_dim, n = seqs->tokens;
+        const bool in_place = q->dev == q_out->dev && (n == 1 || q->stride_token == q_out->stride_token) &&
+                              (heads == 1 || q->stride_head == q_out->stride_head);
+        if (!in_place && rows_share(q, heads, q_out, heads, n, dim))
+            return report_error(W4A16_ERR_INVALID, "q_out must be q or not overlap it");
+        if (rows_share(k, hkv, q_out, heads, n, dim) || rows_share(v, hkv, q_out, heads, n, dim))
+            return report_error(W4A16_ERR_INVALID, "q_out must not overlap k or v");
+    }
     AppendArgs a = {};
     a.pages = page_view(pages);
     a.seqs = seq_view(seqs);
@@ -254,7 +319,8 @@ int w4a16_paged_attention(const w4a16_pages* pages, const w4a16_seqs* seqs, cons
     rc = check_rows(q, "q");
     if (rc == W4A16_OK) rc = check_written(out, seqs->tokens, heads, pages->head_dim, "out");
     if (rc != W4A16_OK) return rc;
-    if (q->dev == out->dev) return report_error(W4A16_ERR_INVALID, "out must not be q");
+    if (rows_share(q, heads, out, heads, seqs->tokens, pages->head_dim))
+        return report_error(W4A16_ERR_INVALID, "out must not overlap q");
     AttnArgs a = attn_args(pages, seqs, heads, window, sinks);
     a.q = static_cast<const uint16_t*>(q->dev);
     a.q_token = q->stride_token, a.q_head = q->stride_head;
@@ -299,8 +365,15 @@ int w4a16_copy_pages(void* k_dev, void* v_dev, int64_t stride_layer_bytes, int64
                             static_cast<long long>(page_bytes));
     if (page_bytes % 16 || stride_page_bytes % 16 || stride_layer_bytes % 16 || !aligned16(k_dev) || !aligned16(v_dev))
         return report_error(W4A16_ERR_INVALID, "pages and their strides must be multiples of 16 bytes");
-    if (stride_page_bytes < page_bytes || stride_layer_bytes < 0)
+    const int64_t in_layer = (num_pages - 1) * stride_page_bytes + page_bytes;
+    if (stride_page_bytes < page_bytes || stride_layer_bytes < 0 ||
+        (layers > 1 && stride_layer_bytes < in_layer &&
+         (num_pages > 1 ? stride_page_bytes < (layers - 1) * stride_layer_bytes + page_bytes : true)) ||
+        (layers > 1 && stride_layer_bytes < page_bytes))
         return report_error(W4A16_ERR_INVALID, "pages that overlap");
+    // the same memory for both is copied twice to the same effect
+    if (k_dev != v_dev && share_alike(k_dev, v_dev, {layers, stride_layer_bytes}, {num_pages, stride_page_bytes}, {1, 0}, page_bytes))
+        return report_error(W4A16_ERR_INVALID, "K and V pages that overlap");
     if (pairs == 0 || layers == 0) return W4A16_OK;
     if (!src_host || !dst_host) return report_error(W4A16_ERR_INVALID, "null page ids");
     std::vector<uint8_t> seen(num_pages, 0);  // 1 written, 2 read

@@ -42,7 +42,8 @@ def append_kv(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, v: 
               rope: Optional[torch.Tensor] = None, interleaved: bool = False,
               q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """Store the new tokens' k and v [tokens, key-value heads, head dim] into their pages and
-    return q [tokens, heads, head dim] rotated (in ``q_out``, which may be q; None without q).
+    return q [tokens, heads, head dim] rotated (in ``q_out``, which may be q and must not overlap
+    it, k or v otherwise; None without q).
 
     ``rope`` is a float32 table [positions, rope dim]: a position's cosines, then its sines
     (``rope_table``); q and k are rotated by it, dimension i with i + rope dim / 2, or 2 i

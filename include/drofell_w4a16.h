@@ -278,9 +278,9 @@ typedef struct w4a16_rows {
  * width * page_size. Dimensions i and i + rope_dim / 2 rotate together, with interleaved
  * 2 i and 2 i + 1; those past rope_dim pass through. rope_dim is a multiple of 16 (8 when
  * interleaved). fp32 arithmetic, rounded once. Pages that two sequences share must not be
- * written to; pages, or rows of q_out, that overlap in memory are refused. Tokens of a
- * negative position (more new tokens than the length) are not stored, their q passes
- * unrotated. */
+ * written to. Pages that overlap in memory (K's and V's, too), and rows of q_out that overlap
+ * or lie on k, v or, other than q itself, q, are refused. Tokens of a negative position (more
+ * new tokens than the length) are not stored, their q passes unrotated. */
 W4A16_API int w4a16_append_kv(const w4a16_pages* pages, const w4a16_seqs* seqs, const w4a16_rows* k,
                               const w4a16_rows* v, const w4a16_rows* q, const w4a16_rows* q_out, int heads,
                               const float* rope_dev, int rope_positions, int rope_dim, int interleaved, void* stream);
@@ -305,8 +305,9 @@ W4A16_API int w4a16_paged_error(int device, void* stream, int* err_out);
 
 /* Copy whole pages, of every layer and of K and V: page dst_host[i] gets page src_host[i].
  * A page is page_bytes contiguous bytes at layer * stride_layer_bytes + id *
- * stride_page_bytes (all multiples of 16). The ids are read on the host during the call. No
- * page may be written twice, or both read and written. */
+ * stride_page_bytes (all multiples of 16), pages and layers apart from one another, K and V apart
+ * or the same memory. The ids are read on the host during the call. No page may be written
+ * twice, or both read and written. */
 W4A16_API int w4a16_copy_pages(void* k_dev, void* v_dev, int64_t stride_layer_bytes, int64_t stride_page_bytes,
                                int layers, int num_pages, int64_t page_bytes, const int32_t* src_host,
                                const int32_t* dst_host, int pairs, int device, void* stream);
