@@ -376,17 +376,28 @@ int w4a16_copy_pages(void* k_dev, void* v_dev, int64_t stride_layer_bytes, int64
         return report_error(W4A16_ERR_INVALID, "K and V pages that overlap");
     if (pairs == 0 || layers == 0) return W4A16_OK;
     if (!src_host || !dst_host) return report_error(W4A16_ERR_INVALID, "null page ids");
-    std::vector<uint8_t> seen(num_pages, 0);  // 1 written, 2 read
-    for (int i = 0; i < pairs; ++i) {
-        const int s = src_host[i], d = dst_host[i];
-        if (s < 0 || s >= num_pages || d < 0 || d >= num_pages)
-            return report_error(W4A16_ERR_INVALID, "copy %d of page %d to %d: %d pages", i, s, d, num_pages);
-        if (seen[d] || s == d || (seen[s] & 1))
-            return report_error(W4A16_ERR_INVALID, "copy %d of page %d to %d: a page written twice, or read and written", i,
-                                s, d);
-        seen[d] = 1;
-        seen[s] |= 2;
+    for (int i = 0; i < pairs; ++i)
+        if (src_host[i] < 0 || src_host[i] >= num_pages || dst_host[i] < 0 || dst_host[i] >= num_pages)
+            return report_error(W4A16_ERR_INVALID, "copy %d of page %d to %d: %d pages", i, src_host[i], dst_host[i], num_pages);
+    // The pages written: a byte for every page of the cache, or a sorted list where the copies are few
+    // beside it, so that the cost is that of the copies. 3000 of 8000 pages 136 us a call with bytes,
+    // 215 sorted; 1 of 200000 14.8 with bytes, 8.2 sorted; 511 of 2000 34 with either.
+    std::vector<uint8_t> is_written;
+    std::vector<int32_t> written;
+    if (num_pages / 16 <= pairs) {
+        is_written.assign(num_pages, 0);
+    } else {
+        written.assign(dst_host, dst_host + pairs);
+        std::sort(written.begin(), written.end());
     }
+    for (int i = 0; i < pairs; ++i) {
+        const bool twice = written.empty() ? is_written[dst_host[i]] != 0 : i > 0 && written[i] == written[i - 1];
+        if (twice) return report_error(W4A16_ERR_INVALID, "page %d written twice", written.empty() ? dst_host[i] : written[i]);
+        if (written.empty()) is_written[dst_host[i]] = 1;
+    }
+    for (int i = 0; i < pairs; ++i)
+        if (written.empty() ? is_written[src_host[i]] != 0 : std::binary_search(written.begin(), written.end(), src_host[i]))
+            return report_error(W4A16_ERR_INVALID, "copy %d of page %d to %d: a page read and written", i, src_host[i], dst_host[i]);
     DeviceGuard guard(device);
     if (!guard.ok) return report_error(W4A16_ERR_INVALID, "device %d", device);
     CopyArgs a = {};

@@ -5,7 +5,9 @@ A call that passes its checks would go on to the GPU: the cases that have to be 
 a later refusal, or are asked of the search alone."""
 import ctypes
 import itertools
+import math
 import random
+import time
 
 import pytest
 
@@ -127,3 +129,31 @@ def test_layers_inside_pages(layers, stride_layer, stride_page, bad):
     ids = (ctypes.c_int * 1)(0)
     assert _capi.lib().w4a16_copy_pages(FAKE, FAKE, stride_layer, stride_page, layers, 5, 4096, ids, ids, 1, 0, None) == INVALID
     assert ("overlap" in message()) == bad
+
+
+# ---------------------------------------------------------------- the ids of a copy
+def test_copies_cost_what_they_copy():
+    """The checks of two copies take no longer, and no more memory, in a cache of 2^31 - 1 pages."""
+    best = math.inf
+    for _ in range(5):
+        start = time.perf_counter()
+        assert copy([1, 2], [3, 3], num=(1 << 31) - 1, size=16, stride_page=16, layers=1) == INVALID
+        best = min(best, time.perf_counter() - start)
+    assert "written twice" in message()
+    assert best < 0.005
+
+
+@pytest.mark.parametrize("num", [10, 1000])  # as many pages as copies, and many more
+def test_copies_against_sets(num):
+    r = random.Random(11)
+    seen = set()
+    for _ in range(2000):
+        n = r.randrange(1, 7)
+        src, dst = [r.randrange(-1, 11) for _ in range(n)], [r.randrange(0, 10) for _ in range(n)]
+        if min(src) >= 0 and max(src) < num and len(set(dst)) == n and not set(src) & set(dst):
+            continue  # would be launched
+        assert copy(src, dst, num=num, stride_page=4096, stride_layer=1 << 30) == INVALID
+        want = ("pages" if min(src) < 0 or max(src) >= num else "written twice" if len(set(dst)) < n else "read and written")
+        assert want in message()
+        seen.add(want)
+    assert len(seen) == 3
