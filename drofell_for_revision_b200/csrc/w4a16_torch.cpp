@@ -244,8 +244,8 @@ at::Tensor append_kv(const at::Tensor& k_pages, const at::Tensor& v_pages, const
         qor = w4a16_rows{out.data_ptr(), out.stride(0), out.stride(1)};
     }
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(k_pages.device().index()).stream();
-    if (tokens > 0 && (!q.has_value() || heads > 0))
-        check(w4a16_append_kv(&p.pages, &p.seqs, &kr, &vr, q.has_value() ? &qr : nullptr, &qor, static_cast<int>(heads),
+    if (tokens > 0)  // a q without heads is no q: k and v are stored all the same
+        check(w4a16_append_kv(&p.pages, &p.seqs, &kr, &vr, heads > 0 ? &qr : nullptr, &qor, static_cast<int>(heads),
                               rope.has_value() ? rope->data_ptr<float>() : nullptr,
                               rope.has_value() ? static_cast<int>(std::min<int64_t>(rope->size(0), 0x7fffffff)) : 0,
                               rope.has_value() ? static_cast<int>(rope->size(1)) : 0, interleaved ? 1 : 0, stream));

@@ -265,3 +265,14 @@ def test_max_q_may_be_left_out(new):
     paged.attention(bt.q, bt.k, bt.v, bt.tables, bt.lens, cu_q=cu, out=out)
     want, spread = exact_attention(bt, 0.125, 0, 0)
     assert ((out.double() - want).abs() <= 2.0 ** -11 * (want.abs() + spread) + 1e-5 * float(bt.v.abs().max())).all()
+
+
+def test_append_with_a_q_of_no_heads():
+    """k and v are stored whatever q holds."""
+    bt = Batch([40, 7], [1, 1], 4, 2, 64, 16, torch.float16, seed=113)
+    kn, vn = (torch.randn(2, 2, 64, device=DEV).half() for _ in range(2))
+    k, v = bt.k.clone(), bt.v.clone()
+    paged.append_kv(k, v, kn, vn, bt.tables, bt.lens)
+    got = paged.append_kv(bt.k, bt.v, kn, vn, bt.tables, bt.lens, q=torch.empty(2, 0, 64, dtype=torch.float16, device=DEV))
+    assert got.shape == (2, 0, 64)
+    assert torch.equal(bt.k, k) and torch.equal(bt.v, v)
