@@ -111,7 +111,7 @@ def attention_forward(layernorm: torch.Tensor, norm_epsilon: float, q_proj: int,
 
 def _ids(x: PageIds) -> torch.Tensor:
     if not isinstance(x, torch.Tensor):
-        x = torch.tensor(x, dtype=torch.int64)
+        x = torch.as_tensor(x) if len(x) else torch.empty(0, dtype=torch.int64)
     if x.is_floating_point() or x.is_complex() or x.dtype == torch.bool:
         raise RuntimeError("page ids must be whole numbers")
     if x.is_cuda:

@@ -9,9 +9,11 @@ import math
 import random
 import time
 
+import numpy
 import pytest
+import torch
 
-from drofell_for_revision_b200 import _capi
+from drofell_for_revision_b200 import _capi, paged
 from test_paged_cpu import FAKE, INVALID, append, attention, copy, pages, rows, seqs
 
 
@@ -157,3 +159,17 @@ def test_copies_against_sets(num):
         assert want in message()
         seen.add(want)
     assert len(seen) == 3
+
+
+def test_ids_that_are_not_whole_are_refused():
+    """Whatever holds them: none is rounded."""
+    k = torch.zeros(3, 6, 2, 16, 64, dtype=torch.float16)
+    for bad in ((1.5,), numpy.array([1.5]), (1.0,), numpy.array([2.0], dtype=numpy.float32)):
+        for pair in ((bad, [2]), ([2], bad), ((2,), bad)):
+            with pytest.raises(RuntimeError, match="whole numbers"):
+                paged.copy_pages(k, k.clone(), *pair)
+    for good in ((1,), range(1, 2), numpy.array([1]), numpy.array([1], dtype=numpy.uint8), torch.tensor([1])):
+        with pytest.raises(RuntimeError, match="CUDA tensor"):
+            paged.copy_pages(k, k.clone(), good, (2,))
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        paged.copy_pages(k, k.clone(), (), [])
