@@ -90,6 +90,9 @@ def attention_forward(layernorm: torch.Tensor, norm_epsilon: float, q_proj: int,
     q, k, v projections (``attention_forward_qkv_stage_v2``), k and v into the pages, attention
     over them, the o projection. x [rows, hidden] fp16, one row per new token; the projections
     are q4 handles (``q4_matrix.cuda_q4``). Returns [rows, hidden] without the residual."""
+    for t, name in ((x, "x"), (layernorm, "layernorm")):
+        if torch.is_grad_enabled() and t.requires_grad:
+            raise RuntimeError(f"{name} requires a gradient: the paged cache is for serving and has none (use torch.no_grad())")
     hq, hk, hv, ho = (exllama._handle(h) for h in (q_proj, k_proj, v_proj, o_proj))
     if x.dim() != 2 or x.shape[1] != hq.K:
         raise RuntimeError(f"x must be [rows, {hq.K}]")

@@ -1,5 +1,5 @@
-"""Memory that two operands of the paged cache share is refused before any CUDA call, and only
-that: against a search through all elements.
+"""Refusals of the paged cache before any CUDA call. Memory that two operands share is refused, and
+only that: against a search through all elements.
 
 A call that passes its checks would go on to the GPU: the cases that have to be accepted end in
 a later refusal, or are asked of the search alone."""
@@ -173,3 +173,19 @@ def test_ids_that_are_not_whole_are_refused():
             paged.copy_pages(k, k.clone(), good, (2,))
     with pytest.raises(RuntimeError, match="CUDA tensor"):
         paged.copy_pages(k, k.clone(), (), [])
+
+
+@pytest.mark.parametrize("which", ["x", "layernorm"])
+def test_the_block_refuses_gradients(which):
+    """Its result would carry none, whatever was asked."""
+    a = dict(x=torch.zeros(1, 8, dtype=torch.float16), layernorm=torch.ones(8, dtype=torch.float16))
+    a[which].requires_grad_()
+    k = torch.zeros(2, 1, 8, 8, dtype=torch.float16)
+    tables, lens = torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+
+    def call():
+        paged.attention_forward(a["layernorm"], 1e-6, 12345, 12345, 12345, 12345, a["x"], k, k.clone(), tables, lens)
+    with pytest.raises(RuntimeError, match=f"{which} requires a gradient"):
+        call()
+    with torch.no_grad(), pytest.raises(RuntimeError, match="unknown or released"):
+        call()
