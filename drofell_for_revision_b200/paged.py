@@ -62,8 +62,14 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tab
     (positive) 1 / sqrt(head dim) unless given. ``max_q`` is at least the most new tokens of a
     sequence: rows beyond it get no result. Left out, it is the number of rows (1 without
     ``cu_q``); given, it lets the call choose its kernel and cut its work by what is there. Rows
-    that see nothing are 0; rows of no sequence are left as they were (undefined in an output
-    that this call makes). ``out`` must not overlap q or hold an element twice."""
+    that see nothing are 0 (also where every score is -inf); rows of no sequence are left as they
+    were (undefined in an output that this call makes). ``out`` must not overlap q or hold an
+    element twice.
+
+    Scores, softmax statistics and sums are fp32. The weights enter the value product in two
+    16-bit parts where a sequence has few new rows, and rounded once to the inputs' type where it
+    has more (over 32 of new tokens x heads of a key-value head, over 16 on tables of 1024 tokens and
+    more): there the error is up to 1.45 times that of an fp32 product."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     if max_q is None:

@@ -288,8 +288,11 @@ W4A16_API int w4a16_append_kv(const w4a16_pages* pages, const w4a16_seqs* seqs, 
 /* out = softmax(scale q k^T) v (scale > 0) of every new token over the visible tokens of its sequence:
  * not after it, and with window > 0 the last `window` ones (itself counted) and the first
  * `sinks` ones. heads is a multiple of heads_kv; query head i reads key-value head
- * i / (heads / heads_kv); out must not overlap q or itself. Rows that see nothing are 0.
- * Softmax statistics and sums in fp32. No host synchronisation and no allocation: capturable.
+ * i / (heads / heads_kv); out must not overlap q or itself. Rows that see nothing are 0,
+ * also where every score is -inf. Scores, softmax statistics and sums in fp32; the weights
+ * enter the value product in two 16-bit parts, or, from 33 rows (new tokens x heads of a
+ * key-value head; 17 on tables of 1024 tokens and more) of max_q on, rounded once to the
+ * inputs' type. No host synchronisation and no allocation: capturable.
  * Calls that may overlap on the GPU need workspaces of their own; a workspace is 32-byte
  * aligned, its contents mean nothing before and after a call. */
 W4A16_API int w4a16_paged_attention(const w4a16_pages* pages, const w4a16_seqs* seqs, const w4a16_rows* q,

@@ -1,4 +1,5 @@
-"""The paged cache where scores and values are extreme: weights far below the largest, infinities and NaN.
+"""The paged cache where scores and values are extreme: weights far below the largest, maxima that rise along
+the keys, infinities and NaN, empty slots of a padded batch.
 
 Tolerances. As in test_gpu_paged.py an output is off by at most half a step of its own and half a
 step of the weights, (eps / 2) (|out| + sum p |v|) together. What comes on top is counted here:
@@ -276,3 +277,89 @@ def test_append_with_a_q_of_no_heads():
     got = paged.append_kv(bt.k, bt.v, kn, vn, bt.tables, bt.lens, q=torch.empty(2, 0, 64, dtype=torch.float16, device=DEV))
     assert got.shape == (2, 0, 64)
     assert torch.equal(bt.k, k) and torch.equal(bt.v, v)
+
+
+# ---------------------------------------------------------------- scores that are not finite
+def by_selection(bt, scale, window=0):
+    """The rule in 64 bits, rows by heads: 'nan' where a visible score is NaN or +inf (softmax of an
+    infinity), 0 where every visible one is -inf, else the result without the keys at -inf."""
+    heads, hkv = bt.q.shape[1], bt.k.shape[1]
+    out = torch.zeros(bt.q.shape, dtype=torch.float64, device=DEV)
+    spread = torch.zeros_like(out)
+    for b, (n, m) in enumerate(zip(bt.lens_l, bt.new_l)):
+        k, v = bt.keys(b, bt.k), bt.keys(b, bt.v)
+        rows = slice(bt.cu_l[b], bt.cu_l[b] + m)
+        p = torch.arange(n - m, n, device=DEV)[:, None]
+        j = torch.arange(n, device=DEV)[None]
+        seen = (j <= p) & ((p - j < window) if window else True)
+        for h in range(heads):
+            q = bt.q[rows, h].double()
+            prod = q[:, None] * k[h * hkv // heads][None]
+            s = prod.sum(-1) * scale
+            s = torch.where(seen, s, -math.inf)
+            bad = (torch.isnan(s) | (s == math.inf)).any(-1)
+            top = s.nan_to_num(0.0, 0.0, -math.inf).amax(-1, keepdim=True)
+            w = torch.exp(torch.where(s == -math.inf, -math.inf, s.nan_to_num(0.0, 0.0)) - top.nan_to_num(0.0, 0.0, 0.0))
+            w = w / w.sum(-1, keepdim=True).clamp_min(1e-300)
+            vv = v[h * hkv // heads]
+            out[rows, h] = torch.where(bad[:, None], math.nan, w @ vv)
+            spread[rows, h] = w @ vv.abs()
+    return out, spread
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("what", ["k", "every k", "q", "q to -inf"])
+@pytest.mark.parametrize("n,new", [(40, 1), (1500, 1), (90, 6), (200, 150), (1500, 140)])
+def test_scores_that_are_not_finite(dtype, value, what, n, new):
+    bt = Batch([n, 30], [new, 1], 4, 2, 128, 16, dtype, seed=83)
+    if what == "k":  # one key, one dimension: +inf for queries of one sign, -inf for the others
+        j = n // 2
+        bt.k[int(bt.tables[0, j // 16]), 0, j % 16, 7] = value
+    elif what == "every k":
+        bt.k[bt.tables[0].long().clamp_min(0), 1, :, 7] = value
+    elif what == "q":
+        bt.q[0, 1, 7] = value
+    else:  # every score of the row -inf
+        bt.k[..., 7] = -bt.k[..., 7].abs() - 0.5
+        bt.q[0, 1, 7] = value
+    want, spread = by_selection(bt, 1 / math.sqrt(128))
+    got = attend(bt, 1 / math.sqrt(128))
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    half = torch.finfo(dtype).eps / 2
+    ok = ~torch.isnan(want)
+    room = half * (want.abs() + spread) + (n / 16 + 400) * 2.0 ** -23 * spread + n * 2.0 ** -32 * float(bt.v.abs().max())
+    assert ((got.double() - want).abs() <= room + 2.0 ** -25)[ok].all()
+    if what == "q to -inf" and value == math.inf:
+        assert (got[0, 1] == 0).all()
+
+
+# ---------------------------------------------------------------- maxima that rise along the keys
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,hkv,dim", [(4, 4, 128), (8, 1, 64), (6, 2, 128)])
+@pytest.mark.parametrize("n,new,window,sinks", [(2600, 260, 0, 0), (700, 700, 0, 0), (2600, 1, 0, 0), (2600, 5, 0, 0),
+                                                (2600, 300, 500, 4), (5000, 40, 0, 0)])
+def test_maxima_that_rise(dtype, heads, hkv, dim, n, new, window, sinks):
+    """Each tile of 128 keys raises the maximum of a row by its own factor: not at all, by just less
+    and just more than what is tolerated without rescaling (2^8), by far more, or it falls. Rows
+    of all kinds lie side by side in a warp; under the window the first tiles show some of them
+    nothing."""
+    bt = Batch([n], [new], heads, hkv, dim, 64, dtype, seed=89)
+    bt.q.mul_(0.02)
+    bt.k.mul_(0.5)
+    factors = torch.tensor([0.0, 7.875, 8.125, 20.0, -3.0, 0.5, 16.0], device=DEV)
+    rows = torch.arange(new * heads, device=DEV).view(new, heads)
+    bt.q[..., 0] = factors[rows % 7].to(dtype)
+    used = -(-n // 64)
+    for i in range(used):
+        bt.k[int(bt.tables[0, i]), :, :, 0] = float(i // 2 % 16)  # and starts again behind 2048 keys
+    check(bt, math.log(2), n, score_error=2.0 ** -13, window=window, sinks=sinks)
+
+
+# ---------------------------------------------------------------- long contexts of ordinary data
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens,new", [([60001, 5], [1, 1]), ([20000], [4]), ([40000], [150]), ([9000, 9000, 100], [200, 1, 100])])
+def test_long_contexts_without_an_absolute_term(dtype, lens, new):
+    """Outputs of a long context are small: a bound in terms of sum p |v| and the type alone."""
+    bt = Batch(lens, new, 8, 2, 128, 64, dtype, seed=127)
+    check(bt, 1 / math.sqrt(128), max(lens))
