@@ -1,8 +1,9 @@
 // Filling a paged key-value cache (rotary embedding fused) and copying its pages. Both move
 // every byte once, 16 bytes a thread, and are bound by HBM (small calls by launch latency).
-// Measured: 5 prompts, 5020 tokens of 64 + 8 + 8 heads of 128: 17.5 us, 6.0 TB/s; 8 single
-// tokens of 32 + 32 + 32 heads: 2.2 us; copies of 8 pages of 32 layers (134 MB moved): 22.3 us,
-// 6.0 TB/s; of 511 pages of 16 layers (4.3 GB): 650 us, 6.6 TB/s.
+// Measured, the fills in a graph of calls (from Python: 19.3 and 5.6 us): 5 prompts, 5020 tokens of
+// 64 + 8 + 8 heads of 128: 17.5 us, 6.0 TB/s; 8 single tokens of 32 + 32 + 32 heads: 2.2 us. Copies,
+// from Python: 8 pages of 32 layers (134 MB moved) 22.3 us, 6.0 TB/s; 511 pages of 16 layers (4.3 GB)
+// 650 us, 6.6 TB/s.
 #include <algorithm>
 
 #include "w4a16_paged.cuh"
@@ -176,14 +177,16 @@ cudaError_t launch_pdl(K kern, dim3 grid, int threads, const A& a, cudaStream_t 
 
 }  // namespace
 
-cudaError_t launch_append(const AppendArgs& a, bool bf16, cudaStream_t s) {
+cudaError_t launch_append(const AppendArgs& a, bool bf16, int num_sms, cudaStream_t s) {
     if (a.seqs.tokens == 0) return cudaSuccess;
     const int half = a.rope && !a.interleaved ? a.rope_dim >> 4 : 0;
     const int rows = kAppendThreads / ((a.pages.dim >> 3) - half);
     const int all = (a.q ? a.heads : 0) + 2 * a.pages.heads_kv;
     // few tokens: one head per thread row, so that a decode step is one round trip; many:
-    // the heads of a token in one CTA, so that the angles are read once
-    const int ny = a.seqs.tokens >= 296 ? 1 : (all + rows - 1) / rows;
+    // the heads of a token in one CTA, so that the angles are read once. In a graph, us, one head
+    // against all: 8 tokens of 32 + 32 + 32 heads 2.2 / 3.5, 148 2.9 / 3.7, 296 4.7 / 4.9, 444 6.0 / 6.1,
+    // 592 7.8 / 7.1, 2368 25.7 / 20.0; of 64 + 8 + 8 heads 148 2.8 / 3.5, 296 4.1 / 3.8, 592 6.7 / 5.6
+    const int ny = a.seqs.tokens >= 2 * num_sms ? 1 : (all + rows - 1) / rows;
     const dim3 grid(a.seqs.tokens, ny);
     return launch_pdl(bf16 ? append_kernel<true> : append_kernel<false>, grid, kAppendThreads, a, s);
 }

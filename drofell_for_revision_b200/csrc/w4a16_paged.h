@@ -52,7 +52,7 @@ struct AttnArgs {
     float* ws;          // partial results of the split kernel
 };
 
-cudaError_t launch_append(const AppendArgs& a, bool bf16, cudaStream_t s);
+cudaError_t launch_append(const AppendArgs& a, bool bf16, int num_sms, cudaStream_t s);
 
 // Attention split over the cache's length and joined.
 struct SplitPlan {

@@ -296,7 +296,9 @@ int w4a16_append_kv(const w4a16_pages* pages, const w4a16_seqs* seqs, const w4a1
     a.seqs.max_q = INT_MAX;
     DeviceGuard guard(pages->device);
     if (!guard.ok) return report_error(W4A16_ERR_INVALID, "device %d", pages->device);
-    const cudaError_t e = launch_append(a, pages->dtype == W4A16_DTYPE_BF16, static_cast<cudaStream_t>(stream));
+    const int sms = sm_count(pages->device);
+    if (sms == 0) return report_error(W4A16_ERR_CUDA, "no device %d", pages->device);
+    const cudaError_t e = launch_append(a, pages->dtype == W4A16_DTYPE_BF16, sms, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? W4A16_OK : cuda_error(e, "append_kv launch");
 }
 
