@@ -26,14 +26,16 @@
 // each: while one is in its softmax, the tensor cores work for the other. One warp for both
 // left them idle a third of the time: its waits, slowed to some 300 cycles each by the
 // exponentials that share the queue to the shared-memory and special-function units, added up.
+// Rows whose sums come out not finite are marked and settled by the softmax warps behind the CTA's
+// last item.
 //
 // What bounds it: the tensor cores and, between them, the chain scores - softmax - product of
 // each row tile, at the clock that the power cap leaves. The MMAs of a step (both row tiles,
 // 128 keys, 128 dimensions) take 2896 cycles by themselves: 16 of M = N = 128 with both
 // operands in shared memory at 107, 16 with P in TMEM at 74. A step takes 3260 of them in a
 // long prompt, and 7 thousand go to an item's beginning and end. One prompt of 8192 tokens, 32
-// heads, bf16: 474 us while the clock is at 1.8 GHz (1160 TFLOP/s over the visible pairs), 575
-// to 590 us (930 to 957) under load for long, at 1.5 GHz.
+// heads, bf16: 474 us while the clock is at 1.8 GHz (1160 TFLOP/s over the visible pairs), 574
+// to 592 us (928 to 957) under load for long, at 1.5 GHz.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>

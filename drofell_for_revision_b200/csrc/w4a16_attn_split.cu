@@ -18,8 +18,8 @@
 // adds them in range order (the same result for the same lengths, whatever runs when).
 //
 // Measured (keys and values of 128 dimensions): two sequences of 130001 tokens, 64 heads on 8:
-// 171 to 186 us, 5.7 to 6.2 TB/s; 48 uneven ones of up to 8191: 53 us, 5.0 TB/s; 24 under a
-// window of 1024, 40 heads: 49 us, 5.0 TB/s; one sequence of 777 tokens, 32 heads: 10 us. What
+// 169 to 190 us by box, 5.6 to 6.3 TB/s; 48 uneven ones of up to 8191: 53 to 54 us, 5.0 TB/s; 24
+// under a window of 1024, 40 heads: 47 to 50 us, 5.0 TB/s; one sequence of 777 tokens, 32 heads: 10 us. What
 // is left there: some 4 us until the first keys arrive (length, place, page id, key: four
 // reads that wait for one another) and 4 us for the join's launch and its two reads.
 #include <algorithm>
