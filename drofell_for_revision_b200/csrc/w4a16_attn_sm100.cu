@@ -1031,7 +1031,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) prompt_join_kernel(const __gr
 #pragma unroll 4
         for (int c = 0; c < pieces; ++c) {
             const float* s = part_slot<DP>(a, first + c);
-            const float f = exp2_approx(s[r] - base);
+            const float f = exp2_approx(s[r] - base + kJoinBias);
             l += f * s[2 * kTileRows + r];
             float v[E];
 #pragma unroll

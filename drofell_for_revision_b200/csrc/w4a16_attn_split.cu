@@ -533,7 +533,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) split_join_kernel(const __gri
 #pragma unroll
                 for (int d = kJoinPieces / 2; d; d >>= 1) m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, d));
                 const float base = m2 == -INFINITY ? 0.f : m2;
-                const float old = m == -INFINITY ? 0.f : exp2_approx(m - base), f = exp2_approx(mc - base);
+                const float old = m == -INFINITY ? 0.f : exp2_approx(m - base), f = exp2_approx(mc - base + kJoinBias);
                 m = m2;
                 float sum = lc * f;
 #pragma unroll

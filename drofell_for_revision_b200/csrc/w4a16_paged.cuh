@@ -116,6 +116,14 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
     }
 }
 
+// The same for rows that are computed anew: bf16 has fp32's range, so that a sum of values may pass
+// it where their mean does not. Such a sum comes out not finite and is made anew with weights of
+// 2^-24 (fewer than 2^24 keys of equal weight, then); a part's maximum is stored as much higher.
+template <bool BF16, int TILE>
+constexpr float kAnewBias = BF16 ? -24.f : kWeightBias<BF16, TILE>;
+// And for the join of parts, each finite: at most 2^12 of them.
+constexpr float kJoinBias = -12.f;
+
 // f v of a piece's sum v under a factor f of at most 1 that may have run out to 0. No weight is
 // 0, so an infinity or NaN among the values stays one, however small its piece's share.
 __device__ __forceinline__ float share_of(float f, float v) {
@@ -165,7 +173,7 @@ __device__ __noinline__ void row_by_keys(const AttnArgs& a, int b, int h, int t0
             for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
             s *= a.scale_log2;
             const float m = fmaxf(r.m, s), base = m == -INFINITY ? 0.f : m;
-            const float f = r.m == m ? 1.f : exp2_approx(r.m - base), w = exp2_approx(s - base + kWeightBias<BF16, TILE>);
+            const float f = r.m == m ? 1.f : exp2_approx(r.m - base), w = exp2_approx(s - base + kAnewBias<BF16, TILE>);
             r.m = m;
             r.l = r.l * f + w;
 #pragma unroll
@@ -173,7 +181,7 @@ __device__ __noinline__ void row_by_keys(const AttnArgs& a, int b, int h, int t0
         }
     }
     if (part && (threadIdx.x & 31) == 0) {
-        part[part_row] = r.m;
+        part[part_row] = r.m + (kWeightBias<BF16, TILE> - kAnewBias<BF16, TILE>);
         part[part_rows + part_row] = r.l;
     }
     const float inv = part ? 1.f : r.l == 0.f ? 0.f : 1.f / r.l;
@@ -276,7 +284,7 @@ __device__ __noinline__ void rows_by_tiles(const AttnArgs& a, int b, int h, int 
                     o[n][2 * r] *= f;
                     o[n][2 * r + 1] *= f;
                 }
-                const float base = (x == -INFINITY ? 0.f : x) - kWeightBias<BF16, 128>;
+                const float base = (x == -INFINITY ? 0.f : x) - kAnewBias<BF16, 128>;
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
                     const float y = exp2_approx(s[n][2 * r] * a.scale_log2 - base);
@@ -310,7 +318,7 @@ __device__ __noinline__ void rows_by_tiles(const AttnArgs& a, int b, int h, int 
             const int row = row0 + g + 8 * r, token = row / a.group, at = part_row + g + 8 * r;
             uint16_t* out = a.out + static_cast<int64_t>(t0 + token) * a.o_token + (h * a.group + row - token * a.group) * a.o_head;
             if (part && tq == 0) {
-                part[at] = m[r];
+                part[at] = m[r] + (kWeightBias<BF16, 128> - kAnewBias<BF16, 128>);
                 part[part_rows + at] = l[r];
             }
             const float inv = part ? 1.f : l[r] == 0.f ? 0.f : 1.f / l[r];

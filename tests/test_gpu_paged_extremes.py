@@ -363,3 +363,23 @@ def test_long_contexts_without_an_absolute_term(dtype, lens, new):
     """Outputs of a long context are small: a bound in terms of sum p |v| and the type alone."""
     bt = Batch(lens, new, 8, 2, 128, 64, dtype, seed=127)
     check(bt, 1 / math.sqrt(128), max(lens))
+
+
+# ---------------------------------------------------------------- values near the type's end
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens,new", [([900], [1]), ([50000], [1]), ([700, 20], [4, 2]), ([6000], [200]), ([400, 30], [400, 30]),
+                                      ([900] * 80, [64] * 80), ([500] * 200, [1] * 200)])
+def test_values_near_the_types_end(dtype, lens, new):
+    """A mean of values is no larger than they are, though the sum that it is made of may pass fp32's
+    range (bf16 has fp32's exponents)."""
+    bt = Batch(lens, new, 8, 4, 64, 16, dtype, seed=131)
+    g = torch.Generator(device=DEV).manual_seed(131)
+    top = float(torch.finfo(dtype).max)
+    bt.v.copy_((top * (0.5 + 0.4 * torch.rand(bt.v.shape, device=DEV, generator=g))).to(dtype))
+    bt.v[..., 3] *= -1
+    want, spread = exact_attention(bt, 0.125, 0, 0)
+    got = attend(bt, 0.125)
+    room = torch.finfo(dtype).eps / 2 * (want.abs() + spread) + (max(lens) / 16 + 400) * 2.0 ** -23 * spread
+    if dtype == torch.float16:
+        room = room + max(lens) * 2.0 ** -32 * top
+    assert torch.isfinite(got).all() and ((got.double() - want).abs() <= room).all()
