@@ -175,6 +175,11 @@ __device__ __forceinline__ float2 exp2_fma(float2 x) {
     return make_float2(__int_as_float(__float_as_int(a.x) + (__float_as_int(b.x) << 23)),
                        __int_as_float(__float_as_int(a.y) + (__float_as_int(b.y) << 23)));
 }
+// Weights are 2^(sc s - base) in one fused operation, base rounded: a factor that the row's weights share,
+// but for maxima far beyond what data gives rise to it would take them out of their range. Rows
+// that had such a maximum (2^22 in base 2: a factor of 2^(1/4)) are computed anew.
+constexpr float kLargeBase = 4194304.f;
+
 // What is taken from a row's scaled scores: its maximum so far, and the weights' factor.
 template <bool BF16>
 __device__ __forceinline__ float base_of(float m, float sc) {
@@ -398,19 +403,24 @@ constexpr uint32_t kExponent = BF16 ? 0x7f80u : 0x7c00u;
 template <bool BF16>
 constexpr uint32_t kMark = kExponent<BF16> | 1u;
 
-// Marks the rows of a warp whose bit is set, a lane a row; `l` is the sum of weights if it is a part's.
-// Of item k, which is noted in *items.
+// Marks the rows of a warp whose bit is set, a lane a row: all of it if it is to be computed anew. A
+// row of a part lies at `o`, its sum of weights at `l`. Of item k, which is noted in *items.
 template <bool BF16>
-__device__ __noinline__ void mark_rows(uint32_t rows, uint16_t* row, int dim, float* l, volatile uint32_t* items, int k) {
+__device__ __noinline__ void mark_rows(uint32_t rows, bool all, uint16_t* row, int dim, float* l, float* o,
+                                       volatile uint32_t* items, int k) {
     const int lane = threadIdx.x & 31;
     const bool mine = (rows >> lane) & 1u;
     if (lane == 0) *items |= 1u << (k & 31);
-    if (mine && l) *l = -*l;
+    if (mine && l) *l = all ? -1.f : -*l;
 #pragma unroll 1
-    for (int d = 0; mine && !l && d < dim; d += 2) {
+    for (int d = 0; mine && d < dim; d += 2) {
+        if (l) {
+            if (all) o[d] = o[d + 1] = NAN;
+            continue;
+        }
         uint32_t x = *reinterpret_cast<uint32_t*>(row + d);
-        if ((x & kExponent<BF16>) == kExponent<BF16>) x = (x & 0xffff0000u) | kMark<BF16>;
-        if (((x >> 16) & kExponent<BF16>) == kExponent<BF16>) x = (x & 0xffffu) | (kMark<BF16> << 16);
+        if (all || (x & kExponent<BF16>) == kExponent<BF16>) x = (x & 0xffff0000u) | kMark<BF16>;
+        if (all || ((x >> 16) & kExponent<BF16>) == kExponent<BF16>) x = (x & 0xffffu) | (kMark<BF16> << 16);
         *reinterpret_cast<uint32_t*>(row + d) = x;
     }
     __syncwarp();
@@ -847,7 +857,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool live_row = row < it.rows;
             const int p = live_row ? max(-1, it.p0 + row / a.group) : -1;
             float m = -INFINITY, l = 0.f;  // m in units of the unscaled score
-            bool first = true;
+            bool first = true, large = false;
 #pragma unroll 1
             for (int j = it.j0; j < it.j1; ++j, ++i) {
                 const int k0 = vw.kt.first(j);
@@ -897,6 +907,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (__builtin_expect(first, 0)) {
                         ptx::tmem_ld_wait();
                         m = fmaxf(top, largest(s + 64));
+                        large = fabsf(base_of<BF16>(m, sc)) > kLargeBase;
                     }
                     part = weights<BF16>(s, sc, base_of<BF16>(m, sc));
                     if (first) break;
@@ -906,6 +917,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (__builtin_expect(!__any_sync(0xffffffffu, grow), 1)) break;
                     const float f = grow ? exp2_approx((m - top) * sc) : 1.f;
                     if (grow) m = top;
+                    large |= fabsf(base_of<BF16>(m, sc)) > kLargeBase;
                     l *= f;
 #pragma unroll 1
                     for (int c = 0; c < DP; c += 32) {
@@ -987,9 +999,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             // rows whose sums are not finite while their sums of weights are
             // rows whose sums are not finite while their sums of weights are
-            const uint32_t rows = __ballot_sync(0xffffffffu, odd && live_row && l == l);
+            const uint32_t rows = __ballot_sync(0xffffffffu, live_row && ((odd && l == l) || large));
             if (rows)
-                mark_rows<BF16>(rows, a.out + o_off, a.pages.dim, part ? slot + 2 * kTileRows + pr : nullptr, to_settle + warp, k);
+                mark_rows<BF16>(rows, large, a.out + o_off, a.pages.dim, part ? slot + 2 * kTileRows + pr : nullptr,
+                                slot + 4 * kTileRows + pr * DP, to_settle + warp, k);
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");  // the softmax warps alone
         uint32_t items = 0;

@@ -356,8 +356,8 @@ __global__ void __launch_bounds__(kThreads, DEEP ? 1 : 2) split_kernel(const __g
                             if (!in || !visible(key, p1, a.window, a.sinks)) s[j][2 + e] = -INFINITY;
                         }
                 }
-                float x0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])) * a.scale_log2;
-                float x1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3])) * a.scale_log2;
+                float x0 = __fmul_rn(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])), a.scale_log2);
+                float x1 = __fmul_rn(fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3])), a.scale_log2);
                 x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
                 x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
                 x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
@@ -377,14 +377,13 @@ __global__ void __launch_bounds__(kThreads, DEEP ? 1 : 2) split_kernel(const __g
                     m0 = n0;
                     m1 = n1;
                 }
-                const float c0 = (m0 == -INFINITY ? 0.f : m0) - kWeightBias<BF16, kTile>;
-                const float c1 = (m1 == -INFINITY ? 0.f : m1) - kWeightBias<BF16, kTile>;
+                const float c0 = m0 == -INFINITY ? 0.f : m0, c1 = m1 == -INFINITY ? 0.f : m1;
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        s[j][e] = exp2_approx(s[j][e] * a.scale_log2 - c0);
-                        s[j][2 + e] = exp2_approx(s[j][2 + e] * a.scale_log2 - c1);
+                        s[j][e] = weight_of(s[j][e], a.scale_log2, c0, kWeightBias<BF16, kTile>);
+                        s[j][2 + e] = weight_of(s[j][2 + e], a.scale_log2, c1, kWeightBias<BF16, kTile>);
                         l0 += s[j][e];
                         l1 += s[j][2 + e];
                     }

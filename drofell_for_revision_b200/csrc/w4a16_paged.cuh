@@ -124,6 +124,12 @@ constexpr float kAnewBias = BF16 ? -24.f : kWeightBias<BF16, TILE>;
 // And for the join of parts, each finite: at most 2^12 of them.
 constexpr float kJoinBias = -12.f;
 
+// 2^(scale s - top + bias), top the rounded product of the largest s. Every product is rounded alike
+// and none is fused: the largest weight is 2^bias exactly, however large the scores are.
+__device__ __forceinline__ float weight_of(float s, float scale, float top, float bias) {
+    return exp2_approx((__fmul_rn(s, scale) - top) + bias);
+}
+
 // f v of a piece's sum v under a factor f of at most 1 that may have run out to 0. No weight is
 // 0, so an infinity or NaN among the values stays one, however small its piece's share.
 __device__ __forceinline__ float share_of(float f, float v) {
@@ -171,9 +177,9 @@ __device__ __noinline__ void row_by_keys(const AttnArgs& a, int b, int h, int t0
             float s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
 #pragma unroll
             for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-            s *= a.scale_log2;
-            const float m = fmaxf(r.m, s), base = m == -INFINITY ? 0.f : m;
-            const float f = r.m == m ? 1.f : exp2_approx(r.m - base), w = exp2_approx(s - base + kAnewBias<BF16, TILE>);
+            const float m = fmaxf(r.m, __fmul_rn(s, a.scale_log2)), base = m == -INFINITY ? 0.f : m;
+            const float f = r.m == m ? 1.f : exp2_approx(r.m - base);
+            const float w = weight_of(s, a.scale_log2, base, kAnewBias<BF16, TILE>);
             r.m = m;
             r.l = r.l * f + w;
 #pragma unroll
@@ -272,7 +278,7 @@ __device__ __noinline__ void rows_by_tiles(const AttnArgs& a, int b, int h, int 
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                float x = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1])) * a.scale_log2;
+                float x = __fmul_rn(fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1])), a.scale_log2);
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
                 x = fmaxf(x, m[r]);
@@ -284,11 +290,11 @@ __device__ __noinline__ void rows_by_tiles(const AttnArgs& a, int b, int h, int 
                     o[n][2 * r] *= f;
                     o[n][2 * r + 1] *= f;
                 }
-                const float base = (x == -INFINITY ? 0.f : x) - kAnewBias<BF16, 128>;
+                const float base = x == -INFINITY ? 0.f : x;
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
-                    const float y = exp2_approx(s[n][2 * r] * a.scale_log2 - base);
-                    const float w = exp2_approx(s[n][2 * r + 1] * a.scale_log2 - base);
+                    const float y = weight_of(s[n][2 * r], a.scale_log2, base, kAnewBias<BF16, 128>);
+                    const float w = weight_of(s[n][2 * r + 1], a.scale_log2, base, kAnewBias<BF16, 128>);
                     l[r] += y + w;
                     hi[2 * n + r] = pack2<BF16>(y, w);
                     const float2 z = unpack2<BF16>(hi[2 * n + r]);

@@ -383,3 +383,26 @@ def test_values_near_the_types_end(dtype, lens, new):
     if dtype == torch.float16:
         room = room + max(lens) * 2.0 ** -32 * top
     assert torch.isfinite(got).all() and ((got.double() - want).abs() <= room).all()
+
+
+# ---------------------------------------------------------------- scores of any size
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens,new", [([900], [1]), ([1000], [4]), ([1000], [30]), ([900], [200]), ([1000], [1000]),
+                                      ([700] * 120, [20] * 120)])
+def test_scores_of_any_size(dtype, lens, new):
+    """Scores from 1 to 2^30 in size, the largest of them far above or far below 0: where they are that
+    large one key takes all the weight, and no rounding of a maximum may reach the weights."""
+    bt = Batch(lens, new, 8, 4, 64, 16, dtype, seed=137)
+    n = max(lens)
+    g = torch.Generator().manual_seed(137)
+    steps = 128 if dtype == torch.bfloat16 else 1024  # numbers between 2^15 and 2^16
+    rows = torch.arange(bt.q.shape[0] * 8).view(-1, 8)
+    bt.q.zero_()
+    bt.q[..., 0] = ((2.0 ** (rows % 15)) * (1 - 2 * (rows % 2))).to(dtype).to(DEV)
+    for b, length in enumerate(lens):
+        k = 2.0 ** 15 * (1 + torch.randperm(n, generator=g)[:length] % steps / steps)
+        k = (k * (1 - 2 * (torch.arange(length) // 300 % 2)) if b % 3 == 0 else k if b % 3 == 1 else -k).to(dtype).to(DEV)
+        at = torch.arange(length, device=DEV)
+        bt.k[bt.tables[b].long()[at // 16], :, at % 16, 0] = k[:, None]
+    bt.k[..., 1:] = 0
+    check(bt, 1.0, n)
